@@ -31,7 +31,7 @@ typedef struct it_host_step it_host_step; /* buffers and streams of it_host_step
 typedef int32_t it_status;
 enum {
   IT_OK = 0,
-  IT_ERR_INVALID_ARG = -1,       /* null pointer, negative size, undersized workspace */
+  IT_ERR_INVALID_ARG = -1,       /* null pointer, negative size, undersized workspace; on the device, a length outside a cache */
   IT_ERR_UNSUPPORTED_SHAPE = -2, /* head_dim outside 1..128 (assert at src/ops/flash_attention.rs:98) */
   IT_ERR_PRECISION = -3,         /* dtype not handled (asserts at src/ops/flash_attention.rs:78-80) */
   IT_ERR_ALIGNMENT = -4,         /* a tensor pointer is not 16-byte aligned */
@@ -260,6 +260,63 @@ it_status it_attention_packed_bwd(it_ctx* ctx, it_stream* stream, it_dtype dtype
                                   int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t causal, float rope_base,
                                   int32_t position_offset, const void* qkv, const void* o, const void* d_o,
                                   const float* lse, void* dqkv, void* workspace, size_t workspace_bytes);
+
+/* ---- serving from quantised weights and a quantised key/value cache -----------------------------------------------------
+ * (No counterpart in the reference, which lists the cache and inference in fewer bits as future work: docs/PRESENTATION.md:576.)
+ * Sequences of a batch may stand at different lengths: `lengths`, `positions`, `starts` and `counts` are DEVICE arrays of
+ * 32-bit integers, read when the kernel runs, so that a captured graph of a generation step can be replayed as they grow. */
+
+/* Rotary embedding at positions given per token: q [batch, seq, heads, head_dim], k [batch, seq, kv_heads, head_dim] (kv_heads 0:
+ * none), positions [axes, batch, seq].  Dimension pair i (columns 2i, 2i + 1) turns by positions[axis(i)][token] * f(i), an angle
+ * in 64 bits.  sections[a], a < axes (1 to 4), pairs belong to axis a, in order; they add up to head_dim / 2.  per_axis 0: f(i) =
+ * base^(-2i / head_dim), one ladder over all pairs (text and video tokens of one model).  per_axis 1: the j-th of an axis's n
+ * pairs has f = base^(-j / n), a ladder per axis (images).  inverse != 0 turns back: the gradient.  In place is allowed. */
+it_status it_rope_positions(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t batch, int32_t seq, int32_t heads,
+                            int32_t kv_heads, int32_t head_dim, float rope_base, int32_t axes, const int32_t* sections,
+                            int32_t per_axis, int32_t inverse, const int32_t* positions, const void* q_in, const void* k_in,
+                            void* q_out, void* k_out);
+
+/* A key/value cache in 4 bits.  32 neighbouring columns of a head share a scale, (their largest magnitude / 7) rounded to 5
+ * significant bits; a value is scale * c with a whole number c in -7..7, exact in bf16.  groups = ceil(head_dim / 32):
+ *   codes  [batch, kv_heads, max_len, 16 * groups] bytes: a position's row is 4 * groups 32-bit words, of which word
+ *          t * groups + j holds columns 32 j + 8 t + e, e = 0..7, as c + 8 in the 4 bits from 4 * (e / 2) + 16 * (e % 2)
+ *   scales [batch, kv_heads, max_len, groups] bf16
+ * for keys and for values each; 4.5 bits a value where head_dim is a multiple of 32.  32 columns whose largest magnitude is below
+ * 2^-100 are zeros, one above 7 * 2^122 saturates, and with a NaN or an infinity among them all 32 read back as NaN.
+ * head_dim a multiple of 8 up to 128.  A length below 0 or above max_len is taken as the nearest that is not, no memory outside the
+ * cache is touched, and the context's status word reports it (IT_ERR_INVALID_ARG from it_stream_sync and the like). */
+
+/* k, v [batch, tokens, kv_heads, head_dim] into the cache behind the lengths[b] positions of each sequence: of sequence b its first
+ * counts[b] tokens (null: all).  new_lengths[b] = what is there afterwards; it must not be `lengths`.  Nothing else of the cache is
+ * written.  A token that does not fit is dropped and reported as above. */
+it_status it_kv_cache_q4_append(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t batch, int32_t tokens, int32_t kv_heads,
+                                int32_t head_dim, int32_t max_len, const void* k, const void* v, const int32_t* lengths,
+                                const int32_t* counts, int32_t* new_lengths, void* k_codes, void* k_scales, void* v_codes,
+                                void* v_scales);
+/* Positions starts[b] .. starts[b] + tokens - 1 (starts null: from 0) out of the cache as k, v [batch, tokens, kv_heads,
+ * head_dim]; zeros where a position is negative or not below lengths[b] (null: max_len). */
+it_status it_kv_cache_q4_read(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t batch, int32_t tokens, int32_t kv_heads,
+                              int32_t head_dim, int32_t max_len, const void* k_codes, const void* k_scales, const void* v_codes,
+                              const void* v_scales, const int32_t* starts, const int32_t* lengths, void* k, void* v);
+/* it_attention_decode over such a cache, sequence b over its first lengths[b] positions: q, o [batch, heads, head_dim], lse [batch,
+ * heads] (may be null).  A sequence without positions gives zeros, and -inf in lse.  fp32 math; results repeat bit for bit. */
+it_status it_attention_decode_q4_workspace_bytes(int32_t batch, int32_t heads, int32_t head_dim, size_t* out_bytes);
+it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t batch, int32_t heads, int32_t kv_heads,
+                                 int32_t head_dim, int32_t max_len, const void* q, const void* k_codes, const void* k_scales,
+                                 const void* v_codes, const void* v_scales, const int32_t* lengths, void* o, float* lse,
+                                 void* workspace, size_t workspace_bytes);
+
+/* Projections in 8-bit integers.  it_quantize_rows_i8: x [rows, cols] -> codes [rows, cols] signed bytes, scales [rows] fp32; a
+ * row's scale is (its largest magnitude / 127) rounded to 8 significant bits, a value is scale * c with c in -127..127 (rows below
+ * 2^-100: zeros; with a NaN or an infinity: the scale is NaN).  Tokens are rows of activations, channels rows of weights.
+ * it_linear_i8_fwd: y[i, o] = sum_k x_codes[i, k] w_codes[o, k] * (x_scales[i] * w_scales[o]) with exact 32-bit sums, on tcgen05
+ * (kind::i8).  The columns of y go to n_outs (1 to 3) tensors [n, widths[r]] of the given type, side by side: one call for the
+ * stacked weights [Wq; Wk; Wv].  in_dim a multiple of 16 up to 65536; out_dim = the sum of the widths, multiples of 8 each. */
+it_status it_quantize_rows_i8(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t rows, int32_t cols, const void* x,
+                              int8_t* codes, float* scales);
+it_status it_linear_i8_fwd(it_ctx* ctx, it_stream* stream, it_dtype out_dtype, int32_t n, int32_t in_dim, int32_t out_dim,
+                           const int8_t* x_codes, const float* x_scales, const int8_t* w_codes, const float* w_scales,
+                           int32_t n_outs, const int32_t* widths, void* const* outs);
 
 /* Forward + backward for tensors that live in page-locked HOST memory (the reference's buffers are unified memory, so
  * its ops never copy: src/tensor.rs:73; on a discrete GPU a caller with host data pays the host link both ways).  One

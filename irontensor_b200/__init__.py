@@ -9,7 +9,9 @@ import importlib
 _MODULES = ("ops", "synth", "_lib")
 __all__ = ["CommandBatch", "Precision", "Tensor", "attention", "attention_backward", "attention_backward_recompute", "attention_gqa",
            "attention_gqa_backward", "attention_decode", "attention_packed", "attention_packed_backward", "linear_backward",
-           "linear_forward", "qkv_rope_forward", "rope", "rope_qk", "flash_attention", "context", "raw", "HostAttentionStep"]
+           "linear_forward", "qkv_rope_forward", "rope", "rope_qk", "flash_attention", "context", "raw", "HostAttentionStep", "rope_positions",
+           "QuantizedCache", "kv_cache_append", "kv_cache_read", "attention_decode_quantized", "QuantizedRows", "quantize_rows",
+           "linear_int8_forward"]
 
 
 def __getattr__(name):

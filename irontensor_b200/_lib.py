@@ -67,6 +67,13 @@ SIGNATURES = {
     "it_qkv_rope_workspace_bytes": [_i32, _i32, _c.POINTER(_c.c_size_t)],
     "it_qkv_rope_fwd": [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _c.c_float, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _c.c_size_t],
     "it_linear_bwd": [_vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp],
+    "it_rope_positions": [_vp, _vp, _c.c_int, _i32, _i32, _i32, _i32, _i32, _c.c_float, _i32, _c.POINTER(_i32), _i32, _i32] + [_vp] * 5,
+    "it_kv_cache_q4_append": [_vp, _vp, _c.c_int, _i32, _i32, _i32, _i32, _i32] + [_vp] * 9,
+    "it_kv_cache_q4_read": [_vp, _vp, _c.c_int, _i32, _i32, _i32, _i32, _i32] + [_vp] * 8,
+    "it_attention_decode_q4_workspace_bytes": [_i32, _i32, _i32, _c.POINTER(_c.c_size_t)],
+    "it_attention_decode_q4": [_vp, _vp, _c.c_int, _i32, _i32, _i32, _i32, _i32] + [_vp] * 9 + [_c.c_size_t],
+    "it_quantize_rows_i8": [_vp, _vp, _c.c_int, _i32, _i32, _vp, _vp, _vp],
+    "it_linear_i8_fwd": [_vp, _vp, _c.c_int, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _c.POINTER(_i32), _c.POINTER(_vp)],
     "it_flash_attention_bwd_noalloc": [_vp, _vp, _c.c_int, _i32, _i32, _i32, _i32, _i32] + [_vp] * 9,
     "it_attention_status_poll": [_vp, _vp, _c.POINTER(_i32)],
     "it_ctx_launch_count": [_vp, _c.POINTER(_c.c_uint64)],

@@ -4,6 +4,7 @@ side of the Python ops, with g++ against the installed torch.
     python -m irontensor_b200.build [--force] [--verbose]
 """
 import os
+import re
 import subprocess
 import sys
 
@@ -15,17 +16,30 @@ _HOST_SRC = os.path.join(_CSRC, "host_ops.cpp")
 _HOST_OUT = os.path.join(_HERE, "_host_ops.so")
 
 
-def _sources():
-    deps = [os.path.join(_CSRC, f) for f in sorted(os.listdir(_CSRC)) if f.endswith((".cu", ".cuh"))]
-    deps.append(os.path.join(_INC, "irontensor_b200.h"))
-    return deps
+_UNITS = ("it_capi.cu", "it_quant.cu")   # translation units of libirontensor_b200.so
+
+
+def _depends(path, seen=None):
+    """`path` and the files of this repository that it includes."""
+    seen = set() if seen is None else seen
+    if path not in seen and os.path.exists(path):
+        seen.add(path)
+        with open(path) as f:
+            for name in re.findall(r'^\s*#include "([^"]+)"', f.read(), re.M):
+                _depends(os.path.normpath(os.path.join(os.path.dirname(path), name)), seen)
+    return seen
+
+
+def _object(unit):
+    return os.path.join(_HERE, os.path.splitext(unit)[0] + ".o")
+
+
+def _newer(out, sources):
+    return os.path.exists(out) and all(os.path.getmtime(s) <= os.path.getmtime(out) for s in sources)
 
 
 def up_to_date():
-    if not os.path.exists(_OUT):
-        return False
-    t = os.path.getmtime(_OUT)
-    return all(os.path.getmtime(s) <= t for s in _sources())
+    return all(_newer(_OUT, _depends(os.path.join(_CSRC, u))) for u in _UNITS)
 
 
 def _host_up_to_date():
@@ -54,11 +68,22 @@ def build(force=False, verbose=False):
         build_host()
         return _OUT
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-    cmd = [nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-           "-shared", "-Xcompiler", "-fPIC", "-o", _OUT, os.path.join(_CSRC, "it_capi.cu")]
+    arch = ["-gencode", "arch=compute_100a,code=sm_100a"]
+    flags = [*arch, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
     if verbose:
-        cmd[1:1] = ["-Xptxas", "-v"]
-    subprocess.run(cmd, check=True)
+        flags = ["-Xptxas", "-v"] + flags
+    running = []   # the units that changed, side by side
+    for unit in _UNITS:
+        src, obj = os.path.join(_CSRC, unit), _object(unit)
+        if force or not _newer(obj, _depends(src)):
+            cmd = [nvcc, *flags, "-c", "-o", obj + ".new", src]
+            running.append((cmd, obj, subprocess.Popen(cmd)))
+    codes = [p.wait() for _, _, p in running]
+    for (cmd, obj, _), rc in zip(running, codes):
+        if rc != 0:
+            raise subprocess.CalledProcessError(rc, cmd)
+        os.replace(obj + ".new", obj)
+    subprocess.run([nvcc, *arch, "-shared", "-o", _OUT, *[_object(u) for u in _UNITS]], check=True)
     build_host(force)
     return _OUT
 

@@ -2,7 +2,7 @@
 // events, buffers, and the attention forward / backward dispatch onto the sm_100a kernels.
 // Host-side validation mirrors the reference's asserts (src/ops/flash_attention.rs:78-104) but
 // returns status codes instead of panicking.
-#include "../../include/irontensor_b200.h"
+#include "capi_common.h"
 
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -33,8 +33,8 @@
 #include "selftest_sm100.cuh"
 
 namespace {
-
 thread_local char g_err[512] = "";
+}  // namespace
 
 it_status fail(it_status code, const char* fmt, ...) {
   va_list ap;
@@ -44,69 +44,6 @@ it_status fail(it_status code, const char* fmt, ...) {
   return code;
 }
 
-#define IT_CUDA(expr)                                                                              \
-  do {                                                                                             \
-    cudaError_t e_ = (expr);                                                                       \
-    if (e_ != cudaSuccess) return fail(IT_ERR_CUDA, "%s: %s", #expr, cudaGetErrorString(e_));      \
-  } while (0)
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-}  // namespace
-
-// The counters of captured launches.  A graph gives its launches' back when it and the executable graphs made from it are
-// gone, possibly after the context and from a thread of the driver's: hence shared ownership.
-struct CaptureSlots {
-  struct Held {   // what a graph holds
-    std::shared_ptr<CaptureSlots> slots;
-    int i = 0;
-    Held* next = nullptr;
-  };
-  std::mutex mutex;
-  int next = 0;
-  Held *oldest = nullptr, *newest = nullptr;   // given back: reused oldest first, and only once every one has been out
-  ~CaptureSlots() {
-    while (oldest != nullptr) {
-      Held* h = oldest;
-      oldest = h->next;
-      delete h;
-    }
-  }
-};
-struct it_ctx {
-  int device = 0;
-  int sm_count = 0;
-  int* d_status = nullptr;      // device status word written by kernels whose waits run out
-  int* h_status = nullptr;      // pinned mirror
-  cudaStream_t status_stream = nullptr;   // reads the status word without touching a caller's stream
-  std::mutex status_mutex;      // h_status and status_stream are shared by every thread using the context
-  EncodeTiledFn encode = nullptr;
-  int timing = 0;               // events around: 1 the backward main kernel; 2 the forward kernel too; 3 the backward's prepare and finish passes too
-  // [forward | backward main | backward prepare | backward finish][start | stop]; the prepare pass starts where the
-  // previous timer stopped only in time, not in events: three pairs share the boundaries prepare|main|finish
-  cudaEvent_t ev[4][2] = {};
-  bool ev_valid[4] = {false, false, false, false};
-  std::atomic<uint64_t> launches{0};
-  // Work-item counters of the forward kernel that walks its items in a loop: a pair of ints per live stream object (launches
-  // on one stream run one after the other, so a stream needs one pair), handed out from a pool allocated with the
-  // context so that wrapping a stream calls nothing a stream capture forbids; and behind those one per captured launch.
-  // Zeroed once, here; every launch leaves its pair at zero, also one that gave up.
-  static constexpr int WORK_SLOTS = 4096, CAPTURE_SLOTS = 61440;
-  static constexpr size_t WORK_BYTES = 2 * sizeof(int) * (WORK_SLOTS + CAPTURE_SLOTS);
-  std::shared_ptr<CaptureSlots> captured;
-  int* d_work_pool = nullptr;
-  std::mutex work_mutex;
-  std::vector<int> work_free;
-  int work_next = 0;
-};
-struct it_stream {
-  cudaStream_t s = nullptr;
-  bool owned = false;
-  int* d_work = nullptr;     // this stream's work-item counter; null when the pool ran out (the launcher then starts one CTA per item)
-  bool work_used = false;    // a launch has drawn from the counter
-};
 namespace {
 int* take_work_slot(it_ctx* ctx) {
   std::lock_guard<std::mutex> lock(ctx->work_mutex);
@@ -204,16 +141,20 @@ it_status read_device_status(it_ctx* ctx, int* out) {
   return IT_OK;
 }
 
+// The error that a device status word stands for.  `left`: it stays set.
+it_status device_status_error(int st, bool left) {
+  const char* then = left ? ": results of launches since then are invalid, and further launches on this context do nothing until "
+                            "it_attention_status_poll clears it"
+                          : "";
+  if (st == it::DEV_ERR_CACHE_RANGE)
+    return fail(IT_ERR_INVALID_ARG, "a sequence's length lay outside its quantised cache (device status %d)%s", st, then);
+  return fail(IT_ERR_TIMEOUT, "a bounded wait inside a kernel ran out (device status %d)%s", st, then);
+}
+
 it_status fail_if_device_status(it_ctx* ctx) {
   int st = 0;
   it_status rc = read_device_status(ctx, &st);
-  if (rc != IT_OK) return rc;
-  if (st != 0)
-    return fail(IT_ERR_TIMEOUT,
-                "a bounded wait inside a kernel ran out (device status %d): results of launches since then are "
-                "invalid, and further launches on this context do nothing until it_attention_status_poll clears it",
-                st);
-  return IT_OK;
+  return rc != IT_OK ? rc : st != 0 ? device_status_error(st, true) : IT_OK;
 }
 
 // A bf16 attention tensor viewed by TMA as a 4-D tensor (head_dim, seq, heads, batch) with the
@@ -257,8 +198,6 @@ it::RopeFreqs make_rope_freqs(int D, float base, int position_offset, bool enabl
   return f;
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 it_status check_common(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t B, int32_t H, int32_t S, int32_t D) {
   if (ctx == nullptr || stream == nullptr) return fail(IT_ERR_INVALID_ARG, "null context or stream");
   if (dtype != IT_F32 && dtype != IT_BF16) return fail(IT_ERR_PRECISION, "dtype %d is not F32 or BF16", (int)dtype);
@@ -267,31 +206,6 @@ it_status check_common(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t B
   if (static_cast<int64_t>(B) * H > 65535)
     return fail(IT_ERR_UNSUPPORTED_SHAPE, "batch*heads must be <= 65535, got %lld", (long long)B * H);
   return IT_OK;
-}
-
-// Launch with the programmatic-stream-serialization attribute: the kernel may be set up while the kernel in front of it
-// in the stream still runs, and waits in griddepcontrol.wait for that kernel's completion before it touches its results.
-// launch_cluster: in clusters of `cluster` CTAs along x (1: no clusters).
-template <typename... KArgs, typename... Args>
-cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, int cluster, Args&&... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(std::forward<Args>(args))...);
-}
-template <typename... KArgs, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args&&... args) {
-  return launch_cluster(kernel, grid, block, smem, s, 1, std::forward<Args>(args)...);
 }
 
 // The tensor-core kernels take bf16 tensors whose rows TMA can address (a multiple of 8 columns = 16 bytes); rows past the
@@ -1863,7 +1777,7 @@ it_status it_attention_status_poll(it_ctx* ctx, it_stream* stream, int32_t* devi
   if (*device_status != 0) {
     IT_CUDA(cudaMemsetAsync(ctx->d_status, 0, sizeof(int), stream->s));
     IT_CUDA(cudaStreamSynchronize(stream->s));
-    return fail(IT_ERR_TIMEOUT, "a bounded wait inside a kernel ran out (device status %d)", *device_status);
+    return device_status_error(*device_status, false);
   }
   return IT_OK;
 }

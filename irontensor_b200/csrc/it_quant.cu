@@ -1,0 +1,307 @@
+// C ABI of serving from quantised weights and a quantised key/value cache (declared in include/irontensor_b200.h): argument
+// checks, choice of kernels, launches.
+#include "capi_common.h"
+
+#include <algorithm>
+#include <cmath>
+
+#include "fa_decode_q4.cuh"
+#include "gemm_i8_sm100.cuh"
+#include "kv_q4.cuh"
+#include "rope_positions.cuh"
+
+namespace {
+
+it_status check_call(it_ctx* ctx, it_stream* stream, it_dtype dtype) {
+  if (ctx == nullptr || stream == nullptr) return fail(IT_ERR_INVALID_ARG, "null context or stream");
+  if (dtype != IT_F32 && dtype != IT_BF16) return fail(IT_ERR_PRECISION, "dtype %d is not F32 or BF16", (int)dtype);
+  return IT_OK;
+}
+
+// What the three cache calls have in common.  *empty: there is nothing to do.
+it_status check_cache(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t B, int32_t n, int32_t Hkv, int32_t D, int32_t max_len,
+                      const void* kc, const void* ks, const void* vc, const void* vs) {
+  it_status st = check_call(ctx, stream, dtype);
+  if (st != IT_OK) return st;
+  if (B < 0 || n < 0 || Hkv < 1 || max_len < 1) return fail(IT_ERR_INVALID_ARG, "bad dimension: batch %d, %d, kv_heads %d, max_len %d", B, n, Hkv, max_len);
+  if (D < 8 || D > 128 || (D & 7)) return fail(IT_ERR_UNSUPPORTED_SHAPE, "a quantised cache needs head_dim a multiple of 8 in 8..128, got %d", D);
+  if (B == 0) return IT_OK;
+  if (kc == nullptr || ks == nullptr || vc == nullptr || vs == nullptr) return fail(IT_ERR_INVALID_ARG, "null cache");
+  if (!aligned16(kc) || !aligned16(vc)) return fail(IT_ERR_ALIGNMENT, "codes must be 16-byte aligned");
+  const int groups = (D + 31) / 32, unit = 2 * (groups & -groups);   // a position's scales are read together where they are 2 or 4
+  if ((reinterpret_cast<uintptr_t>(ks) | reinterpret_cast<uintptr_t>(vs)) & (unit - 1))
+    return fail(IT_ERR_ALIGNMENT, "scales must be %d-byte aligned", unit);
+  return IT_OK;
+}
+
+// CTAs of 256 threads for so many threads; 0 where a launch does not hold them.
+unsigned ctas_of(double threads) {
+  const double n = std::ceil(threads / 256.0);
+  return n <= 2147483647.0 ? static_cast<unsigned>(n) : 0u;
+}
+
+it::KvQ4 half_of(const void* codes, const void* scales) {
+  return it::KvQ4{static_cast<uint32_t*>(const_cast<void*>(codes)), static_cast<__nv_bfloat16*>(const_cast<void*>(scales))};
+}
+
+}  // namespace
+
+extern "C" {
+
+it_status it_rope_positions(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t B, int32_t S, int32_t H, int32_t Hkv, int32_t D,
+                            float rope_base, int32_t n_axes, const int32_t* sections, int32_t per_axis, int32_t inverse,
+                            const int32_t* positions, const void* q_in, const void* k_in, void* q_out, void* k_out) {
+  it_status st = check_call(ctx, stream, dtype);
+  if (st != IT_OK) return st;
+  if (B < 0 || S < 0 || H < 0 || Hkv < 0) return fail(IT_ERR_INVALID_ARG, "negative dimension");
+  if (D < 2 || D > 128 || (D & 1)) return fail(IT_ERR_UNSUPPORTED_SHAPE, "rotary embedding needs an even head_dim in 2..128, got %d", D);
+  if (!(rope_base > 0.f) || !std::isfinite(rope_base)) return fail(IT_ERR_INVALID_ARG, "rotary base must be positive and finite");
+  if (n_axes < 1 || n_axes > 4 || sections == nullptr) return fail(IT_ERR_INVALID_ARG, "1 to 4 axes with a section each, got %d", n_axes);
+  it::RopeAxes axes{};
+  int pair = 0;
+  for (int a = 0; a < n_axes; ++a) {
+    if (sections[a] < 0 || sections[a] > D / 2 - pair) return fail(IT_ERR_INVALID_ARG, "sections must add up to head_dim / 2 = %d", D / 2);
+    for (int j = 0; j < sections[a]; ++j, ++pair) {
+      axes.freq[pair] = std::pow(static_cast<double>(rope_base), per_axis ? -static_cast<double>(j) / sections[a] : -2.0 * pair / D);
+      axes.axis[pair] = static_cast<uint8_t>(a);
+    }
+  }
+  if (pair != D / 2) return fail(IT_ERR_INVALID_ARG, "sections must add up to head_dim / 2 = %d", D / 2);
+  const int64_t rows = static_cast<int64_t>(B) * S;
+  if (rows == 0 || (H == 0 && Hkv == 0)) return IT_OK;
+  if (static_cast<int64_t>(H) + Hkv > 65535) return fail(IT_ERR_UNSUPPORTED_SHAPE, "heads + kv_heads must be at most 65535");
+  if (positions == nullptr) return fail(IT_ERR_INVALID_ARG, "null positions");
+  if (H > 0 && (q_in == nullptr || q_out == nullptr)) return fail(IT_ERR_INVALID_ARG, "null q tensor");
+  if (Hkv > 0 && (k_in == nullptr || k_out == nullptr)) return fail(IT_ERR_INVALID_ARG, "null k tensor");
+  IT_CUDA(cudaSetDevice(ctx->device));
+  const int half = D / 2, elem = dtype == IT_F32 ? 4 : 2;
+  const bool chunks = (D * elem) % 16 == 0 && aligned16(q_in) && aligned16(q_out) && aligned16(k_in) && aligned16(k_out);
+  const uintptr_t pair_mask = 2 * elem - 1;
+  if (!chunks && ((reinterpret_cast<uintptr_t>(q_in) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k_in) |
+                   reinterpret_cast<uintptr_t>(k_out)) & pair_mask))
+    return fail(IT_ERR_ALIGNMENT, "q and k must be aligned to a pair of elements");
+  const int n_pos = static_cast<int>(std::clamp<int64_t>(rows / (4LL * ctx->sm_count), 1, 256 / half));
+  const int64_t ctas = (rows + n_pos - 1) / n_pos;
+  if (ctas > 2147483647LL) return fail(IT_ERR_UNSUPPORTED_SHAPE, "too many tokens");
+  auto launch = [&](auto kernel, auto* q, auto* k, auto* qo, auto* ko) -> it_status {
+    IT_CUDA(launch_dependent(kernel, static_cast<unsigned>(ctas), 256, 0, stream->s, q, k, qo, ko, positions, static_cast<long long>(rows), n_pos,
+                             H, Hkv, D, inverse ? 1 : 0, axes));
+    ctx->launches += 1;
+    return IT_OK;
+  };
+  if (dtype == IT_F32)
+    return launch(chunks ? it::rope_positions_kernel<float, 4> : it::rope_positions_kernel<float, 2>, static_cast<const float*>(q_in),
+                  static_cast<const float*>(k_in), static_cast<float*>(q_out), static_cast<float*>(k_out));
+  using BF = __nv_bfloat16;
+  return launch(chunks ? it::rope_positions_kernel<BF, 8> : it::rope_positions_kernel<BF, 2>, static_cast<const BF*>(q_in),
+                static_cast<const BF*>(k_in), static_cast<BF*>(q_out), static_cast<BF*>(k_out));
+}
+
+it_status it_kv_cache_q4_append(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t B, int32_t T, int32_t Hkv, int32_t D,
+                                int32_t max_len, const void* k, const void* v, const int32_t* lengths, const int32_t* counts,
+                                int32_t* new_lengths, void* k_codes, void* k_scales, void* v_codes, void* v_scales) {
+  it_status st = check_cache(ctx, stream, dtype, B, T, Hkv, D, max_len, k_codes, k_scales, v_codes, v_scales);
+  if (st != IT_OK || B == 0) return st;
+  if (lengths == nullptr || new_lengths == nullptr) return fail(IT_ERR_INVALID_ARG, "null lengths");
+  if (lengths == new_lengths || counts == new_lengths) return fail(IT_ERR_INVALID_ARG, "new_lengths must be another array than lengths and counts");
+  if (T > 0 && (k == nullptr || v == nullptr)) return fail(IT_ERR_INVALID_ARG, "null tensor");
+  if (!aligned16(k) || !aligned16(v)) return fail(IT_ERR_ALIGNMENT, "k and v must be 16-byte aligned");
+  const int lanes = 4 * ((D + 31) / 32);
+  const unsigned ctas = ctas_of(std::max(2.0 * B * T * Hkv * lanes, static_cast<double>(B)));
+  if (ctas == 0) return fail(IT_ERR_UNSUPPORTED_SHAPE, "too many tokens");
+  IT_CUDA(cudaSetDevice(ctx->device));
+  auto launch = [&](auto kernel, auto* kk, auto* vv) -> it_status {
+    IT_CUDA(launch_dependent(kernel, ctas, 256, 0, stream->s, kk, vv, half_of(k_codes, k_scales), half_of(v_codes, v_scales), lengths, counts,
+                             new_lengths, B, T, Hkv, D, max_len, ctx->d_status));
+    ctx->launches += 1;
+    return IT_OK;
+  };
+  return dtype == IT_F32 ? launch(it::kv_q4_append_kernel<float>, static_cast<const float*>(k), static_cast<const float*>(v))
+                         : launch(it::kv_q4_append_kernel<__nv_bfloat16>, static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v));
+}
+
+it_status it_kv_cache_q4_read(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t B, int32_t T, int32_t Hkv, int32_t D, int32_t max_len,
+                              const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, const int32_t* starts,
+                              const int32_t* lengths, void* k, void* v) {
+  it_status st = check_cache(ctx, stream, dtype, B, T, Hkv, D, max_len, k_codes, k_scales, v_codes, v_scales);
+  if (st != IT_OK || B == 0 || T == 0) return st;
+  if (k == nullptr || v == nullptr) return fail(IT_ERR_INVALID_ARG, "null tensor");
+  if (!aligned16(k) || !aligned16(v)) return fail(IT_ERR_ALIGNMENT, "k and v must be 16-byte aligned");
+  const unsigned ctas = ctas_of(2.0 * B * T * Hkv * (D / 8));
+  if (ctas == 0) return fail(IT_ERR_UNSUPPORTED_SHAPE, "too many tokens");
+  IT_CUDA(cudaSetDevice(ctx->device));
+  auto launch = [&](auto kernel, auto* kk, auto* vv) -> it_status {
+    IT_CUDA(launch_dependent(kernel, ctas, 256, 0, stream->s, kk, vv, half_of(k_codes, k_scales), half_of(v_codes, v_scales), starts, lengths, B, T,
+                             Hkv, D, max_len));
+    ctx->launches += 1;
+    return IT_OK;
+  };
+  return dtype == IT_F32 ? launch(it::kv_q4_read_kernel<float>, static_cast<float*>(k), static_cast<float*>(v))
+                         : launch(it::kv_q4_read_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v));
+}
+
+it_status it_attention_decode_q4_workspace_bytes(int32_t B, int32_t H, int32_t D, size_t* out_bytes) {
+  if (out_bytes == nullptr) return fail(IT_ERR_INVALID_ARG, "out_bytes is null");
+  if (B < 0 || H < 0) return fail(IT_ERR_INVALID_ARG, "negative dimension");
+  if (D < 8 || D > 128 || (D & 7)) return fail(IT_ERR_UNSUPPORTED_SHAPE, "a quantised cache needs head_dim a multiple of 8 in 8..128, got %d", D);
+  const size_t n = static_cast<size_t>(B) * H * it::DQ_MAX_SPLITS * (static_cast<size_t>(D) + 2) * sizeof(float);
+  *out_bytes = (n + 255) / 256 * 256 + 256;
+  return IT_OK;
+}
+
+it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t B, int32_t H, int32_t Hkv, int32_t D,
+                                 int32_t max_len, const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
+                                 const void* v_scales, const int32_t* lengths, void* o, float* lse, void* workspace,
+                                 size_t workspace_bytes) {
+  it_status st = check_cache(ctx, stream, dtype, B, H, Hkv, D, max_len, k_codes, k_scales, v_codes, v_scales);
+  if (st != IT_OK) return st;
+  if (H % Hkv != 0) return fail(IT_ERR_INVALID_ARG, "heads (%d) must be divisible by kv_heads (%d)", H, Hkv);
+  if (static_cast<int64_t>(B) * H > 65535) return fail(IT_ERR_UNSUPPORTED_SHAPE, "batch*heads must be <= 65535, got %lld", (long long)B * H);
+  if (B == 0 || H == 0) return IT_OK;
+  if (q == nullptr || o == nullptr || lengths == nullptr) return fail(IT_ERR_INVALID_ARG, "null tensor");
+  if (!aligned16(q) || !aligned16(o)) return fail(IT_ERR_ALIGNMENT, "q and o must be 16-byte aligned");
+  size_t need = 0;
+  it_attention_decode_q4_workspace_bytes(B, H, D, &need);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(IT_ERR_INVALID_ARG, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return fail(IT_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+  IT_CUDA(cudaSetDevice(ctx->device));
+  it::DecodeQ4Params p;
+  p.q = q;
+  p.k_codes = static_cast<const uint32_t*>(k_codes);
+  p.v_codes = static_cast<const uint32_t*>(v_codes);
+  p.k_scales = static_cast<const __nv_bfloat16*>(k_scales);
+  p.v_scales = static_cast<const __nv_bfloat16*>(v_scales);
+  p.lengths = lengths;
+  p.o = o;
+  p.lse = lse;
+  p.status = ctx->d_status;
+  p.H = H;
+  p.Hkv = Hkv;
+  p.D = D;
+  p.max_len = max_len;
+  p.scale_log2 = (1.0f / sqrtf(static_cast<float>(D))) * 1.4426950408889634f;
+  // As many shares of a sequence as fill the GPU, none of less than a round of the CTA's warps at max_len
+  const int G = H / Hkv, chunks = (G + it::DQ_HEADS - 1) / it::DQ_HEADS;
+  const long long base = static_cast<long long>(B) * Hkv * chunks, round = it::DQ_WARPS * it::DQ_BLOCK;
+  p.n_splits = static_cast<int>(std::max(1LL, std::min<long long>({(ctx->sm_count + base - 1) / base, (max_len + round - 1) / round, it::DQ_MAX_SPLITS})));
+  float* ws = static_cast<float*>(workspace);
+  p.part_o = ws;
+  p.part_ml = ws + static_cast<size_t>(B) * H * p.n_splits * D;
+  const dim3 grid(p.n_splits, Hkv * chunks, B);
+  auto launch = [&](auto kernel) -> it_status {
+    IT_CUDA(launch_dependent(kernel, grid, 32 * it::DQ_WARPS, 0, stream->s, p));
+    ctx->launches += 1;
+    return IT_OK;
+  };
+  const int groups = (D + 31) / 32;
+  if (dtype == IT_F32)
+    st = groups == 1 ? launch(it::fa_decode_q4_kernel<1, 3>) : groups == 2 ? launch(it::fa_decode_q4_kernel<2, 3>)
+         : groups == 3 ? launch(it::fa_decode_q4_kernel<3, 3>) : launch(it::fa_decode_q4_kernel<4, 3>);
+  else
+    st = groups == 1 ? launch(it::fa_decode_q4_kernel<1, 1>) : groups == 2 ? launch(it::fa_decode_q4_kernel<2, 1>)
+         : groups == 3 ? launch(it::fa_decode_q4_kernel<3, 1>) : launch(it::fa_decode_q4_kernel<4, 1>);
+  if (st != IT_OK || p.n_splits == 1) return st;
+  auto merge = [&](auto kernel, auto* out) -> it_status {
+    IT_CUDA(launch_dependent(kernel, static_cast<unsigned>(B * H), 128, 0, stream->s, static_cast<const float*>(p.part_o),
+                             static_cast<const float*>(p.part_ml), lengths, out, lse, p.n_splits, H, D));
+    ctx->launches += 1;
+    return IT_OK;
+  };
+  return dtype == IT_F32 ? merge(it::fa_decode_q4_merge_kernel<float>, static_cast<float*>(o))
+                         : merge(it::fa_decode_q4_merge_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(o));
+}
+
+it_status it_quantize_rows_i8(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t rows, int32_t cols, const void* x, int8_t* codes,
+                              float* scales) {
+  it_status st = check_call(ctx, stream, dtype);
+  if (st != IT_OK) return st;
+  if (rows < 0 || cols < 0) return fail(IT_ERR_INVALID_ARG, "negative dimension");
+  if (cols == 0 || (cols & 15)) return fail(IT_ERR_UNSUPPORTED_SHAPE, "rows to quantise need a multiple of 16 columns, got %d", cols);
+  if (rows == 0) return IT_OK;
+  if (x == nullptr || codes == nullptr || scales == nullptr) return fail(IT_ERR_INVALID_ARG, "null tensor");
+  if (!aligned16(x) || !aligned16(codes)) return fail(IT_ERR_ALIGNMENT, "x and codes must be 16-byte aligned");
+  IT_CUDA(cudaSetDevice(ctx->device));
+  auto launch = [&](auto kernel, auto* src) -> it_status {
+    IT_CUDA(launch_dependent(kernel, static_cast<unsigned>(rows), 256, 0, stream->s, src, codes, scales, cols));
+    ctx->launches += 1;
+    return IT_OK;
+  };
+  return dtype == IT_F32 ? launch(it::quantize_rows_kernel<float>, static_cast<const float*>(x))
+                         : launch(it::quantize_rows_kernel<__nv_bfloat16>, static_cast<const __nv_bfloat16*>(x));
+}
+
+}  // extern "C"
+
+namespace {
+
+// [rows, K] bytes as TMA sees them: boxes of 128 columns by `box_rows` rows, 128-byte swizzle, zeros outside.
+it_status make_bytes_map(it_ctx* ctx, CUtensorMap* map, const void* base, int rows, int K, int box_rows) {
+  const cuuint64_t n = static_cast<cuuint64_t>(rows), k = static_cast<cuuint64_t>(K);
+  const cuuint64_t dims[4] = {k, n, 1, 1}, strides[3] = {k, k * n, k * n};
+  const cuuint32_t box[4] = {128, static_cast<cuuint32_t>(box_rows), 1, 1}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = ctx->encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, estr,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? IT_OK : fail(IT_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", static_cast<int>(r));
+}
+
+template <int BN, int CG>
+it_status launch_gemm_i8(it_ctx* ctx, cudaStream_t s, const int8_t* x, const int8_t* w, it::GemmI8Params p) {
+  using T = it::GemmTraits<BN, CG>;
+  CUtensorMap ma, mb;
+  it_status st;
+  if ((st = make_bytes_map(ctx, &ma, x, p.M, p.K, T::BM)) != IT_OK || (st = make_bytes_map(ctx, &mb, w, p.N, p.K, T::B_ROWS)) != IT_OK) return st;
+  static std::atomic<bool> attr_set[16];
+  if (!attr_set[ctx->device & 15]) {
+    IT_CUDA(cudaFuncSetAttribute(it::gemm_i8_sm100_kernel<BN, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM_BYTES));
+    attr_set[ctx->device & 15] = true;
+  }
+  const long long tiles = static_cast<long long>((p.M + CG * T::BM - 1) / (CG * T::BM)) * ((p.N + BN - 1) / BN);
+  const int grid = static_cast<int>(std::min<long long>(tiles, ctx->sm_count / CG)) * CG;
+  IT_CUDA(launch_cluster(it::gemm_i8_sm100_kernel<BN, CG>, grid, T::THREADS, T::SMEM_BYTES, s, CG, ma, mb, p));
+  ctx->launches += 1;
+  return IT_OK;
+}
+
+}  // namespace
+
+extern "C" it_status it_linear_i8_fwd(it_ctx* ctx, it_stream* stream, it_dtype out_dtype, int32_t n, int32_t in_dim, int32_t out_dim,
+                                      const int8_t* x_codes, const float* x_scales, const int8_t* w_codes, const float* w_scales,
+                                      int32_t n_outs, const int32_t* widths, void* const* outs) {
+  it_status st = check_call(ctx, stream, out_dtype);
+  if (st != IT_OK) return st;
+  if (n < 0 || in_dim < 0 || out_dim < 0) return fail(IT_ERR_INVALID_ARG, "negative dimension");
+  if (in_dim < 16 || in_dim > 65536 || (in_dim & 15))
+    return fail(IT_ERR_UNSUPPORTED_SHAPE, "in_dim must be a multiple of 16 in 16..65536, got %d", in_dim);
+  if (n_outs < 1 || n_outs > 3 || widths == nullptr || outs == nullptr) return fail(IT_ERR_INVALID_ARG, "1 to 3 results, got %d", n_outs);
+  it::GemmI8Params p{};
+  int64_t end = 0;
+  for (int r = 0; r < 3; ++r) {
+    const int width = r < n_outs ? widths[r] : 0;
+    if (width < 0) return fail(IT_ERR_INVALID_ARG, "negative width");
+    if (width & 7) return fail(IT_ERR_UNSUPPORTED_SHAPE, "widths must be multiples of 8, got %d", width);
+    end += width;
+    if (end > out_dim) break;
+    p.out.end[r] = static_cast<int>(end);
+    p.out.ptr[r] = r < n_outs ? outs[r] : nullptr;
+    if (width > 0 && n > 0) {
+      if (outs[r] == nullptr) return fail(IT_ERR_INVALID_ARG, "null tensor");
+      if (!aligned16(outs[r])) return fail(IT_ERR_ALIGNMENT, "results must be 16-byte aligned");
+    }
+  }
+  if (end != out_dim) return fail(IT_ERR_INVALID_ARG, "widths must add up to out_dim = %d", out_dim);
+  if (n == 0 || out_dim == 0) return IT_OK;
+  if (x_codes == nullptr || x_scales == nullptr || w_codes == nullptr || w_scales == nullptr) return fail(IT_ERR_INVALID_ARG, "null tensor");
+  if (!aligned16(x_codes) || !aligned16(w_codes) || !aligned16(w_scales))
+    return fail(IT_ERR_ALIGNMENT, "codes and weight scales must be 16-byte aligned");
+  IT_CUDA(cudaSetDevice(ctx->device));
+  p.sx = x_scales;
+  p.sw = w_scales;
+  p.out.is_f32 = out_dtype == IT_F32;
+  p.M = n;
+  p.N = out_dim;
+  p.K = in_dim;
+  p.status = ctx->d_status;
+  return launch_gemm_i8<128, 1>(ctx, stream->s, x_codes, w_codes, p);
+}

@@ -151,7 +151,7 @@ __device__ __forceinline__ void rope_fill_table(float2* table, int S, int half, 
     table[i] = make_float2(c, s);
   }
 }
-__global__ void rope_table_kernel(float2* __restrict__ table, int S, int half, const __grid_constant__ RopeFreqs freqs) {
+static __global__ void rope_table_kernel(float2* __restrict__ table, int S, int half, const __grid_constant__ RopeFreqs freqs) {
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
   rope_fill_table(table, S, half, freqs, static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x,

@@ -1,0 +1,74 @@
+// Rotary embedding at positions given per token, on one or several axes (time, height and width of image and video tokens; the
+// lengths of a ragged batch's sequences), and its inverse.
+//
+// Dimension pair i turns by   angle = positions[axis(i)][token] * f(i)   as in rope.cuh: (x0, x1) -> (x0 cos - x1 sin, x0 sin + x1 cos).
+// The inverse turns back and is the gradient.  The pairs of a head are cut into one section per axis; f(i) and axis(i) come from
+// the host.
+// Angles are in 64 bits: at position 200000 an angle in 32 bits, as rope.cuh has it, is off by up to 0.01, which is 2^-7 of a
+// result; here the whole turns are taken off in 64 bits and the rest of at most pi, then rounded to 32, is off by 2^-24 of itself.
+#pragma once
+#include <cuda_bf16.h>
+
+#include <cstdint>
+
+#include "rope.cuh"
+#include "sm100_ptx.cuh"
+
+namespace it {
+
+struct RopeAxes {
+  double freq[64];      // f(i), i < head_dim / 2
+  uint8_t axis[64];
+};
+
+// (cos, sin) of position * freq.  |position| < 2^31 and freq is at most a few: up to 2^30 whole turns, so the turn is given in two
+// parts and the product with its first is exact in the fma.
+__device__ __forceinline__ float2 rope_turn(int position, double freq) {
+  const double a = static_cast<double>(position) * freq;
+  const double n = rint(a * 0.15915494309189535);            // 1 / (2 pi)
+  double r = fma(-n, 6.283185307179586, a);
+  r = fma(-n, 2.4492935982947064e-16, r);                    // 2 pi - its first part
+  float s, c;
+  sincosf(static_cast<float>(r), &s, &c);
+  return make_float2(c, s);
+}
+
+// A CTA owns n_pos tokens: one sine per thread into shared memory, then the heads of q and k in 16-byte chunks (see
+// rope_qk_chunks_kernel).  VEC: elements of a chunk; 2 where rows are not whole chunks.
+template <typename ST, int VEC>
+__global__ void __launch_bounds__(256)
+rope_positions_kernel(const ST* q_in, const ST* k_in, ST* q_out, ST* k_out, const int* __restrict__ positions, long long rows, int n_pos,
+                      int H, int Hkv, int D, int inverse, const __grid_constant__ RopeAxes axes) {
+  __shared__ float2 tab[256];
+  struct alignas(VEC * sizeof(ST)) Chunk { ST e[VEC]; };
+  const int half = D >> 1, per_head = D / VEC, n_heads = H + Hkv;
+  const long long row0 = static_cast<long long>(blockIdx.x) * n_pos;
+  const int n_rows = static_cast<int>(min(static_cast<long long>(n_pos), rows - row0));
+  const int n_chunks = n_rows * n_heads * per_head;
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch();
+  for (int t = static_cast<int>(threadIdx.x); t < n_rows * half; t += 256) {
+    const int r = t / half, pair = t - r * half;
+    float2 cs = rope_turn(positions[axes.axis[pair] * rows + row0 + r], axes.freq[pair]);
+    if (inverse) cs.y = -cs.y;
+    tab[t] = cs;
+  }
+  __syncthreads();
+  for (int i = static_cast<int>(threadIdx.x); i < n_chunks; i += 256) {
+    const int head_row = i / per_head, d = (i - head_row * per_head) * VEC;
+    const int r = head_row / n_heads, hh = head_row - r * n_heads;
+    const bool is_q = hh < H;
+    const long long off = (is_q ? (row0 + r) * H + hh : (row0 + r) * Hkv + (hh - H)) * D + d;
+    Chunk x = *reinterpret_cast<const Chunk*>((is_q ? q_in : k_in) + off);
+    const float2* cs = &tab[r * half + (d >> 1)];
+#pragma unroll
+    for (int p = 0; p < VEC / 2; ++p) {
+      const float x0 = rope_ld(&x.e[2 * p]), x1 = rope_ld(&x.e[2 * p + 1]);
+      rope_st(&x.e[2 * p], x0 * cs[p].x - x1 * cs[p].y);
+      rope_st(&x.e[2 * p + 1], x0 * cs[p].y + x1 * cs[p].x);
+    }
+    *reinterpret_cast<Chunk*>((is_q ? q_out : k_out) + off) = x;
+  }
+}
+
+}  // namespace it

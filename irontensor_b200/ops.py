@@ -734,6 +734,216 @@ def attention_backward_recompute(grad_output, q, k, v, o=None, lse=None, causal=
     return dq, dk, dv
 
 
+def _on_current_device(*tensors):
+    """Refuses torch tensors that the kernels of the current device cannot address, or not as packed rows."""
+    device = _torch().cuda.current_device()
+    for t in tensors:
+        assert t.is_cuda and t.get_device() == device, f"tensors must be on the current CUDA device {device}, got one on {t.device}"
+        assert t.is_contiguous(), "tensors must be contiguous"
+
+
+def _int32(t, shape, name):
+    import torch
+    assert isinstance(t, torch.Tensor) and t.dtype is torch.int32, f"{name} must be a torch tensor of type int32"
+    assert list(t.shape) == list(shape), f"{name} must have the shape {list(shape)}, got {list(t.shape)}"
+    return t
+
+
+def rope_positions(q, k, positions, base=10000.0, sections=None, per_axis=False, inverse=False):
+    """rope_qk at positions given per token: q [batch, seq, heads, head_dim], k [batch, seq, kv_heads, head_dim] (or None: q alone
+    is returned), positions a torch tensor of int32, [batch, seq], or [axes, batch, seq] for tokens that stand on several axes
+    (time, height and width in a video).  Sequences of a batch that stand at different lengths are one axis.
+
+    `sections` says how many of the head_dim / 2 dimension pairs turn by each axis, in order (None: all by the one axis).  Pair i turns
+    by position * base^(-2i / head_dim); with `per_axis`, the j-th of an axis's n pairs by position * base^(-j / n).  Angles are
+    in 64 bits: far positions keep their digits.  `inverse` turns back, which is the gradient."""
+    p = q.precision()
+    assert len(q.shape()) == 4, "q must be 4D [batch, seq, heads, head_dim]"
+    B, S, H, D = q.shape()
+    assert D % 2 == 0 and D <= 128, "head_dim must be even and <= 128"
+    Hkv = 0
+    if k is not None:
+        assert len(k.shape()) == 4 and k.precision() is p, "k must be 4D and have the precision of q"
+        Hkv = k.shape()[2]
+        assert k.shape() == [B, S, Hkv, D], "k must be [batch, seq, kv_heads, head_dim]"
+    axes = positions.shape[0] if positions.dim() == 3 else 1
+    _int32(positions, [axes, B, S] if positions.dim() == 3 else [B, S], "positions")
+    if sections is None:
+        assert axes == 1, "several axes need their sections"
+        sections = [D // 2]
+    assert len(sections) == axes and 1 <= axes <= 4, "1 to 4 axes, one section for each"
+    assert all(n >= 0 for n in sections) and sum(sections) == D // 2, "sections must add up to head_dim / 2"
+    _on_current_device(q.torch(), positions, *([] if k is None else [k.torch()]))
+    qo = Tensor.empty([B, S, H, D], p)
+    ko = None if k is None else Tensor.empty([B, S, Hkv, D], p)
+    c = context()
+    _lib.check(c.lib.it_rope_positions(c.handle, c.stream(), _dtype_code(p), B, S, H, Hkv, D, float(base), axes,
+                                       (ctypes.c_int32 * axes)(*sections), int(per_axis), int(inverse), positions.data_ptr(), q.data_ptr(),
+                                       None if k is None else k.data_ptr(), qo.data_ptr(), None if k is None else ko.data_ptr()))
+    return qo if k is None else (qo, ko)
+
+
+class QuantizedCache:
+    """A key/value cache in 4 bits: 32 neighbouring columns of a head share a scale, and a value is scale * c with a whole number c in
+    -7..7.  4.5 bits a value where head_dim is a multiple of 32; the form is described at it_kv_cache_q4_append.
+
+    codes: uint8 [2, batch, kv_heads, max_len, 16 * groups] and scales: bfloat16 [2, batch, kv_heads, max_len, groups], keys first,
+    groups = ceil(head_dim / 32).  The object holds these two torch tensors and nothing else; how many positions of each sequence
+    are valid is the caller's, an int32 tensor [batch] on the device, as kv_len is for attention_decode."""
+
+    __slots__ = ("codes", "scales", "head_dim")
+
+    def __init__(self, codes, scales, head_dim):
+        import torch
+        assert 8 <= head_dim <= 128 and head_dim % 8 == 0, "head_dim must be a multiple of 8 in 8..128"
+        groups = -(-head_dim // 32)
+        assert codes.dtype is torch.uint8 and codes.dim() == 5 and codes.shape[0] == 2 and codes.shape[4] == 16 * groups, \
+            f"codes must be uint8 [2, batch, kv_heads, max_len, {16 * groups}]"
+        assert scales.dtype is torch.bfloat16 and scales.shape == codes.shape[:4] + (groups,), \
+            f"scales must be bfloat16 [2, batch, kv_heads, max_len, {groups}], like the codes"
+        assert codes.shape[2] >= 1 and codes.shape[3] >= 1, "kv_heads and max_len must be positive"
+        self.codes, self.scales, self.head_dim = codes, scales, head_dim
+
+    @staticmethod
+    def zeros(batch, max_len, kv_heads, head_dim):
+        torch = _torch()
+        groups = -(-head_dim // 32)
+        return QuantizedCache(torch.full((2, batch, kv_heads, max_len, 16 * groups), 0x88, dtype=torch.uint8, device="cuda"),
+                              torch.zeros((2, batch, kv_heads, max_len, groups), dtype=torch.bfloat16, device="cuda"), head_dim)
+
+    def shape(self):
+        """[batch, max_len, kv_heads, head_dim], as the caches of attention_decode have it."""
+        _, B, Hkv, max_len, _ = self.codes.shape
+        return [B, max_len, Hkv, self.head_dim]
+
+    def byte_size(self):
+        return self.codes.numel() + 2 * self.scales.numel()
+
+    def _halves(self):
+        """Addresses of the keys' codes and scales and of the values'."""
+        _on_current_device(self.codes, self.scales)
+        k, ks = self.codes.data_ptr(), self.scales.data_ptr()
+        return k, ks, k + self.codes.numel() // 2, ks + self.scales.numel()
+
+
+def kv_cache_append(cache, k, v, lengths, counts=None):
+    """Quantises new tokens into a QuantizedCache: k, v [batch, tokens, kv_heads, head_dim] (rotated, as attention_decode's caches hold
+    them) go behind the first lengths[b] positions of each sequence; with `counts`, of sequence b only its first counts[b] tokens
+    (prompts padded to one length).  Returns the new lengths, an int32 tensor [batch].
+
+    lengths and counts are int32 tensors [batch] on the device and read there, so that the call can be captured in a CUDA graph.  A
+    token that does not fit into max_len positions is dropped and reported when the stream is next synchronised (ITError)."""
+    p = k.precision()
+    B, max_len, Hkv, D = cache.shape()
+    assert v.precision() is p and k.shape() == v.shape(), "k and v must have the same shape and precision"
+    assert len(k.shape()) == 4 and k.shape() == [B, k.shape()[1], Hkv, D], "k and v must be [batch, tokens, kv_heads, head_dim] of the cache"
+    T = k.shape()[1]
+    _int32(lengths, [B], "lengths")
+    if counts is not None:
+        _int32(counts, [B], "counts")
+    halves = cache._halves()
+    _on_current_device(k.torch(), v.torch(), lengths, *([] if counts is None else [counts]))
+    new = lengths.new_empty(B)
+    c = context()
+    _lib.check(c.lib.it_kv_cache_q4_append(c.handle, c.stream(), _dtype_code(p), B, T, Hkv, D, max_len, k.data_ptr(), v.data_ptr(),
+                                           lengths.data_ptr(), None if counts is None else counts.data_ptr(), new.data_ptr(), *halves))
+    return new
+
+
+def kv_cache_read(cache, tokens, starts=None, lengths=None, precision=Precision.BF16):
+    """Positions starts[b] .. starts[b] + tokens - 1 of a QuantizedCache (None: from 0) as k, v [batch, tokens, kv_heads, head_dim]:
+    the very values that attention_decode_quantized works with, exact in BF16.  A position that is negative or not below
+    lengths[b] (None: max_len) gives zeros.  starts and lengths: int32 tensors [batch] on the device."""
+    B, max_len, Hkv, D = cache.shape()
+    assert tokens >= 0, "tokens must not be negative"
+    for t, name in ((starts, "starts"), (lengths, "lengths")):
+        if t is not None:
+            _int32(t, [B], name)
+    halves = cache._halves()
+    _on_current_device(*[t for t in (starts, lengths) if t is not None])
+    k, v = Tensor.empty([B, tokens, Hkv, D], precision), Tensor.empty([B, tokens, Hkv, D], precision)
+    c = context()
+    _lib.check(c.lib.it_kv_cache_q4_read(c.handle, c.stream(), _dtype_code(precision), B, tokens, Hkv, D, max_len, *halves,
+                                         None if starts is None else starts.data_ptr(), None if lengths is None else lengths.data_ptr(),
+                                         k.data_ptr(), v.data_ptr()))
+    return k, v
+
+
+def attention_decode_quantized(q, cache, lengths):
+    """attention_decode against a QuantizedCache, each sequence at its own length: q [batch, heads, head_dim], of sequence b the
+    first lengths[b] positions (the new token's included: kv_cache_append comes first).  lengths: int32 tensor [batch] on the
+    device.  A sequence of length 0 gives zeros.  The result carries `.lse` ([batch, heads]; -inf for an empty sequence)."""
+    p = q.precision()
+    B, max_len, Hkv, D = cache.shape()
+    assert len(q.shape()) == 3 and q.shape() == [B, q.shape()[1], D], "q must be [batch, heads, head_dim] of the cache"
+    H = q.shape()[1]
+    assert H % Hkv == 0, "num_heads must be divisible by num_kv_heads"
+    _int32(lengths, [B], "lengths")
+    halves = cache._halves()
+    _on_current_device(q.torch(), lengths)
+    out = Tensor.empty([B, H, D], p)
+    out.lse = Tensor.empty([B, H], Precision.FP32)
+    n = ctypes.c_size_t()
+    c = context()
+    _lib.check(c.lib.it_attention_decode_q4_workspace_bytes(B, H, D, ctypes.byref(n)))
+    ws = _workspace(n.value)
+    _lib.check(c.lib.it_attention_decode_q4(c.handle, c.stream(), _dtype_code(p), B, H, Hkv, D, max_len, q.data_ptr(), *halves,
+                                            lengths.data_ptr(), out.data_ptr(), out.lse.data_ptr(), ws.data_ptr(), ws.numel()))
+    return out
+
+
+class QuantizedRows:
+    """A matrix in 8-bit integers with a scale per row: row r is scales[r] * codes[r], codes int8 [rows, cols] in -127..127, scales
+    float32 [rows] (torch tensors).  Tokens' activations, or weights [out, in] with a scale per output channel."""
+
+    __slots__ = ("codes", "scales")
+
+    def __init__(self, codes, scales):
+        import torch
+        assert codes.dtype is torch.int8 and codes.dim() == 2, "codes must be int8 [rows, cols]"
+        assert scales.dtype is torch.float32 and list(scales.shape) == [codes.shape[0]], "scales must be float32 [rows]"
+        self.codes, self.scales = codes, scales
+
+    def shape(self):
+        return list(self.codes.shape)
+
+    def to_f32(self):
+        return Tensor(self.codes.float() * self.scales[:, None], self.shape(), Precision.FP32)
+
+
+def quantize_rows(input):
+    """input [rows, cols], FP32 or BF16, as QuantizedRows: a row's scale is its largest magnitude / 127 rounded to 8 significant
+    bits.  For weights once, when they are loaded; for activations in front of linear_int8_forward.  cols: a multiple of 16."""
+    assert len(input.shape()) == 2, "quantize_rows takes [rows, cols]"
+    rows, cols = input.shape()
+    _on_current_device(input.torch())
+    torch = _torch()
+    codes = torch.empty((rows, cols), dtype=torch.int8, device="cuda")
+    scales = torch.empty(rows, dtype=torch.float32, device="cuda")
+    c = context()
+    _lib.check(c.lib.it_quantize_rows_i8(c.handle, c.stream(), _dtype_code(input.precision()), rows, cols, input.data_ptr(), codes.data_ptr(),
+                                         scales.data_ptr()))
+    return QuantizedRows(codes, scales)
+
+
+def linear_int8_forward(input, weight, precision=Precision.BF16, splits=None):
+    """output = input @ weight.T for QuantizedRows: input [n, in] (quantize_rows of the activations), weight [out, in].  Sums are
+    exact, the output is [n, out] of `precision`.  `splits`, up to three widths that add up to out, returns that many tensors of
+    column ranges instead: q, k and v from the stacked weights [Wq; Wk; Wv]."""
+    n, k = input.shape()
+    out_dim, k2 = weight.shape()
+    assert k == k2, "inner dimensions must match"
+    widths = [out_dim] if splits is None else [int(w) for w in splits]
+    assert 1 <= len(widths) <= 3 and all(w >= 0 for w in widths) and sum(widths) == out_dim, "splits: up to three widths that add up to out"
+    _on_current_device(input.codes, input.scales, weight.codes, weight.scales)
+    y = tuple(Tensor.empty([n, w], precision) for w in widths)
+    c = context()
+    _lib.check(c.lib.it_linear_i8_fwd(c.handle, c.stream(), _dtype_code(precision), n, k, out_dim, input.codes.data_ptr(),
+                                      input.scales.data_ptr(), weight.codes.data_ptr(), weight.scales.data_ptr(), len(widths),
+                                      (ctypes.c_int32 * len(widths))(*widths), (ctypes.c_void_p * len(widths))(*[t.data_ptr() for t in y])))
+    return y[0] if splits is None else y
+
+
 class HostAttentionStep:
     """Forward + backward for tensors that live in page-locked HOST memory (it_host_step_* of the C ABI).
 

@@ -1,0 +1,507 @@
+"""GPU parity of the quantised serving operators against their definitions in 64 bits (quant_ref.py).
+
+What is held in 4 or 8 bits is compared bit for bit.  Other results: a rounding to bf16 is off by at most 2^-8 of the value, to
+fp32 by 2^-24."""
+import math
+
+import numpy as np
+import pytest
+
+import quant_ref as qr
+from irontensor_b200 import (Precision, QuantizedCache, QuantizedRows, Tensor, _lib, attention_decode_quantized, attention_gqa, kv_cache_append,
+                             kv_cache_read, linear_int8_forward, quantize_rows, rope_positions, synth)
+
+pytestmark = pytest.mark.gpu
+FP32, BF16 = Precision.FP32, Precision.BF16
+
+
+def ints(a):
+    import torch
+    return torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")
+
+
+def to_tensor(a, precision):
+    a = np.ascontiguousarray(a, np.float32)
+    make = Tensor.from_f32_slice if precision is FP32 else Tensor.from_f32_as_bf16
+    return make(a.reshape(-1), list(a.shape))
+
+
+def values(rng, shape, precision, scale=1.0):
+    x = (rng.standard_normal(shape) * scale).astype(np.float32)
+    return x if precision is FP32 else synth.round_bf16(x).reshape(shape)
+
+
+def cache_of(k, v, max_len, junk=True):
+    """A QuantizedCache [B, max_len] of rows k, v [B, L, Hkv, D] laid out by the checker; positions behind L hold all bits and NaN."""
+    import torch
+    B, L, Hkv, D = k.shape
+    g = -(-D // 32)
+    codes = np.full((2, B, Hkv, max_len, 16 * g), 0xFF if junk else 0x88, np.uint8)
+    scales = np.full((2, B, Hkv, max_len, g), np.nan if junk else 0.0)
+    for i, x in enumerate((k, v)):
+        c, s = qr.q4(x.transpose(0, 2, 1, 3))
+        codes[i, :, :, :L], scales[i, :, :, :L] = qr.q4_bytes(c), s
+    return QuantizedCache(torch.from_numpy(codes).cuda(), torch.from_numpy(scales).to(torch.bfloat16).cuda(), D)
+
+
+def host(cache):
+    return cache.codes.cpu().numpy(), cache.scales.double().cpu().numpy()
+
+
+# ------------------------------------------------------------------------------------------------ writing
+def hard_rows(rng, shape, precision):
+    """Values with ties, zeros, subnormal, huge and non-finite groups among ordinary ones."""
+    x = values(rng, shape, precision)
+    flat = x.reshape(-1, shape[-1])
+    for r in range(flat.shape[0]):
+        kind = r % 12
+        if kind == 1:
+            flat[r] = 0.0
+        elif kind == 2:      # 14 steps: every half of a step is hit
+            flat[r] = rng.integers(-14, 15, shape[-1]) * 2.0 ** int(rng.integers(-20, 20))
+        elif kind == 3:
+            flat[r] *= 2.0 ** -101
+        elif kind == 4:
+            flat[r] = np.sign(flat[r]) * 3.0e38
+        elif kind == 5:
+            flat[r, 0] = np.nan
+        elif kind == 6:
+            flat[r, -1] = -np.inf
+        elif kind == 7:      # one large value
+            flat[r, 3] = 1000.0
+        elif kind == 8:
+            flat[r] = rng.integers(-7, 8, shape[-1]) * 0.5
+        elif kind == 9:
+            flat[r] *= 2.0 ** -90
+    return x if precision is FP32 else synth.round_bf16(x).reshape(shape)
+
+
+@pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B,T,Hkv,D,starts,counts", [
+    (1, 1, 1, 8, [0], None), (3, 1, 2, 64, [0, 5, 19], None), (2, 7, 3, 128, [4, 0], None), (2, 7, 3, 80, [4, 0], [0, 7]),
+    (9, 13, 1, 96, [0, 1, 2, 3, 4, 5, 6, 7, 0], [13, 0, 1, 2, 3, 12, 13, 5, 6]), (2, 20, 4, 32, [0, 0], [20, 19]), (1, 9, 2, 40, [11], None),
+])
+def test_append_writes_the_documented_bytes_and_nothing_else(it_ctx, precision, B, T, Hkv, D, starts, counts):
+    import torch
+    rng = np.random.default_rng(B * 100 + T + D)
+    k, v = hard_rows(rng, (B, T, Hkv, D), precision), hard_rows(rng, (B, T, Hkv, D), precision)
+    max_len, g = 20, -(-D // 32)
+    codes = rng.integers(0, 256, (2, B, Hkv, max_len, 16 * g)).astype(np.uint8)
+    scales = rng.integers(1, 100, (2, B, Hkv, max_len, g)).astype(np.float64)
+    cache = QuantizedCache(torch.from_numpy(codes.copy()).cuda(), torch.from_numpy(scales).to(torch.bfloat16).cuda(), D)
+    new = kv_cache_append(cache, to_tensor(k, precision), to_tensor(v, precision), ints(starts), None if counts is None else ints(counts))
+    assert it_ctx.poll_status() == 0
+    n = [T] * B if counts is None else counts
+    assert new.tolist() == [a + b for a, b in zip(starts, n)]
+    for i, x in enumerate((k, v)):
+        c, s = qr.q4(x)
+        bytes_ = qr.q4_bytes(c)
+        for b in range(B):
+            for t in range(n[b]):
+                codes[i, b, :, starts[b] + t], scales[i, b, :, starts[b] + t] = bytes_[b, t], s[b, t]
+    got_codes, got_scales = host(cache)
+    assert np.array_equal(got_scales, scales, equal_nan=True)
+    assert np.array_equal(got_codes, codes)
+
+
+def test_append_beyond_the_cache_is_dropped_and_reported(it_ctx):
+    """max_len 6: sequence 0 has room for one of two tokens, sequence 1 starts before the cache, sequence 2 behind it, 3 fits."""
+    import torch
+    rng = np.random.default_rng(5)
+    k, v = values(rng, (4, 2, 1, 32), FP32), values(rng, (4, 2, 1, 32), FP32)
+    cache = QuantizedCache.zeros(4, 6, 1, 32)
+    new = kv_cache_append(cache, to_tensor(k, FP32), to_tensor(v, FP32), ints([5, -1, 9, 4]))
+    torch.cuda.synchronize()
+    with pytest.raises(_lib.ITError, match="length lay outside") as e:
+        it_ctx.poll_status()
+    assert e.value.status == _lib.IT_ERR_INVALID_ARG
+    assert it_ctx.poll_status() == 0 and new.tolist() == [6, 1, 6, 6]
+    _, scales = host(cache)
+    written = scales[0, :, 0, :, 0] > 0
+    assert written.tolist() == [[False] * 5 + [True], [True] + [False] * 5, [False] * 6, [False] * 4 + [True] * 2]
+    # counts outside 0..tokens
+    new = kv_cache_append(cache, to_tensor(k, FP32), to_tensor(v, FP32), ints([0, 0, 0, 0]), ints([-3, 5, 2, 0]))
+    torch.cuda.synchronize()
+    with pytest.raises(_lib.ITError, match="length lay outside"):
+        it_ctx.poll_status()
+    assert new.tolist() == [0, 2, 2, 0]
+
+
+@pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B,L,Hkv,D,count,starts,lengths", [
+    (1, 1, 1, 8, 1, None, None), (2, 9, 3, 64, 9, None, None), (3, 17, 2, 80, 5, [0, 12, 16], None), (2, 9, 1, 128, 12, [-2, 5], [9, 7]),
+    (2, 11, 4, 96, 11, None, [0, 20]), (1, 40, 2, 40, 33, [3], [36]),
+])
+def test_read_gives_the_held_values_and_zeros_outside(it_ctx, precision, B, L, Hkv, D, count, starts, lengths):
+    rng = np.random.default_rng(L + D)
+    k, v = values(rng, (B, L, Hkv, D), FP32), values(rng, (B, L, Hkv, D), FP32)
+    cache = cache_of(k, v, L, junk=False)
+    got = kv_cache_read(cache, count, None if starts is None else ints(starts), None if lengths is None else ints(lengths), precision)
+    assert it_ctx.poll_status() == 0
+    for x, y in zip((k, v), got):
+        held, want = qr.q4_values(x), np.zeros((B, count, Hkv, D))
+        for b in range(B):
+            for t in range(count):
+                p = (starts[b] if starts else 0) + t
+                if 0 <= p < min(L, lengths[b] if lengths else L):
+                    want[b, t] = held[b, p]
+        assert y.precision() is precision and np.array_equal(y.to_f32_host(), want)
+
+
+# ------------------------------------------------------------------------------------------------ attention
+def check_decode(it_ctx, precision, q, k, v, lengths, max_len, bound=1.0):
+    """Error against 64 bits on the held values.  A score is a sum of D exact products in fp32, off by at most 2^-20 of the products'
+    magnitudes (16 partial sums of at most 2^-23 each, with room for two); that, through exp, is a relative error of p.  P has 16
+    bits (bf16 q) or 24.  With A = the largest |v|: 2 x 2^-20 x (sum of |q k| / sqrt(D), below 32 here) x A = 2^-14 A, plus 2^-16 A for P
+    and less than 2^-16 A for sums of at most 40 terms a warp and the merges; and the rounding of the result."""
+    cache = cache_of(k, v, max_len)
+    o = attention_decode_quantized(to_tensor(q, precision), cache, ints(lengths))
+    assert it_ctx.poll_status() == 0
+    want, lse = qr.decode(q, qr.q4_values(k), qr.q4_values(v), lengths)
+    got, got_lse = o.to_f32_host(), o.lse.to_f32_host()
+    assert o.precision() is precision and np.isfinite(got).all()
+    A = np.abs(qr.q4_values(v)).max()
+    limit = (2.0 ** -14 + 2.0 ** -16) * A * bound + (2.0 ** -8 if precision is BF16 else 2.0 ** -24) * np.abs(want)
+    assert np.all(np.abs(got - want) <= limit), np.abs(got - want).max()
+    empty = np.asarray(lengths) == 0
+    assert np.all(got[empty] == 0) and np.all(got_lse[empty] == -np.inf)
+    assert np.all(np.abs(got_lse[~empty] - lse[~empty]) <= 2.0 ** -15 * bound + 2.0 ** -23 * np.abs(lse[~empty]))
+    return o, cache
+
+
+@pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("H,Hkv,D,lengths,max_len", [
+    (1, 1, 8, [1], 1), (4, 4, 64, [100], 100), (4, 1, 128, [0, 1, 2, 31, 32, 33, 255, 256, 257], 300), (8, 1, 96, [40, 7], 64),
+    (7, 7, 32, [5, 300], 301), (12, 4, 80, [600, 0, 64], 640), (16, 1, 64, [777], 1024), (24, 2, 128, [90, 1000], 1000), (2, 2, 120, [513], 700),
+    (40, 2, 16, [129, 3], 130), (3, 1, 128, [4001], 8192), (6, 2, 56, [1500, 20, 700], 2048),
+])
+def test_decode_at_every_sequences_own_length(it_ctx, precision, H, Hkv, D, lengths, max_len):
+    rng = np.random.default_rng(D + H + max_len)
+    B, L = len(lengths), max(lengths)
+    q = values(rng, (B, H, D), precision)
+    k, v = values(rng, (B, L, Hkv, D), FP32), values(rng, (B, L, Hkv, D), FP32)
+    check_decode(it_ctx, precision, q, k, v, lengths, max_len)
+
+
+@pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
+def test_decode_of_scales_far_apart(it_ctx, precision):
+    """Values over many powers of two: a scale is taken as it is, and a group of zeros stays zero."""
+    rng = np.random.default_rng(11)
+    H, Hkv, D, lengths = 8, 2, 96, [200, 37]
+    q = values(rng, (2, H, D), precision)
+    k, v = values(rng, (2, 200, Hkv, D), FP32), values(rng, (2, 200, Hkv, D), FP32)
+    k *= 2.0 ** rng.integers(-60, 1, (2, 200, Hkv, 1))
+    v *= 2.0 ** rng.integers(-100, 1, (2, 200, Hkv, 1))
+    k[:, 5], v[:, 6, :, 32:64] = 0.0, 0.0
+    check_decode(it_ctx, precision, q, k, v, lengths, 256)
+    v *= 2.0 ** 100
+    check_decode(it_ctx, precision, q, k, v, lengths, 256)
+
+
+def test_decode_with_one_overwhelming_key(it_ctx):
+    """The maximum arrives late and dwarfs what was summed before it: the result is that key's value alone."""
+    rng = np.random.default_rng(12)
+    q, k, v = values(rng, (1, 4, 64), FP32), values(rng, (1, 900, 1, 64), FP32), values(rng, (1, 900, 1, 64), FP32)
+    q[:] = np.abs(q[:, :1])
+    k[:, 700] = 40.0 * np.sign(q[0, 0])
+    o, _ = check_decode(it_ctx, FP32, q, k, v, [900], 900, bound=64.0)   # scores up to 64 times as large
+    assert np.allclose(o.to_f32_host()[0], qr.q4_values(v)[0, 700, 0], rtol=1e-6, atol=1e-6)
+
+
+def test_non_finite_keys_and_values_reach_their_sequence_only(it_ctx):
+    import torch
+    rng = np.random.default_rng(13)
+    q, k, v = values(rng, (3, 4, 64), BF16), values(rng, (3, 50, 2, 64), BF16), values(rng, (3, 50, 2, 64), BF16)
+    k[0, 10, 0, 3], v[1, 20, 1, 40] = np.nan, np.inf
+    cache = QuantizedCache.zeros(3, 64, 2, 64)
+    n = kv_cache_append(cache, to_tensor(k, BF16), to_tensor(v, BF16), torch.zeros(3, dtype=torch.int32, device="cuda"))
+    o = attention_decode_quantized(to_tensor(q, BF16), cache, n).to_f32_host()
+    assert it_ctx.poll_status() == 0
+    assert np.isnan(o[0, :2]).all() and np.isfinite(o[0, 2:]).all()            # the heads that read K/V head 0
+    assert np.isfinite(o[1, :2]).all() and np.isnan(o[1, 2:, 32:]).all() and np.isfinite(o[1, 2:, :32]).all()   # the group of 32
+    assert np.isfinite(o[2]).all()
+
+
+def test_decode_of_lengths_outside_the_cache(it_ctx):
+    """Taken as the nearest length inside, and reported."""
+    rng = np.random.default_rng(14)
+    q, k, v = values(rng, (2, 2, 32), FP32), values(rng, (2, 70, 1, 32), FP32), values(rng, (2, 70, 1, 32), FP32)
+    cache = cache_of(k, v, 70)
+    import torch
+    o = attention_decode_quantized(to_tensor(q, FP32), cache, ints([1000, -7]))
+    got = o.torch().cpu().numpy()
+    torch.cuda.synchronize()
+    with pytest.raises(_lib.ITError, match="length lay outside"):
+        it_ctx.poll_status()
+    assert it_ctx.poll_status() == 0
+    want, _ = qr.decode(q, qr.q4_values(k), qr.q4_values(v), [70, 0])
+    assert np.abs(got - want).max() <= 2.0 ** -13 * np.abs(v).max() and np.all(got[1] == 0)
+
+
+def test_decode_repeats_bit_for_bit_and_on_other_streams(it_ctx):
+    import torch
+    rng = np.random.default_rng(15)
+    q, k, v = values(rng, (5, 16, 128), BF16), values(rng, (5, 3000, 2, 128), FP32), values(rng, (5, 3000, 2, 128), FP32)
+    lengths = [3000, 1, 0, 2999, 1024]
+    o, cache = check_decode(it_ctx, BF16, q, k, v, lengths, 4096)
+    n, tq = ints(lengths), to_tensor(q, BF16)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(attention_decode_quantized(tq, cache, n))
+    torch.cuda.synchronize()
+    for x in outs:
+        assert torch.equal(x.torch(), o.torch()) and torch.equal(x.lse.torch(), o.lse.torch())
+
+
+def test_cache_offsets_beyond_32_bits(it_ctx):
+    """140 million rows of 64 bytes: the last sequence's and head's rows lie past 2^32 bytes and 2^31 words."""
+    import torch
+    rng = np.random.default_rng(16)
+    B, Hkv, max_len, D, T = 34, 64, 65536, 128, 5
+    cache = QuantizedCache(torch.empty((2, B, Hkv, max_len, 64), dtype=torch.uint8, device="cuda"),
+                           torch.empty((2, B, Hkv, max_len, 4), dtype=torch.bfloat16, device="cuda"), D)
+    assert cache.codes.numel() // 8 > 2 ** 31
+    k, v, q = values(rng, (B, T, Hkv, D), BF16), values(rng, (B, T, Hkv, D), BF16), values(rng, (B, Hkv, D), BF16)
+    starts = torch.zeros(B, dtype=torch.int32, device="cuda")
+    n = kv_cache_append(cache, to_tensor(k, BF16), to_tensor(v, BF16), starts)
+    kr, vr = kv_cache_read(cache, T)
+    o = attention_decode_quantized(to_tensor(q, BF16), cache, n).to_f32_host()
+    far = kv_cache_append(cache, to_tensor(k, BF16), to_tensor(v, BF16), starts + (max_len - T))
+    kf, _ = kv_cache_read(cache, T, starts + (max_len - T))
+    assert it_ctx.poll_status() == 0 and far.tolist() == [max_len] * B
+    hk, hv = qr.q4_values(k), qr.q4_values(v)
+    assert np.array_equal(kr.to_f32_host(), hk) and np.array_equal(vr.to_f32_host(), hv) and np.array_equal(kf.to_f32_host(), hk)
+    want, _ = qr.decode(q[-1:], hk[-1:], hv[-1:], [T])
+    assert np.all(np.abs(o[-1:] - want) <= 2.0 ** -13 * np.abs(hv).max() + 2.0 ** -8 * np.abs(want))
+
+
+# ------------------------------------------------------------------------------------------------ rotary embedding
+@pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B,S,H,Hkv,D,sections,per_axis,base", [
+    (1, 1, 1, 0, 2, [1], False, 10000.0), (3, 5, 4, 2, 64, [32], False, 10000.0), (2, 33, 2, 1, 96, [20, 14, 14], False, 500000.0),
+    (1, 70, 3, 3, 128, [0, 30, 34], True, 10000.0), (2, 7, 5, 1, 10, [2, 3], True, 100.0), (1, 300, 12, 4, 80, [10, 10, 10, 10], False, 10000.0),
+    (40, 1, 32, 8, 128, [64], False, 10000.0),
+])
+def test_rope_at_given_positions(it_ctx, precision, B, S, H, Hkv, D, sections, per_axis, base):
+    """A sine of an angle rounded to 32 bits after whole turns are taken off is off by 2^-23 (angle) and 2^-23 (the function), so a
+    result by 2^-22 (|x0| + |x1|) and two roundings."""
+    rng = np.random.default_rng(D + S)
+    q, k = values(rng, (B, S, H, D), precision), values(rng, (B, S, max(Hkv, 1), D), precision)
+    positions = rng.integers(-2 ** 31, 2 ** 31 - 1, (len(sections), B, S)) if S % 2 else rng.integers(0, 200000, (len(sections), B, S))
+    tq, tk = to_tensor(q, precision), to_tensor(k, precision)
+    at = ints(positions if len(sections) > 1 else positions[0])
+    for inverse in (False, True):
+        got = rope_positions(tq, tk if Hkv else None, at, base, sections, per_axis, inverse)
+        assert it_ctx.poll_status() == 0
+        for x, y in zip((q, k), got if Hkv else (got,)):
+            want = qr.rope(x, positions, float(np.float32(base)), sections, per_axis, inverse)
+            size = np.repeat(np.abs(x[..., 0::2]) + np.abs(x[..., 1::2]), 2, -1)
+            limit = 2.0 ** -21 * size + (2.0 ** -8 if precision is BF16 else 2.0 ** -24) * np.abs(want)
+            assert np.all(np.abs(y.to_f32_host() - want) <= limit)
+
+
+def test_rope_inverse_is_the_gradient(it_ctx):
+    """Against differences: the rotation is linear, so with L = sum(g * rope(x)), dL/dx . d = L(x + d) - L(x) but for rounding."""
+    rng = np.random.default_rng(21)
+    x, g, d = (values(rng, (2, 9, 3, 64), FP32) for _ in range(3))
+    at = ints(rng.integers(0, 5000, (2, 9)))
+    turned = [rope_positions(to_tensor(t, FP32), None, at).to_f32_host().astype(np.float64) for t in (x + d, x)]
+    grad = rope_positions(to_tensor(g, FP32), None, at, inverse=True).to_f32_host().astype(np.float64)
+    diff = (g * (turned[0] - turned[1])).sum()
+    assert abs((grad * d).sum() - diff) <= 2.0 ** -20 * (np.abs(g) * (np.abs(x) + np.abs(d)) * 4).sum()
+
+
+def test_rope_in_place_and_of_odd_addresses(it_ctx):
+    """Rows that start between 16-byte boundaries go in pairs."""
+    import torch
+    rng = np.random.default_rng(22)
+    x = values(rng, (1, 6, 2, 64), BF16)
+    flat = torch.zeros(x.size + 2, dtype=torch.bfloat16, device="cuda")
+    flat[2:] = torch.from_numpy(x.reshape(-1)).to(torch.bfloat16).cuda()
+    at = ints(np.arange(6)[None])
+    a = rope_positions(Tensor(flat[2:], list(x.shape), BF16), None, at)
+    b = rope_positions(to_tensor(x, BF16), None, at)
+    assert it_ctx.poll_status() == 0 and torch.equal(a.torch(), b.torch())
+
+
+# ------------------------------------------------------------------------------------------------ 8-bit projections
+@pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("rows,cols", [(1, 16), (12, 48), (5, 2048), (3, 8192), (25, 8208), (2, 20000)])
+def test_quantize_rows(it_ctx, precision, rows, cols):
+    rng = np.random.default_rng(rows + cols)
+    x = hard_rows(rng, (rows, cols), precision)
+    if rows >= 12:   # ties of 127 steps
+        x[2] = rng.integers(-254, 255, cols)
+        x[2, 0] = 254
+    got = quantize_rows(to_tensor(x, precision))
+    assert it_ctx.poll_status() == 0
+    c, s = qr.q8(x)
+    assert np.array_equal(got.scales.double().cpu().numpy(), s, equal_nan=True)
+    assert np.array_equal(got.codes.cpu().numpy(), c.astype(np.int8))
+
+
+@pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("n,k,widths", [
+    (1, 16, [8]), (3, 48, [24]), (8, 272, [120]), (9, 2048, [200]), (16, 80, [1000]), (17, 528, [16, 8, 16]), (31, 2048, [512, 64, 64]),
+    (33, 144, [200]), (64, 4112, [520]), (130, 272, [9480]), (129, 128, [136, 128]), (700, 208, [4000, 0, 1000]), (2500, 144, [3080]), (300, 1040, [264]),
+])
+def test_linear_int8(it_ctx, precision, n, k, widths):
+    """The integer sums are exact; they become fp32 (2^-24), are multiplied by the product of the scales (2^-24 and, with scales of
+    more than 8 bits as here, 2^-24), and are stored."""
+    import torch
+    rng = np.random.default_rng(n + k)
+    out = sum(widths)
+    cx, cw = rng.integers(-127, 128, (n, k)).astype(np.int8), rng.integers(-127, 128, (out, k)).astype(np.int8)
+    cx[0], cw[0] = 127, 127     # the largest sum
+    sx, sw = rng.uniform(0.5, 2, n).astype(np.float32), rng.uniform(0.5, 2, out).astype(np.float32)
+    x = QuantizedRows(torch.from_numpy(cx).cuda(), torch.from_numpy(sx).cuda())
+    w = QuantizedRows(torch.from_numpy(cw).cuda(), torch.from_numpy(sw).cuda())
+    got = linear_int8_forward(x, w, precision, widths if len(widths) > 1 else None)
+    assert it_ctx.poll_status() == 0
+    want = (cx.astype(np.float64) @ cw.T.astype(np.float64)) * sx[:, None].astype(np.float64) * sw.astype(np.float64)
+    at = 0
+    for width, y in zip(widths, got if len(widths) > 1 else (got,)):
+        part = want[:, at:at + width]
+        at += width
+        assert y.precision() is precision and y.shape() == [n, width]
+        assert np.all(np.abs(y.to_f32_host() - part) <= ((2.0 ** -8 if precision is BF16 else 2.0 ** -24) + 2.0 ** -22) * np.abs(part))
+
+
+def test_linear_int8_of_the_longest_rows(it_ctx):
+    """65536 products of 128 * 128 are 2^30: no sum leaves 32 bits."""
+    import torch
+    x = QuantizedRows(torch.full((2, 65536), -128, dtype=torch.int8, device="cuda"), torch.ones(2, device="cuda"))
+    w = QuantizedRows(torch.full((8, 65536), -128, dtype=torch.int8, device="cuda"), torch.ones(8, device="cuda"))
+    y = linear_int8_forward(x, w, FP32)
+    assert it_ctx.poll_status() == 0 and np.all(y.to_f32_host() == 2.0 ** 30)
+    big = QuantizedRows(torch.zeros((1, 65552), dtype=torch.int8, device="cuda"), torch.ones(1, device="cuda"))
+    with pytest.raises(_lib.ITError, match="in_dim"):
+        linear_int8_forward(big, big)
+
+
+def test_refusals_on_the_device(it_ctx):
+    import torch
+    flat = torch.zeros(4 * 64 + 1, dtype=torch.bfloat16, device="cuda")
+    cache = QuantizedCache.zeros(1, 8, 1, 64)
+    with pytest.raises(_lib.ITError) as e:
+        attention_decode_quantized(Tensor(flat[1:], [1, 4, 64], BF16), cache, ints([1]))
+    assert e.value.status == _lib.IT_ERR_ALIGNMENT
+    with pytest.raises(AssertionError, match="contiguous"):
+        attention_decode_quantized(to_tensor(np.zeros((1, 4, 64)), BF16), QuantizedCache(torch.zeros((2, 1, 8, 2, 32), dtype=torch.uint8, device="cuda").transpose(2, 3),
+                                   torch.zeros((2, 1, 8, 2, 2), dtype=torch.bfloat16, device="cuda").transpose(2, 3), 64), ints([1]))
+    with pytest.raises(AssertionError, match="device"):
+        attention_decode_quantized(to_tensor(np.zeros((1, 4, 64)), BF16), cache, torch.ones(1, dtype=torch.int32))
+    with pytest.raises(_lib.ITError, match="16 columns"):
+        quantize_rows(to_tensor(np.zeros((2, 24)), FP32))
+    x = QuantizedRows(torch.zeros((2, 16), dtype=torch.int8, device="cuda"), torch.zeros(2, device="cuda"))
+    w = QuantizedRows(torch.zeros((12, 16), dtype=torch.int8, device="cuda"), torch.zeros(12, device="cuda"))
+    with pytest.raises(_lib.ITError, match="multiples of 8"):
+        linear_int8_forward(x, w)
+    with pytest.raises(_lib.ITError, match="base"):
+        rope_positions(to_tensor(np.zeros((1, 1, 1, 8)), FP32), None, ints([[0]]), base=-1.0)
+
+
+def test_empty_calls(it_ctx):
+    import torch
+    z = lambda *s: Tensor.zeros(list(s), BF16)
+    cache = QuantizedCache.zeros(2, 8, 1, 64)
+    assert kv_cache_append(cache, z(2, 0, 1, 64), z(2, 0, 1, 64), ints([3, 5])).tolist() == [3, 5]
+    assert kv_cache_read(cache, 0)[0].shape() == [2, 0, 1, 64]
+    none = QuantizedCache.zeros(0, 8, 1, 64)
+    assert attention_decode_quantized(z(0, 4, 64), none, ints([])).shape() == [0, 4, 64]
+    assert attention_decode_quantized(z(2, 0, 64), cache, ints([0, 0])).shape() == [2, 0, 64]
+    assert quantize_rows(z(0, 16)).shape() == [0, 16]
+    e = QuantizedRows(torch.zeros((0, 16), dtype=torch.int8, device="cuda"), torch.zeros(0, device="cuda"))
+    w = QuantizedRows(torch.zeros((8, 16), dtype=torch.int8, device="cuda"), torch.zeros(8, device="cuda"))
+    assert linear_int8_forward(e, w).shape() == [0, 8] and linear_int8_forward(w, e).shape() == [8, 0]
+    assert rope_positions(z(0, 3, 2, 64), None, torch.zeros((0, 3), dtype=torch.int32, device="cuda")).shape() == [0, 3, 2, 64]
+    assert it_ctx.poll_status() == 0
+
+
+# ------------------------------------------------------------------------------------------------ together
+class Layer:
+    """The attention layer of a model served in few bits, with the operators as a user calls them."""
+
+    def __init__(self, rng, hidden, H, Hkv, D):
+        self.H, self.Hkv, self.D, self.hidden = H, Hkv, D, hidden
+        self.w_qkv = quantize_rows(to_tensor(rng.standard_normal(((H + 2 * Hkv) * D, hidden)) * hidden ** -0.5, BF16))
+        self.w_o = quantize_rows(to_tensor(rng.standard_normal((hidden, H * D)) * (H * D) ** -0.5, BF16))
+
+    def projected(self, x, positions):
+        """x [batch, seq, hidden] -> rotated q, k and v."""
+        B, S, _ = x.shape()
+        H, Hkv, D = self.H, self.Hkv, self.D
+        q, k, v = linear_int8_forward(quantize_rows(x.view([B * S, self.hidden])), self.w_qkv, BF16, [H * D, Hkv * D, Hkv * D])
+        q, k = rope_positions(q.view([B, S, H, D]), k.view([B, S, Hkv, D]), positions)
+        return q, k, v.view([B, S, Hkv, D])
+
+    def prompt(self, x, cache, counts):
+        import torch
+        B, S, _ = x.shape()
+        q, k, v = self.projected(x, torch.arange(S, dtype=torch.int32, device="cuda").expand(B, S).contiguous())
+        lengths = kv_cache_append(cache, k, v, torch.zeros_like(counts), counts)
+        return attention_gqa(q, k, v, True), lengths
+
+    def step(self, x, cache, lengths):
+        B = x.shape()[0]
+        q, k, v = self.projected(x, lengths.view(B, 1))
+        new = kv_cache_append(cache, k, v, lengths)
+        o = attention_decode_quantized(q.view([B, self.H, self.D]), cache, new)
+        return linear_int8_forward(quantize_rows(o.view([B, self.H * self.D])), self.w_o), new, (q, o)
+
+
+def test_a_generation_step_of_a_ragged_batch(it_ctx):
+    """Prompts of different lengths, then steps: attention over the cache against 64 bits on the values read back, the layer's output
+    against the dequantised weights, and the rotated q against the reference's rotation at each sequence's own position."""
+    import torch
+    rng = np.random.default_rng(31)
+    B, S, hidden, H, Hkv, D = 4, 70, 256, 8, 2, 64
+    layer, cache, counts = Layer(rng, hidden, H, Hkv, D), QuantizedCache.zeros(B, 96, Hkv, D), [70, 1, 33, 64]
+    x = to_tensor(rng.standard_normal((B, S, hidden)), BF16)
+    _, lengths = layer.prompt(x, cache, ints(counts))
+    assert lengths.tolist() == counts
+    for step in range(3):
+        x = to_tensor(rng.standard_normal((B, 1, hidden)), BF16)
+        y, lengths, (q, o) = layer.step(x, cache, lengths)
+        assert it_ctx.poll_status() == 0 and lengths.tolist() == [c + step + 1 for c in counts]
+        n = max(lengths.tolist())
+        k, v = (t.to_f32_host() for t in kv_cache_read(cache, n, None, lengths, FP32))
+        want, _ = qr.decode(q.view([B, H, D]).to_f32_host(), k, v, lengths.tolist())
+        assert np.all(np.abs(o.to_f32_host() - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -13 * np.abs(v).max())
+        c, s = qr.q8(o.to_f32_host().reshape(B, H * D))
+        full = (c * s[:, None]) @ layer.w_o.to_f32().to_f32_host().astype(np.float64).T
+        # the dequantised weights are rounded to fp32 (2^-24): exact here, 7 + 8 bits
+        assert np.all(np.abs(y.to_f32_host() - full) <= (2.0 ** -8 + 2.0 ** -22) * np.abs(full))
+
+
+def test_a_captured_step_is_replayed_as_the_sequences_grow(it_ctx):
+    """One graph of a step, replayed: lengths live on the device.  Equal, bit for bit, to the same steps called one by one."""
+    import torch
+    rng = np.random.default_rng(32)
+    B, hidden, H, Hkv, D = 3, 128, 4, 2, 32
+    layer = Layer(rng, hidden, H, Hkv, D)
+    xs = [to_tensor(rng.standard_normal((B, 1, hidden)), BF16) for _ in range(5)]
+    eager, lengths, ys = QuantizedCache.zeros(B, 64, Hkv, D), ints([0, 7, 30]), []
+    for x in xs:
+        y, lengths, _ = layer.step(x, eager, lengths)
+        ys.append(y.torch().clone())
+    cache, at = QuantizedCache.zeros(B, 64, Hkv, D), ints([0, 7, 30])
+    x = Tensor(torch.zeros((B, 1, hidden), dtype=torch.bfloat16, device="cuda"), [B, 1, hidden], BF16)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        layer.step(x, QuantizedCache.zeros(B, 64, Hkv, D), at.clone())     # warm
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, new, _ = layer.step(x, cache, at)
+        at.copy_(new)
+    for i, xi in enumerate(xs):
+        x.torch().copy_(xi.torch())
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y.torch(), ys[i]), i
+    assert it_ctx.poll_status() == 0 and at.tolist() == lengths.tolist()
+    assert torch.equal(cache.codes, eager.codes) and torch.equal(cache.scales, eager.scales)
+    del graph
