@@ -482,6 +482,262 @@ PyObject* qkv_rope_forward(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   });
 }
 
+// ------------------------------------------------------------------------------------------------ quantised weights and cache
+struct Ref {   // an owned reference
+  PyObject* o;
+  explicit Ref(PyObject* p) : o(p) {}
+  Ref(const Ref&) = delete;
+  Ref& operator=(const Ref&) = delete;
+  ~Ref() { Py_XDECREF(o); }
+};
+// A packed torch tensor of this type on the current device; the plain case allows no other.
+bool packed(PyObject* o, at::ScalarType type) {
+  if (o == nullptr || !THPVariable_Check(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  return t.scalar_type() == type && t.is_cuda() && t.is_contiguous() && t.get_device() == c10::cuda::current_device();
+}
+// int32 [n] on the current device, or None if that is allowed.  *p: its address, null for None.
+bool int_row(PyObject* o, int64_t n, bool or_none, const int32_t** p) {
+  *p = nullptr;
+  if (or_none && o == Py_None) return true;
+  if (!packed(o, at::kInt)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.dim() != 1 || t.size(0) != n) return false;
+  *p = t.data_ptr<int32_t>();
+  return true;
+}
+bool cache_form(const at::Tensor& c, const at::Tensor& s, int64_t D) {
+  const int64_t g = (D + 31) / 32;
+  return D >= 8 && D <= 128 && D % 8 == 0 && c.scalar_type() == at::kByte && s.scalar_type() == at::kBFloat16 && c.dim() == 5 && s.dim() == 5 &&
+         c.size(0) == 2 && c.size(4) == 16 * g && s.size(4) == g && c.sizes().slice(0, 4) == s.sizes().slice(0, 4) && c.size(2) >= 1 && c.size(3) >= 1 &&
+         c.size(1) <= INT32_MAX && c.size(2) <= INT32_MAX && c.size(3) <= INT32_MAX;
+}
+// The attributes of a QuantizedCache, held while a call uses them.
+struct Cache {
+  Ref codes, scales;
+  int64_t B = 0, Hkv = 0, max_len = 0;
+  int32_t D = 0;
+  const uint8_t* code[2] = {};
+  const char* scale[2] = {};
+  explicit Cache(PyObject* o) : codes(PyObject_GetAttrString(o, "codes")), scales(PyObject_GetAttrString(o, "scales")) {
+    Ref d(PyObject_GetAttrString(o, "head_dim"));
+    PyErr_Clear();   // no such attributes: not a cache, which the Python function says
+    if (d.o == nullptr || !as_int(d.o, &D) || !packed(codes.o, at::kByte) || !packed(scales.o, at::kBFloat16)) return;
+    const at::Tensor &c = THPVariable_Unpack(codes.o), &s = THPVariable_Unpack(scales.o);
+    if (!cache_form(c, s, D) || c.numel() == 0) return;
+    B = c.size(1);
+    Hkv = c.size(2);
+    max_len = c.size(3);
+    code[0] = static_cast<const uint8_t*>(c.data_ptr());
+    code[1] = code[0] + c.numel() / 2;
+    scale[0] = static_cast<const char*>(s.data_ptr());
+    scale[1] = scale[0] + s.numel();   // half of the elements, of two bytes
+  }
+  explicit operator bool() const { return B > 0; }
+  template <typename T>
+  static void* w(const T* p) { return const_cast<void*>(static_cast<const void*>(p)); }
+};
+
+// codes, scales, head_dim: whether they are a QuantizedCache's
+PyObject* is_cache(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  IT_ARGS(3);
+  int32_t D;
+  return PyBool_FromLong(THPVariable_Check(a[0]) && THPVariable_Check(a[1]) && as_int(a[2], &D) &&
+                         cache_form(THPVariable_Unpack(a[0]), THPVariable_Unpack(a[1]), D));
+}
+// codes, scales: whether they are QuantizedRows'
+PyObject* is_rows(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  IT_ARGS(2);
+  if (!THPVariable_Check(a[0]) || !THPVariable_Check(a[1])) Py_RETURN_FALSE;
+  const at::Tensor &c = THPVariable_Unpack(a[0]), &s = THPVariable_Unpack(a[1]);
+  return PyBool_FromLong(c.scalar_type() == at::kChar && c.dim() == 2 && s.scalar_type() == at::kFloat && s.dim() == 1 && s.size(0) == c.size(0));
+}
+
+// q, k (None: q alone), positions, base, sections (None), per_axis, inverse -> (q, k) or q
+PyObject* rope_positions(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  IT_ARGS(7);
+  return guard([&]() -> PyObject* {
+    const bool two = a[1] != Py_None;
+    if (!plain(a[0], 4) || (two && !plain(a[1], 4)) || !packed(a[2], at::kInt)) Py_RETURN_NONE;
+    const at::Tensor &q = ten(a[0]), &at = THPVariable_Unpack(a[2]);
+    const int64_t B = q.size(0), S = q.size(1), H = q.size(2), D = q.size(3);
+    int64_t Hkv = 0;
+    if (two) {
+      const at::Tensor& k = ten(a[1]);
+      Hkv = k.size(2);
+      if (k.scalar_type() != q.scalar_type() || k.size(0) != B || k.size(1) != S || k.size(3) != D) Py_RETURN_NONE;
+    }
+    const int64_t dim = at.dim(), axes = dim == 3 ? at.size(0) : 1;
+    if ((dim != 2 && dim != 3) || axes < 1 || axes > 4 || at.size(dim - 2) != B || at.size(dim - 1) != S || D % 2 != 0 || D > 128) Py_RETURN_NONE;
+    int32_t sections[4] = {static_cast<int32_t>(D / 2)}, sum = 0, per_axis, inverse;
+    if (a[4] != Py_None) {
+      if (!PyList_Check(a[4]) && !PyTuple_Check(a[4])) Py_RETURN_NONE;
+      if (PySequence_Fast_GET_SIZE(a[4]) != axes) Py_RETURN_NONE;
+      for (int i = 0; i < axes; ++i) {
+        if (!as_int(PySequence_Fast_GET_ITEM(a[4], i), &sections[i]) || sections[i] < 0 || sections[i] > 64) Py_RETURN_NONE;
+        sum += sections[i];
+      }
+      if (sum != D / 2) Py_RETURN_NONE;
+    } else if (axes != 1) {
+      Py_RETURN_NONE;
+    }
+    float base;
+    Where w;
+    if (!as_float(a[3], &base) || !as_bool(a[5], &per_axis) || !as_bool(a[6], &inverse)) Py_RETURN_NONE;
+    if (!where(&w)) return nullptr;
+    at::Tensor out[2] = {empty(w, q.sizes(), q.scalar_type()), two ? empty(w, ten(a[1]).sizes(), q.scalar_type()) : at::Tensor()};
+    const void *pq = q.data_ptr(), *pk = two ? ten(a[1]).data_ptr() : nullptr;
+    void *oq = out[0].data_ptr(), *ok = two ? out[1].data_ptr() : nullptr;
+    const int32_t* pos = at.data_ptr<int32_t>();
+    const it_dtype dt = dtype_of(q);
+    if (!call([&] {
+          return it_rope_positions(w.ctx, w.stream, dt, B, S, H, Hkv, D, base, axes, sections, per_axis, inverse, pos, pq, pk, oq, ok);
+        }))
+      return nullptr;
+    return two ? wrap_tuple(out, 2) : wrap(std::move(out[0]));
+  });
+}
+
+// cache, k, v, lengths, counts (None) -> new lengths
+PyObject* kv_cache_append(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  IT_ARGS(5);
+  return guard([&]() -> PyObject* {
+    const Cache c(a[0]);
+    if (!c || !plain(a[1], 4) || !plain(a[2], 4)) Py_RETURN_NONE;
+    const at::Tensor &k = ten(a[1]), &v = ten(a[2]);
+    const int32_t *lengths, *counts;
+    if (!same(k, v) || k.size(0) != c.B || k.size(2) != c.Hkv || k.size(3) != c.D || k.size(1) > INT32_MAX || !int_row(a[3], c.B, false, &lengths) ||
+        !int_row(a[4], c.B, true, &counts))
+      Py_RETURN_NONE;
+    Where w;
+    if (!where(&w)) return nullptr;
+    at::Tensor fresh = empty(w, {c.B}, at::kInt);
+    int32_t* pn = fresh.data_ptr<int32_t>();
+    const void *pk = k.data_ptr(), *pv = v.data_ptr();
+    const int64_t T = k.size(1);
+    const it_dtype dt = dtype_of(k);
+    if (!call([&] {
+          return it_kv_cache_q4_append(w.ctx, w.stream, dt, c.B, T, c.Hkv, c.D, c.max_len, pk, pv, lengths, counts, pn, Cache::w(c.code[0]),
+                                       Cache::w(c.scale[0]), Cache::w(c.code[1]), Cache::w(c.scale[1]));
+        }))
+      return nullptr;
+    return THPVariable_Wrap(std::move(fresh));
+  });
+}
+
+// cache, tokens, starts (None), lengths (None), precision -> (k, v)
+PyObject* kv_cache_read(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  IT_ARGS(5);
+  return guard([&]() -> PyObject* {
+    const Cache c(a[0]);
+    int32_t T;
+    const int32_t *starts, *lengths;
+    if (!c || !as_int(a[1], &T) || T < 1 || !int_row(a[2], c.B, true, &starts) || !int_row(a[3], c.B, true, &lengths) ||
+        (a[4] != g_fp32 && a[4] != g_bf16))
+      Py_RETURN_NONE;
+    Where w;
+    if (!where(&w)) return nullptr;
+    const it_dtype dt = a[4] == g_fp32 ? IT_F32 : IT_BF16;
+    const at::ScalarType type = dt == IT_F32 ? at::kFloat : at::kBFloat16;
+    at::Tensor out[2] = {empty(w, {c.B, T, c.Hkv, c.D}, type), empty(w, {c.B, T, c.Hkv, c.D}, type)};
+    void *pk = out[0].data_ptr(), *pv = out[1].data_ptr();
+    if (!call([&] {
+          return it_kv_cache_q4_read(w.ctx, w.stream, dt, c.B, T, c.Hkv, c.D, c.max_len, c.code[0], c.scale[0], c.code[1], c.scale[1], starts, lengths,
+                                     pk, pv);
+        }))
+      return nullptr;
+    return wrap_tuple(out, 2);
+  });
+}
+
+// q [batch, heads, head_dim], cache, lengths
+PyObject* attention_decode_quantized(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  IT_ARGS(3);
+  return guard([&]() -> PyObject* {
+    const Cache c(a[1]);
+    const int32_t* lengths;
+    if (!c || !plain(a[0], 3) || !int_row(a[2], c.B, false, &lengths)) Py_RETURN_NONE;
+    const at::Tensor& q = ten(a[0]);
+    const int64_t H = q.size(1);
+    if (q.size(0) != c.B || q.size(2) != c.D || H % c.Hkv != 0 || H > INT32_MAX) Py_RETURN_NONE;
+    Where w;
+    size_t ws_bytes = 0;
+    if (!where(&w) || !raise_status(it_attention_decode_q4_workspace_bytes(c.B, H, c.D, &ws_bytes))) return nullptr;
+    at::Tensor o = empty(w, q.sizes(), q.scalar_type()), lse = empty(w, {c.B, H}, at::kFloat), ws = scratch(w, ws_bytes);
+    const void* pq = q.data_ptr();
+    void *po = o.data_ptr(), *pw = ws.data_ptr();
+    float* pl = lse.data_ptr<float>();
+    const it_dtype dt = dtype_of(q);
+    if (!call([&] {
+          return it_attention_decode_q4(w.ctx, w.stream, dt, c.B, H, c.Hkv, c.D, c.max_len, pq, c.code[0], c.scale[0], c.code[1], c.scale[1], lengths,
+                                        po, pl, pw, ws_bytes);
+        }))
+      return nullptr;
+    return wrap_with_lse(std::move(o), std::move(lse));
+  });
+}
+
+// x [rows, cols] -> (codes, scales), torch tensors
+PyObject* quantize_rows(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  IT_ARGS(1);
+  return guard([&]() -> PyObject* {
+    if (!plain(a[0], 2)) Py_RETURN_NONE;
+    const at::Tensor& x = ten(a[0]);
+    const int64_t rows = x.size(0), cols = x.size(1);
+    if (rows > INT32_MAX || cols > INT32_MAX) Py_RETURN_NONE;
+    Where w;
+    if (!where(&w)) return nullptr;
+    at::Tensor codes = empty(w, {rows, cols}, at::kChar), scales = empty(w, {rows}, at::kFloat);
+    const void* px = x.data_ptr();
+    int8_t* pc = codes.data_ptr<int8_t>();
+    float* ps = scales.data_ptr<float>();
+    const it_dtype dt = dtype_of(x);
+    if (!call([&] { return it_quantize_rows_i8(w.ctx, w.stream, dt, rows, cols, px, pc, ps); })) return nullptr;
+    Ref c(THPVariable_Wrap(std::move(codes))), s(THPVariable_Wrap(std::move(scales)));
+    return c.o != nullptr && s.o != nullptr ? PyTuple_Pack(2, c.o, s.o) : nullptr;
+  });
+}
+
+// x codes, x scales, weight codes, weight scales, precision, splits (None) -> y or a tuple
+PyObject* linear_int8_forward(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  IT_ARGS(6);
+  return guard([&]() -> PyObject* {
+    if (!packed(a[0], at::kChar) || !packed(a[1], at::kFloat) || !packed(a[2], at::kChar) || !packed(a[3], at::kFloat)) Py_RETURN_NONE;
+    const at::Tensor &x = THPVariable_Unpack(a[0]), &sx = THPVariable_Unpack(a[1]), &wt = THPVariable_Unpack(a[2]), &sw = THPVariable_Unpack(a[3]);
+    if (x.dim() != 2 || wt.dim() != 2 || x.size(1) != wt.size(1) || sx.numel() != x.size(0) || sw.numel() != wt.size(0) || x.numel() == 0 ||
+        wt.numel() == 0 || (a[4] != g_fp32 && a[4] != g_bf16))
+      Py_RETURN_NONE;
+    const int64_t n = x.size(0), in = x.size(1), out = wt.size(0);
+    if (n > INT32_MAX || in > INT32_MAX || out > INT32_MAX) Py_RETURN_NONE;
+    int32_t widths[3] = {static_cast<int32_t>(out)}, n_outs = 1;
+    if (a[5] != Py_None) {
+      if (!PyList_Check(a[5]) && !PyTuple_Check(a[5])) Py_RETURN_NONE;
+      const Py_ssize_t count = PySequence_Fast_GET_SIZE(a[5]);
+      if (count < 1 || count > 3) Py_RETURN_NONE;
+      n_outs = static_cast<int32_t>(count);
+      int64_t sum = 0;
+      for (int i = 0; i < n_outs; ++i) {
+        if (!as_int(PySequence_Fast_GET_ITEM(a[5], i), &widths[i]) || widths[i] < 0) Py_RETURN_NONE;
+        sum += widths[i];
+      }
+      if (sum != out) Py_RETURN_NONE;
+    }
+    Where w;
+    if (!where(&w)) return nullptr;
+    const it_dtype dt = a[4] == g_fp32 ? IT_F32 : IT_BF16;
+    at::Tensor y[3];
+    void* outs[3] = {};
+    for (int i = 0; i < n_outs; ++i) {
+      y[i] = empty(w, {n, widths[i]}, dt == IT_F32 ? at::kFloat : at::kBFloat16);
+      outs[i] = y[i].data_ptr();
+    }
+    const int8_t *px = x.data_ptr<int8_t>(), *pw = wt.data_ptr<int8_t>();
+    const float *psx = sx.data_ptr<float>(), *psw = sw.data_ptr<float>();
+    if (!call([&] { return it_linear_i8_fwd(w.ctx, w.stream, dt, n, in, out, px, psx, pw, psw, n_outs, widths, outs); })) return nullptr;
+    return a[5] == Py_None ? wrap(std::move(y[0])) : wrap_tuple(y, n_outs);
+  });
+}
+
 // ------------------------------------------------------------------------------------------------ TensorBase
 PyObject* tensor_new(PyTypeObject* type, PyObject*, PyObject*) {
   PyObject* o = type->tp_alloc(type, 0);
@@ -647,6 +903,14 @@ PyMethodDef methods[] = {{"setup", setup, METH_VARARGS, nullptr},
                          IT_FN(linear_forward),
                          IT_FN(linear_backward),
                          IT_FN(qkv_rope_forward),
+                         IT_FN(is_cache),
+                         IT_FN(is_rows),
+                         IT_FN(rope_positions),
+                         IT_FN(kv_cache_append),
+                         IT_FN(kv_cache_read),
+                         IT_FN(attention_decode_quantized),
+                         IT_FN(quantize_rows),
+                         IT_FN(linear_int8_forward),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_ops", "Native host side of the irontensor_b200 ops.", -1, methods};
 

@@ -742,6 +742,11 @@ def _on_current_device(*tensors):
         assert t.is_contiguous(), "tensors must be contiguous"
 
 
+def _c_ints(*values):
+    """Refuses sizes that the C entries' 32-bit arguments would cut off."""
+    assert all(0 <= v < 1 << 31 for v in values), "sizes must be below 2^31"
+
+
 def _int32(t, shape, name):
     import torch
     assert isinstance(t, torch.Tensor) and t.dtype is torch.int32, f"{name} must be a torch tensor of type int32"
@@ -757,6 +762,9 @@ def rope_positions(q, k, positions, base=10000.0, sections=None, per_axis=False,
     `sections` says how many of the head_dim / 2 dimension pairs turn by each axis, in order (None: all by the one axis).  Pair i turns
     by position * base^(-2i / head_dim); with `per_axis`, the j-th of an axis's n pairs by position * base^(-j / n).  Angles are
     in 64 bits: far positions keep their digits.  `inverse` turns back, which is the gradient."""
+    out = _host_ops.rope_positions(q, k, positions, base, sections, per_axis, inverse)
+    if out is not None:
+        return out
     p = q.precision()
     assert len(q.shape()) == 4, "q must be 4D [batch, seq, heads, head_dim]"
     B, S, H, D = q.shape()
@@ -766,8 +774,9 @@ def rope_positions(q, k, positions, base=10000.0, sections=None, per_axis=False,
         assert len(k.shape()) == 4 and k.precision() is p, "k must be 4D and have the precision of q"
         Hkv = k.shape()[2]
         assert k.shape() == [B, S, Hkv, D], "k must be [batch, seq, kv_heads, head_dim]"
-    axes = positions.shape[0] if positions.dim() == 3 else 1
-    _int32(positions, [axes, B, S] if positions.dim() == 3 else [B, S], "positions")
+    _c_ints(B, S, H, Hkv)
+    axes = positions.shape[0] if hasattr(positions, "dim") and positions.dim() == 3 else 1
+    _int32(positions, [B, S] if not hasattr(positions, "dim") or positions.dim() != 3 else [axes, B, S], "positions")
     if sections is None:
         assert axes == 1, "several axes need their sections"
         sections = [D // 2]
@@ -794,6 +803,9 @@ class QuantizedCache:
     __slots__ = ("codes", "scales", "head_dim")
 
     def __init__(self, codes, scales, head_dim):
+        self.codes, self.scales, self.head_dim = codes, scales, head_dim
+        if _host_ops.is_cache(codes, scales, head_dim):
+            return
         import torch
         assert 8 <= head_dim <= 128 and head_dim % 8 == 0, "head_dim must be a multiple of 8 in 8..128"
         groups = -(-head_dim // 32)
@@ -802,7 +814,7 @@ class QuantizedCache:
         assert scales.dtype is torch.bfloat16 and scales.shape == codes.shape[:4] + (groups,), \
             f"scales must be bfloat16 [2, batch, kv_heads, max_len, {groups}], like the codes"
         assert codes.shape[2] >= 1 and codes.shape[3] >= 1, "kv_heads and max_len must be positive"
-        self.codes, self.scales, self.head_dim = codes, scales, head_dim
+        _c_ints(*codes.shape)
 
     @staticmethod
     def zeros(batch, max_len, kv_heads, head_dim):
@@ -833,11 +845,15 @@ def kv_cache_append(cache, k, v, lengths, counts=None):
 
     lengths and counts are int32 tensors [batch] on the device and read there, so that the call can be captured in a CUDA graph.  A
     token that does not fit into max_len positions is dropped and reported when the stream is next synchronised (ITError)."""
+    new = _host_ops.kv_cache_append(cache, k, v, lengths, counts)
+    if new is not None:
+        return new
     p = k.precision()
     B, max_len, Hkv, D = cache.shape()
     assert v.precision() is p and k.shape() == v.shape(), "k and v must have the same shape and precision"
     assert len(k.shape()) == 4 and k.shape() == [B, k.shape()[1], Hkv, D], "k and v must be [batch, tokens, kv_heads, head_dim] of the cache"
     T = k.shape()[1]
+    _c_ints(T)
     _int32(lengths, [B], "lengths")
     if counts is not None:
         _int32(counts, [B], "counts")
@@ -854,8 +870,12 @@ def kv_cache_read(cache, tokens, starts=None, lengths=None, precision=Precision.
     """Positions starts[b] .. starts[b] + tokens - 1 of a QuantizedCache (None: from 0) as k, v [batch, tokens, kv_heads, head_dim]:
     the very values that attention_decode_quantized works with, exact in BF16.  A position that is negative or not below
     lengths[b] (None: max_len) gives zeros.  starts and lengths: int32 tensors [batch] on the device."""
+    out = _host_ops.kv_cache_read(cache, tokens, starts, lengths, precision)
+    if out is not None:
+        return out
     B, max_len, Hkv, D = cache.shape()
     assert tokens >= 0, "tokens must not be negative"
+    _c_ints(tokens)
     for t, name in ((starts, "starts"), (lengths, "lengths")):
         if t is not None:
             _int32(t, [B], name)
@@ -873,6 +893,9 @@ def attention_decode_quantized(q, cache, lengths):
     """attention_decode against a QuantizedCache, each sequence at its own length: q [batch, heads, head_dim], of sequence b the
     first lengths[b] positions (the new token's included: kv_cache_append comes first).  lengths: int32 tensor [batch] on the
     device.  A sequence of length 0 gives zeros.  The result carries `.lse` ([batch, heads]; -inf for an empty sequence)."""
+    out = _host_ops.attention_decode_quantized(q, cache, lengths)
+    if out is not None:
+        return out
     p = q.precision()
     B, max_len, Hkv, D = cache.shape()
     assert len(q.shape()) == 3 and q.shape() == [B, q.shape()[1], D], "q must be [batch, heads, head_dim] of the cache"
@@ -899,10 +922,12 @@ class QuantizedRows:
     __slots__ = ("codes", "scales")
 
     def __init__(self, codes, scales):
+        self.codes, self.scales = codes, scales
+        if _host_ops.is_rows(codes, scales):
+            return
         import torch
         assert codes.dtype is torch.int8 and codes.dim() == 2, "codes must be int8 [rows, cols]"
         assert scales.dtype is torch.float32 and list(scales.shape) == [codes.shape[0]], "scales must be float32 [rows]"
-        self.codes, self.scales = codes, scales
 
     def shape(self):
         return list(self.codes.shape)
@@ -914,8 +939,12 @@ class QuantizedRows:
 def quantize_rows(input):
     """input [rows, cols], FP32 or BF16, as QuantizedRows: a row's scale is its largest magnitude / 127 rounded to 8 significant
     bits.  For weights once, when they are loaded; for activations in front of linear_int8_forward.  cols: a multiple of 16."""
+    out = _host_ops.quantize_rows(input)
+    if out is not None:
+        return QuantizedRows(*out)
     assert len(input.shape()) == 2, "quantize_rows takes [rows, cols]"
     rows, cols = input.shape()
+    _c_ints(rows, cols)
     _on_current_device(input.torch())
     torch = _torch()
     codes = torch.empty((rows, cols), dtype=torch.int8, device="cuda")
@@ -930,9 +959,13 @@ def linear_int8_forward(input, weight, precision=Precision.BF16, splits=None):
     """output = input @ weight.T for QuantizedRows: input [n, in] (quantize_rows of the activations), weight [out, in].  Sums are
     exact, the output is [n, out] of `precision`.  `splits`, up to three widths that add up to out, returns that many tensors of
     column ranges instead: q, k and v from the stacked weights [Wq; Wk; Wv]."""
+    out = _host_ops.linear_int8_forward(input.codes, input.scales, weight.codes, weight.scales, precision, splits)
+    if out is not None:
+        return out
     n, k = input.shape()
     out_dim, k2 = weight.shape()
     assert k == k2, "inner dimensions must match"
+    _c_ints(n, k, out_dim)
     widths = [out_dim] if splits is None else [int(w) for w in splits]
     assert 1 <= len(widths) <= 3 and all(w >= 0 for w in widths) and sum(widths) == out_dim, "splits: up to three widths that add up to out"
     _on_current_device(input.codes, input.scales, weight.codes, weight.scales)
