@@ -5,19 +5,28 @@
 // says 16 is the number 16 + u, and (16 + u) * s - 24 * s = c * s is one fma of two packed values, exact because 24 * s has 7
 // significant bits and c * s at most 8.  So a 32-bit word of eight codes becomes four operand registers by a shift, a mask and an
 // fma each, and everything behind that is bf16 matrix instructions (mma.sync m16n8k16, fp32 sums):
-//   S = Q K^T   rows: up to 8 query heads; B: 8 keys by 16 columns, which lie together in a word of the cache
-//   O = P V     rows: the same heads; B: 16 keys by 8 columns.  A register holds one column of two keys, so two keys' words are
-//               interleaved by halves first (two byte permutes for 16 codes).
-// Eight heads fill half of the 16 rows.  The other half carries the next bits of the same heads' operand: P goes in as the two
-// bf16 terms hi (rows 0-7) and lo (rows 8-15), 16 bits in one instruction, and the two halves of the result are added at the end;
-// an fp32 q likewise, with a third term in an instruction of its own, as has its P.
-// Which key is which column of S, and which column of V is which column of O, is free as long as both products agree: the order
-// is the one in which the words lie (dims_of).
+//   S^T = K Q^T   A: 16 keys by 16 columns, which lie together in a word of the cache; B: the columns of 8 query heads
+//   O^T = V^T P^T A: 16 columns by 16 keys.  A register holds one column of two keys, so two keys' words are interleaved by
+//                 halves first (four byte permutes for 32 codes); B: P of 16 keys and 8 heads, S^T transposed in 8 x 8 tiles
+// with the codes as the larger operand, so that an instruction's 16 rows are all in use whatever the number of heads.
+// P goes in as two bf16 terms, 16 bits; an fp32 q as three terms, as does its P.
+// Which key is which row of S^T, and which column of V is which row of O^T, is free as long as both products agree: the order
+// is the one in which the words lie (q4_dim_of, q4_key_of).
 //
-// A warp walks blocks of 32 keys with an online softmax of its own; warps merge through shared memory, and the ranges of keys
-// that a launch splits a sequence into (even shares of lengths[b], which only the device knows) through a second launch.
+// The work is bound by reading the cache, 144 bytes a position of a K/V head at head_dim 128, and close behind by the instructions
+// that make operands of it: about 2.3 a value, 600 for the 32 keys that a warp takes at a time.  So
+//   * a warp has a ring of three stages of 32 keys in shared memory, filled by asynchronous copies that nobody but it waits for;
+//     no barrier until a CTA's warps merge what they found;
+//   * long caches: a persistent launch (PLAN_EVEN), in which every CTA takes the same number of 32-key units of the whole batch,
+//     whatever the sequences' lengths, which only the device knows: it adds them up and finds its own stretch.  A stretch that
+//     ends inside a sequence leaves its part for fa_decode_q4_merge_kernel.  A CTA has at most two such parts, so the
+//     workspace does not grow with the batch;
+//   * short ones (PLAN_CLUSTER): even shares of a sequence on the 1 to 8 CTAs of a cluster, merged through distributed shared
+//     memory in the same launch, which saves the second one.
 #pragma once
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include <cstdint>
 
@@ -27,7 +36,8 @@
 
 namespace it {
 
-constexpr int DQ_WARPS = 8, DQ_BLOCK = 32, DQ_HEADS = 8, DQ_MAX_SPLITS = 64;
+constexpr int DQ_WARPS = 8, DQ_BLOCK = 32, DQ_STAGES = 3, DQ_MAX_CTAS = 512, DQ_START = 12;
+enum : int { PLAN_CLUSTER = 0, PLAN_EVEN = 1 };
 
 struct DecodeQ4Params {
   const void* q;            // [batch, heads, D]
@@ -36,8 +46,10 @@ struct DecodeQ4Params {
   const int* lengths;
   void* o;
   float *lse, *part_o, *part_ml;
+  int* units;               // PLAN_EVEN: work in front of each sequence [batch + 1], and a CTA's share, for the merge
   int* status;
-  int H, Hkv, D, max_len, n_splits;
+  int B, H, Hkv, D, max_len;
+  int n_splits;             // PLAN_CLUSTER: CTAs of a cluster
   float scale_log2;         // 1/sqrt(D) * log2(e)
 };
 
@@ -51,233 +63,721 @@ __device__ __forceinline__ uint32_t q4_mul2(uint32_t a, uint32_t b) {
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
+// (x & MASK) | magic in one instruction.  It takes one constant in itself and no second one, so `magic` comes in a register; left to
+// itself the compiler makes two instructions of it, and this unit is what the kernel waits for.
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t q4_and_or(uint32_t x, uint32_t magic) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "n"(MASK), "r"(magic));
+  return d;
+}
+__device__ __forceinline__ uint32_t q4_constant(uint32_t c) {   // one that the compiler does not see through
+  uint32_t d;
+  asm volatile("mov.b32 %0, %1;" : "=r"(d) : "r"(c));
+  return d;
+}
 // Nibble I of both halves of w as the values (16 + u) s - 24 s.
 template <int I>
-__device__ __forceinline__ uint32_t q4_pair(uint32_t w, uint32_t s2, uint32_t bias2) {
+__device__ __forceinline__ uint32_t q4_pair(uint32_t w, uint32_t s2, uint32_t bias2, uint32_t magic) {
   const uint32_t at3 = I == 0 ? w << 3 : w >> (4 * I - 3);
-  return q4_fma2((at3 & 0x00780078u) | 0x41804180u, s2, bias2);
+  return q4_fma2(q4_and_or<0x00780078u>(at3, magic), s2, bias2);
+}
+constexpr uint32_t Q4_MAGIC = 0x41804180u;      // 16 in both halves
+
+// D = A B + C in fp16 with fp32 sums.
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                                              float c0, float c1, float c2, float c3) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ uint32_t q4_add2_f16(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 constexpr uint32_t Q4_MINUS_24 = 0xC1C0C1C0u;   // -24 in both halves
 
-// Which column of a head is n-tile nt's column n of O (see the V operand below).
+// Which column of a head is row r (0 .. 15) of O^T's m-tile mt (see the V operand below).
 template <int NG>
-__device__ __forceinline__ int q4_dim_of(int nt, int n) {
+__device__ __forceinline__ int q4_dim_of(int mt, int r) {
   constexpr int F = NG / 2;
-  int w, e;
-  if (nt < 8 * F) {
-    w = n * F + nt / 8;                  // whole sets of 8 words: lane n owns F consecutive words
-    e = nt % 8;
+  const int n = r & 7;
+  int w, i;
+  if (mt < 4 * F) {
+    w = n * F + mt / 4;                  // whole sets of 8 words: lane n owns F consecutive words
+    i = mt % 4;
   } else {
-    w = 8 * F + (n & 3);                 // the last 4 words, of which lanes 4-7 take the odd columns
-    e = 2 * (nt - 8 * F) + (n >> 2);
+    w = 8 * F + (n & 3);                 // the last 4 words, of which lanes 4-7 take the upper columns
+    i = mt - 4 * F + 2 * (n >> 2);
   }
-  return 32 * (w % NG) + 8 * (w / NG) + e;
+  return 32 * (w % NG) + 8 * (w / NG) + 2 * i + (r >> 3);
 }
 
-// NG: groups of 32 columns; TERMS: bf16 terms of q and P (1: bf16 q, two-term P; 3: fp32 q, three-term P).
-template <int NG, int TERMS>
-__global__ void __launch_bounds__(32 * DQ_WARPS, 1)
-fa_decode_q4_kernel(const DecodeQ4Params prm) {
-  using ST = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
-  constexpr int NT = 4 * NG, F = NG / 2, HALF = NG & 1;   // n-tiles of O; whole sets of 8 words; a set of 4
-  __shared__ float s_acc[DQ_WARPS][DQ_HEADS][32 * NG];
-  __shared__ float s_ml[DQ_WARPS][DQ_HEADS][2];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int G = prm.H / prm.Hkv, chunks = (G + DQ_HEADS - 1) / DQ_HEADS;
-  const int b = blockIdx.z, hk = static_cast<int>(blockIdx.y) / chunks, g0 = (static_cast<int>(blockIdx.y) % chunks) * DQ_HEADS;
-  const int gc = min(DQ_HEADS, G - g0), sp = blockIdx.x, D = prm.D;
-  const size_t bh0 = static_cast<size_t>(b) * prm.H + hk * G + g0;
-  ptx::grid_dep_wait();
-  ptx::grid_dep_launch();
-  const int given = prm.lengths[b], len = min(max(given, 0), prm.max_len);
-  if (given != len && threadIdx.x == 0) atomicCAS(prm.status, 0, DEV_ERR_CACHE_RANGE);
-  const int blocks = (len + DQ_BLOCK - 1) / DQ_BLOCK, share = (blocks + prm.n_splits - 1) / prm.n_splits;
-  const int k_begin = min(sp * share * DQ_BLOCK, len), k_end = min((sp + 1) * share * DQ_BLOCK, len);
+__device__ __forceinline__ uint32_t transposed_8x8(uint32_t x) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
+}
 
-  // q: register 4 j + r holds columns 32 j + 8 t + 2 r and the next, of head g; its further terms for fp32
-  uint32_t qa[TERMS][4 * NG];
+template <int NG>
+struct DecodeQ4Stage {
+  static constexpr int CODES = DQ_BLOCK * 16 * NG;                          // of 32 rows
+  static constexpr int SCALES = (DQ_BLOCK * 2 * NG + 2 + 15) / 16 * 16;     // and up to two bytes in front of them
+  static constexpr int BYTES = 2 * CODES + 2 * SCALES;
+  static constexpr int WARP_BYTES = DQ_STAGES * BYTES;
+  static constexpr int CTA_BYTES = DQ_WARPS * WARP_BYTES;
+};
+
+// Position in the block of a score's column: the n-th of 8 is key n / 2 (n even) or 4 + (n / 2 ^ X).  With the V operand's
+// rows (the keys of columns 2t and 2t + 1) as they then come, loads of both operands are free of bank conflicts.
+template <int NG>
+__device__ __forceinline__ int q4_key_of(int n) {
+  return (n & 1) ? 4 + ((n >> 1) ^ (NG == 2 ? 2 : 1)) : n >> 1;
+}
+// Rows of 64 bytes: 16-byte chunk c of row r lies at chunk c ^ 2 ((r / 2) % 2), see q4_key_of.
+template <int NG>
+__device__ __forceinline__ int q4_chunk(int r, int c) { return NG == 4 ? c ^ ((r & 2)) : c; }
+
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, int bytes) {   // of N bytes; zeros behind `bytes`
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Copies the codes and scales of `n` rows (of which 32 at most) from `first` on of one half of a cache into a stage.  Chunk
+// 32 u + lane of the codes is row 8 u + lane / 4 where rows have four, whose place in the swizzle is the lane's alone.
+template <int NG>
+__device__ __forceinline__ void q4_fetch(uint32_t codes_at, uint32_t scales_at, const uint32_t* codes, const __nv_bfloat16* scales, size_t first,
+                                         int n, int lane) {
+  const char* src = reinterpret_cast<const char*>(codes) + first * (16 * NG) + lane * 16;
+  const uint32_t dst = codes_at + (NG == 4 ? (lane >> 2) * 4 + q4_chunk<4>(lane >> 2, lane & 3) : lane) * 16;
+  if (n >= DQ_BLOCK) {
 #pragma unroll
-  for (int i = 0; i < 4 * NG; ++i) {
-    const int d = 32 * (i >> 2) + 8 * t + 2 * (i & 3);
-    float x0 = 0.f, x1 = 0.f;
-    if (g < gc && d < D) {
-      const ST* src = static_cast<const ST*>(prm.q) + (bh0 + g) * D + d;
-      x0 = rope_ld(src);
-      x1 = rope_ld(src + 1);
-    }
+    for (int u = 0; u < NG; ++u) cp_async_16(dst + u * 512, src + u * 512);
+  } else {
 #pragma unroll
-    for (int n = 0; n < TERMS; ++n) {
-      qa[n][i] = ptx::pack_bf16(x0, x1);
-      x0 -= __uint_as_float(qa[n][i] << 16);
-      x1 -= __uint_as_float(qa[n][i] & 0xFFFF0000u);
-    }
+    for (int u = 0; u < NG; ++u)
+      if (u * 32 + lane < n * NG) cp_async_16(dst + u * 512, src + u * 512);
   }
-  float acc[NT][4], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
+  const char* sc = reinterpret_cast<const char*>(scales) + first * (2 * NG);
+  if constexpr (NG % 2 == 0) {
+    if (lane < n) cp_async_small<2 * NG>(scales_at + lane * 2 * NG, sc + lane * 2 * NG, 2 * NG);
+  } else {   // rows of 2 or 6 bytes: whole words from the boundary in front of the first
+    const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(sc) & 2), bytes = min(n, DQ_BLOCK) * 2 * NG + lead;
+    for (int at = lane * 4; at < bytes; at += 128) cp_async_small<4>(scales_at + at, sc - lead + at, min(4, bytes - at));
+  }
+}
 
-  const size_t row0 = (static_cast<size_t>(b) * prm.Hkv + hk) * prm.max_len;
-  for (int k0 = k_begin + warp * DQ_BLOCK; k0 < k_end; k0 += DQ_WARPS * DQ_BLOCK) {
-    // ---- scores of 4 x 8 keys: lane g's key is the n index, lanes t share its columns
-    float s[4][2];
+// The running softmax and output of one warp, of 8 R query heads.
+template <int NG, int TERMS, int R>
+struct DecodeQ4Warp {
+  static constexpr int MT = 2 * NG;
+  float acc[MT][R][4];   // of m-tile, 8 heads: rows g and g + 8 by heads 2t and 2t + 1
+  // Of heads 2t and 2t + 1: what p is relative to, the score above which that is renewed, and this lane's keys' share of the sum.
+  // p is exp2(score - m) with an m that may lie up to RANGE below the largest score: sums and products keep their relative
+  // precision, and after the first keys a renewal is rare.
+  static constexpr float RANGE = 8.f;   // in the exp2 domain
+  float m[R][2], limit[R][2], l[R][2];
+  // fp32 q: K's values are made in bf16 like V's, and q has three bf16 terms.  bf16 q: K's codes alone are the operand, in fp16,
+  // whose ten bits of mantissa take two nibbles by a mask each: u in the lowest is 1024 + u, less 1032 by an addition; u in the next
+  // is 64 + u, and the 72 times the sum of q that this is too much is what the sums begin with.  A shift by 8 brings the other two.
+  // So a word costs five instructions of the unit that this kernel waits for and not eight; its scale is applied to the sums of its
+  // 32 columns in fp32.  q is scaled by a power of two to a largest magnitude in 1 .. 2 for this (fp16 rounds what is below 2^-14
+  // of the largest, by at most 2^-25 of it).
+  static constexpr bool F16 = TERMS == 1;
+  uint32_t magic, magic0, magic1;
+  uint32_t qb[TERMS][R][4 * NG];    // register 4 j + r: columns 32 j + 8 t + 2 r and the next of head g
+  float init[R][NG][2];             // what the sums of group j begin with, heads 2t and 2t + 1
+  float scale[R][2];                // of the scores of these heads, in the exp2 domain
+
+  __device__ __forceinline__ void begin() {
+    magic = q4_constant(Q4_MAGIC);
+    magic0 = q4_constant(0x64006400u);   // 1024 in fp16
+    magic1 = q4_constant(0x54005400u);   // 64
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const size_t row = row0 + min(k0 + 8 * i + g, k_end - 1);
-      const uint32_t* src = prm.k_codes + row * (4 * NG) + t * NG;
-      uint32_t w[NG];
+    for (int h = 0; h < R; ++h) {
 #pragma unroll
-      for (int j = 0; j < NG; ++j) w[j] = __ldg(src + j);
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        const uint32_t s1 = __ldg(reinterpret_cast<const unsigned short*>(prm.k_scales) + row * NG + j);
-        const uint32_t s2 = __byte_perm(s1, 0, 0x1010), bias2 = q4_mul2(s2, Q4_MINUS_24);
-        const uint32_t b0 = q4_pair<0>(w[j], s2, bias2), b1 = q4_pair<1>(w[j], s2, bias2);
-        const uint32_t b2 = q4_pair<2>(w[j], s2, bias2), b3 = q4_pair<3>(w[j], s2, bias2);
-        if constexpr (TERMS == 1) {
-          mma_bf16_16816(c, qa[0][4 * j], 0u, qa[0][4 * j + 1], 0u, b0, b1);
-          mma_bf16_16816(c, qa[0][4 * j + 2], 0u, qa[0][4 * j + 3], 0u, b2, b3);
-        } else {
-          mma_bf16_16816(c, qa[0][4 * j], qa[1][4 * j], qa[0][4 * j + 1], qa[1][4 * j + 1], b0, b1);
-          mma_bf16_16816(c, qa[0][4 * j + 2], qa[1][4 * j + 2], qa[0][4 * j + 3], qa[1][4 * j + 3], b2, b3);
-          mma_bf16_16816(c, 0u, qa[TERMS - 1][4 * j], 0u, qa[TERMS - 1][4 * j + 1], b0, b1);
-          mma_bf16_16816(c, 0u, qa[TERMS - 1][4 * j + 2], 0u, qa[TERMS - 1][4 * j + 3], b2, b3);
-        }
-      }
+        for (int e = 0; e < 4; ++e) acc[i][h][e] = 0.f;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        s[i][e] = TERMS == 1 ? c[e] : c[e] + c[e + 2];
-        if (k0 + 8 * i + 2 * t + e >= k_end) s[i][e] = -INFINITY;
+        m[h][e] = limit[h][e] = -INFINITY;
+        l[h][e] = 0.f;
       }
     }
-    // ---- online softmax of head g; a lane holds 8 of the 32 keys
-    float mx = m;
+  }
+  // q: the first of the heads; scale_log2 = 1/sqrt(D) * log2(e)
+  template <typename ST>
+  __device__ __forceinline__ void load_q(const ST* q, int heads, int D, float scale_log2, int g, int t) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(s[i][0], s[i][1]));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const float m_ref = mx == -INFINITY ? 0.f : mx * prm.scale_log2;
-    if (__any_sync(0xffffffffu, mx > m)) {
-      const float corr = ptx::ex2(fmaf(m, prm.scale_log2, -m_ref));
-      l *= corr;
+    for (int h = 0; h < R; ++h) {
+      const bool live = 8 * h + g < heads;
+      const ST* row = q + (8 * h + g) * D;
+      if constexpr (F16) {
+        uint32_t largest = 0;
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+        for (int i = 0; i < 4 * NG; ++i) {
+          const int d = 32 * (i >> 2) + 8 * t + 2 * (i & 3);
+          qb[0][h][i] = live && d < D ? *reinterpret_cast<const uint32_t*>(row + d) : 0u;
+          largest = max(largest, max(qb[0][h][i] & 0x7FFFu, (qb[0][h][i] >> 16) & 0x7FFFu));
+        }
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+        // 2^-e for the exponent e of the largest; 1 for zeros and where something is not finite
+        const uint32_t field = largest >> 7;
+        const bool as_is = field == 0 || field == 255;
+        const float down = as_is ? 1.f : __uint_as_float((254u - min(field, 253u)) << 23), up = as_is ? 1.f : __uint_as_float(min(field, 253u) << 23);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][e] *= corr;
-      m = mx;
+        for (int j = 0; j < NG; ++j) {
+          float sum = 0.f;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            uint32_t& x = qb[0][h][4 * j + r];
+            const __half2 y = __floats2half2_rn(__uint_as_float(x << 16) * down, __uint_as_float(x & 0xFFFF0000u) * down);
+            x = *reinterpret_cast<const uint32_t*>(&y);
+            if (r & 1) sum += __low2float(y) + __high2float(y);   // the nibbles that come as 64 + u
+          }
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) init[h][j][e] = -72.f * __shfl_sync(0xffffffffu, sum, 8 * t + 4 * e);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) scale[h][e] = scale_log2 * __shfl_sync(0xffffffffu, up, 8 * t + 4 * e);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4 * NG; ++i) {
+          const int d = 32 * (i >> 2) + 8 * t + 2 * (i & 3);
+          float x0 = 0.f, x1 = 0.f;
+          if (live && d < D) {
+            x0 = rope_ld(row + d);
+            x1 = rope_ld(row + d + 1);
+          }
+#pragma unroll
+          for (int n = 0; n < TERMS; ++n) {
+            qb[n][h][i] = ptx::pack_bf16(x0, x1);
+            x0 -= __uint_as_float(qb[n][h][i] << 16);
+            x1 -= __uint_as_float(qb[n][h][i] & 0xFFFF0000u);
+          }
+        }
+        scale[h][0] = scale[h][1] = scale_log2;
+      }
     }
-    uint32_t hi[4], lo[4], third[4];
+  }
+
+  // `n` keys (at most 32) of the stage at `stage`; k_lead, v_lead: where a row's scales begin, in elements behind the stage's.
+  __device__ __forceinline__ void block(const uint8_t* stage, int n, int k_lead, int v_lead, int g, int t) {
+    using S = DecodeQ4Stage<NG>;
+    const unsigned short* ks = reinterpret_cast<const unsigned short*>(stage + 2 * S::CODES) + k_lead;
+    const unsigned short* vs = reinterpret_cast<const unsigned short*>(stage + 2 * S::CODES + S::SCALES) + v_lead;
+    const int key = q4_key_of<NG>(g);   // in 8; 8 more rows do not change a row's swizzle
+    const uint32_t* k_row = reinterpret_cast<const uint32_t*>(stage) + key * 4 * NG + (NG == 4 ? 4 * q4_chunk<NG>(key, t) : t * NG);
+    const unsigned short* k_scale = ks + key * NG;
+    float s[2][R][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float p0 = ptx::ex2(fmaf(s[i][0], prm.scale_log2, -m_ref)), p1 = ptx::ex2(fmaf(s[i][1], prm.scale_log2, -m_ref));
-      l += p0 + p1;
-      hi[i] = ptx::pack_bf16(p0, p1);
-      p0 -= __uint_as_float(hi[i] << 16);
-      p1 -= __uint_as_float(hi[i] & 0xFFFF0000u);
-      lo[i] = ptx::pack_bf16(p0, p1);
-      if (TERMS > 1) third[i] = ptx::pack_bf16_rest(lo[i], p0, p1);
+    for (int i = 0; i < 2; ++i) {   // 16 keys: rows g and g + 8
+      uint32_t w[2][NG], sc[2][NG];   // a scale in the low half of its register
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int first = 16 * i + 8 * x;
+        const uint32_t* src = k_row + first * 4 * NG;
+        if constexpr (NG == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(src);
+          w[x][0] = v.x, w[x][1] = v.y, w[x][2] = v.z, w[x][3] = v.w;
+          const uint2 u = *reinterpret_cast<const uint2*>(k_scale + first * 4);
+          sc[x][0] = u.x, sc[x][1] = u.x >> 16, sc[x][2] = u.y, sc[x][3] = u.y >> 16;
+        } else if constexpr (NG == 2) {
+          const uint2 v = *reinterpret_cast<const uint2*>(src);
+          w[x][0] = v.x, w[x][1] = v.y;
+          const uint32_t u = *reinterpret_cast<const uint32_t*>(k_scale + first * 2);
+          sc[x][0] = u, sc[x][1] = u >> 16;
+        } else {
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            w[x][j] = src[j];
+            sc[x][j] = k_scale[first * NG + j];
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < R; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i][h][e] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        if constexpr (F16) {
+          constexpr uint32_t LESS = 0xE408E408u;   // -1032 in fp16
+          const uint32_t u0 = w[0][j] >> 8, u1 = w[1][j] >> 8;
+          const uint32_t a0 = q4_add2_f16(q4_and_or<0x000F000Fu>(w[0][j], magic0), LESS), a1 = q4_add2_f16(q4_and_or<0x000F000Fu>(w[1][j], magic0), LESS);
+          const uint32_t a2 = q4_and_or<0x00F000F0u>(w[0][j], magic1), a3 = q4_and_or<0x00F000F0u>(w[1][j], magic1);
+          const uint32_t a4 = q4_add2_f16(q4_and_or<0x000F000Fu>(u0, magic0), LESS), a5 = q4_add2_f16(q4_and_or<0x000F000Fu>(u1, magic0), LESS);
+          const uint32_t a6 = q4_and_or<0x00F000F0u>(u0, magic1), a7 = q4_and_or<0x00F000F0u>(u1, magic1);
+          const float f0 = __uint_as_float(sc[0][j] << 16), f1 = __uint_as_float(sc[1][j] << 16);
+#pragma unroll
+          for (int h = 0; h < R; ++h) {
+            float d[4];
+            mma_f16_16816(d, a0, a1, a2, a3, qb[0][h][4 * j], qb[0][h][4 * j + 1], init[h][j][0], init[h][j][1], init[h][j][0], init[h][j][1]);
+            mma_f16_16816(d, a4, a5, a6, a7, qb[0][h][4 * j + 2], qb[0][h][4 * j + 3], d[0], d[1], d[2], d[3]);
+            s[i][h][0] = fmaf(f0, d[0], s[i][h][0]);
+            s[i][h][1] = fmaf(f0, d[1], s[i][h][1]);
+            s[i][h][2] = fmaf(f1, d[2], s[i][h][2]);
+            s[i][h][3] = fmaf(f1, d[3], s[i][h][3]);
+          }
+        } else {
+          const uint32_t s0 = __byte_perm(sc[0][j], 0, 0x1010), s1 = __byte_perm(sc[1][j], 0, 0x1010);
+          const uint32_t bias0 = q4_mul2(s0, Q4_MINUS_24), bias1 = q4_mul2(s1, Q4_MINUS_24);
+          const uint32_t a0 = q4_pair<0>(w[0][j], s0, bias0, magic), a1 = q4_pair<0>(w[1][j], s1, bias1, magic);
+          const uint32_t a2 = q4_pair<1>(w[0][j], s0, bias0, magic), a3 = q4_pair<1>(w[1][j], s1, bias1, magic);
+          const uint32_t a4 = q4_pair<2>(w[0][j], s0, bias0, magic), a5 = q4_pair<2>(w[1][j], s1, bias1, magic);
+          const uint32_t a6 = q4_pair<3>(w[0][j], s0, bias0, magic), a7 = q4_pair<3>(w[1][j], s1, bias1, magic);
+#pragma unroll
+          for (int h = 0; h < R; ++h)
+#pragma unroll
+            for (int x = TERMS - 1; x >= 0; --x) {
+              mma_bf16_16816(s[i][h], a0, a1, a2, a3, qb[x][h][4 * j], qb[x][h][4 * j + 1]);
+              mma_bf16_16816(s[i][h], a4, a5, a6, a7, qb[x][h][4 * j + 2], qb[x][h][4 * j + 3]);
+            }
+        }
+      }
     }
-    // ---- O += P V, 16 keys at a time: registers of keys (2t, 2t + 1) and (2t + 8, 2t + 9)
+    if (n < DQ_BLOCK) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      size_t rows[4];
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int n = 0; n < 4; ++n) rows[n] = row0 + min(k0 + 16 * h + 2 * t + (n & 1) + 8 * (n >> 1), k_end - 1);
-      auto product = [&](int nt, uint32_t b0, uint32_t b1) {
-        mma_bf16_16816(acc[nt], hi[2 * h], lo[2 * h], hi[2 * h + 1], lo[2 * h + 1], b0, b1);
-        if (TERMS > 1) mma_bf16_16816(acc[nt], third[2 * h], 0u, third[2 * h + 1], 0u, b0, b1);
-      };
+        for (int e = 0; e < 4; ++e)
+          if (16 * i + 8 * (e >> 1) + key >= n)
+#pragma unroll
+            for (int h = 0; h < R; ++h) s[i][h][e] = -INFINITY;
+    }
+    // online softmax; a lane holds 4 of the 32 keys of each of its two heads
+    uint32_t p[TERMS == 1 ? 2 : 3][R][4];   // terms of P, transposed: register x of keys 8x .. 8x + 7
+#pragma unroll
+    for (int h = 0; h < R; ++h) {
+      float mx[2], m_ref[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) mx[e] = fmaxf(ptx::fmax3(s[0][h][e], s[0][h][e + 2], s[1][h][e]), s[1][h][e + 2]);
+      if (__any_sync(0xffffffffu, mx[0] > limit[h][0] || mx[1] > limit[h][1])) {
+        float corr[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          mx[e] = fmaxf(mx[e], m[h][e]);
+          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 4));
+          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 8));
+          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 16));
+          corr[e] = mx[e] > m[h][e] ? ptx::ex2((m[h][e] - mx[e]) * scale[h][e]) : 1.f;
+          l[h][e] *= corr[e];
+          m[h][e] = mx[e];
+          limit[h][e] = mx[e] + RANGE / scale[h][e];
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][h][e] *= corr[e & 1];
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) m_ref[e] = m[h][e] == -INFINITY ? 0.f : m[h][e] * scale[h][e];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float p0 = ptx::ex2(fmaf(s[x >> 1][h][2 * (x & 1)], scale[h][0], -m_ref[0]));
+        float p1 = ptx::ex2(fmaf(s[x >> 1][h][2 * (x & 1) + 1], scale[h][1], -m_ref[1]));
+        l[h][0] += p0;
+        l[h][1] += p1;
+#pragma unroll
+        for (int y = 0; y < (TERMS == 1 ? 2 : 3); ++y) {
+          const uint32_t term = ptx::pack_bf16(p0, p1);
+          p0 -= __uint_as_float(term << 16);
+          p1 -= __uint_as_float(term & 0xFFFF0000u);
+          p[y][h][x] = transposed_8x8(term);
+        }
+      }
+    }
+    // O^T += V^T P^T, 16 keys at a time
+    constexpr int F = NG / 2, HALF = NG & 1;   // whole sets of 8 words; a set of 4
+    const uint32_t* v_row[2];
+    const unsigned short* v_scale[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {   // keys 2t and 2t + 1
+      const int row = q4_key_of<NG>(2 * t + x);
+      v_row[x] = reinterpret_cast<const uint32_t*>(stage + S::CODES) + row * 4 * NG + (NG == 4 ? 4 * q4_chunk<NG>(row, g >> 1) + 2 * (g & 1) : 0);
+      v_scale[x] = vs + row * NG + (NG == 4 ? 2 * (g & 1) : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t w[4][F + HALF], sc[4][F + HALF];   // by key (2t, 2t + 1, 2t + 8, 2t + 9) and set of words; scales in the low half
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int first = 16 * i + 8 * (x >> 1);
+        const uint32_t* src = v_row[x & 1] + first * 4 * NG;
+        const unsigned short* scales = v_scale[x & 1] + first * NG;
+        if constexpr (NG == 4) {
+          const uint2 v = *reinterpret_cast<const uint2*>(src);
+          w[x][0] = v.x, w[x][1] = v.y;
+          const uint32_t u = *reinterpret_cast<const uint32_t*>(scales);
+          sc[x][0] = u, sc[x][1] = u >> 16;
+        } else {
+#pragma unroll
+          for (int f = 0; f < F + HALF; ++f) {
+            const int word = f < F ? g * F + f : 8 * F + (g & 3);
+            w[x][f] = src[word];
+            if (f >= F) w[x][f] >>= 8 * (g >> 2);   // lanes 4-7: the upper two nibbles of each half
+            sc[x][f] = scales[word % NG];
+          }
+        }
+      }
 #pragma unroll
       for (int f = 0; f < F + HALF; ++f) {
-        const bool whole = f < F;
-        const int word = whole ? g * F + f : 8 * F + (g & 3);
-        uint32_t w[4], s2[2], bias2[2];
+        uint32_t s2[2], bias2[2], lo[2], hi[2];   // the low halves of two keys' words are even columns, the high halves odd ones
 #pragma unroll
-        for (int n = 0; n < 4; ++n) w[n] = __ldg(prm.v_codes + rows[n] * (4 * NG) + word);
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const unsigned short* sc = reinterpret_cast<const unsigned short*>(prm.v_scales);
-          s2[n] = __byte_perm(__ldg(sc + rows[2 * n] * NG + word % NG), __ldg(sc + rows[2 * n + 1] * NG + word % NG), 0x5410);
-          bias2[n] = q4_mul2(s2[n], Q4_MINUS_24);
+        for (int x = 0; x < 2; ++x) {
+          s2[x] = __byte_perm(sc[2 * x][f], sc[2 * x + 1][f], 0x5410);
+          bias2[x] = q4_mul2(s2[x], Q4_MINUS_24);
+          lo[x] = __byte_perm(w[2 * x][f], w[2 * x + 1][f], 0x5410);
+          hi[x] = __byte_perm(w[2 * x][f], w[2 * x + 1][f], 0x7632);
         }
+        auto product = [&](int mt, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
-        for (int odd = 0; odd < 2; ++odd) {   // the low halves of two keys' words: even columns; the high halves: odd ones
-          if (!whole && odd == 1) break;
-          const uint32_t sel = whole ? (odd ? 0x7632u : 0x5410u) : (g & 4 ? 0x7632u : 0x5410u);
-          const uint32_t a = __byte_perm(w[0], w[1], sel), c = __byte_perm(w[2], w[3], sel);
-          const int nt = whole ? 8 * f + odd : 8 * F, step = whole ? 2 : 1;
-          product(nt, q4_pair<0>(a, s2[0], bias2[0]), q4_pair<0>(c, s2[1], bias2[1]));
-          product(nt + step, q4_pair<1>(a, s2[0], bias2[0]), q4_pair<1>(c, s2[1], bias2[1]));
-          product(nt + 2 * step, q4_pair<2>(a, s2[0], bias2[0]), q4_pair<2>(c, s2[1], bias2[1]));
-          product(nt + 3 * step, q4_pair<3>(a, s2[0], bias2[0]), q4_pair<3>(c, s2[1], bias2[1]));
+          for (int h = 0; h < R; ++h)
+#pragma unroll
+            for (int y = (TERMS == 1 ? 1 : 2); y >= 0; --y) mma_bf16_16816(acc[mt][h], a0, a1, a2, a3, p[y][h][2 * i], p[y][h][2 * i + 1]);
+        };
+        product(4 * f, q4_pair<0>(lo[0], s2[0], bias2[0], magic), q4_pair<0>(hi[0], s2[0], bias2[0], magic), q4_pair<0>(lo[1], s2[1], bias2[1], magic),
+                q4_pair<0>(hi[1], s2[1], bias2[1], magic));
+        product(4 * f + 1, q4_pair<1>(lo[0], s2[0], bias2[0], magic), q4_pair<1>(hi[0], s2[0], bias2[0], magic), q4_pair<1>(lo[1], s2[1], bias2[1], magic),
+                q4_pair<1>(hi[1], s2[1], bias2[1], magic));
+        if (f < F) {
+          product(4 * f + 2, q4_pair<2>(lo[0], s2[0], bias2[0], magic), q4_pair<2>(hi[0], s2[0], bias2[0], magic), q4_pair<2>(lo[1], s2[1], bias2[1], magic),
+                  q4_pair<2>(hi[1], s2[1], bias2[1], magic));
+          product(4 * f + 3, q4_pair<3>(lo[0], s2[0], bias2[0], magic), q4_pair<3>(hi[0], s2[0], bias2[0], magic), q4_pair<3>(lo[1], s2[1], bias2[1], magic),
+                  q4_pair<3>(hi[1], s2[1], bias2[1], magic));
         }
       }
     }
   }
-  // ---- merge the warps
-  l += __shfl_xor_sync(0xffffffffu, l, 1);
-  l += __shfl_xor_sync(0xffffffffu, l, 2);
+
+  // What the warp found: its output relative to its maximum, by head and row of O^T, that maximum in the exp2 domain, and the sum.
+  // With PITCH rows a head the 32 lanes' stores lie in different banks.
+  static constexpr int PITCH = 32 * NG + 4;
+  __device__ __forceinline__ void leave(float* out /* [8 R][PITCH] */, float (*ml)[2], int g, int t) {
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+    for (int h = 0; h < R; ++h)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) s_acc[warp][g][q4_dim_of<NG>(nt, 2 * t + e)] = acc[nt][e] + acc[nt][e + 2];
-  if (t == 0) {
-    s_ml[warp][g][0] = m * prm.scale_log2;
-    s_ml[warp][g][1] = l;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < gc * 32 * NG; i += 32 * DQ_WARPS) {
-    const int h = i / (32 * NG), d = i % (32 * NG);
-    float mx = s_ml[0][h][0];
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[h][e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int head = 8 * h + 2 * t + e;
+        if (g == 0) {
+          ml[head][0] = m[h][e] * scale[h][e];
+          ml[head][1] = sum;
+        }
 #pragma unroll
-    for (int w = 1; w < DQ_WARPS; ++w) mx = fmaxf(mx, s_ml[w][h][0]);
-    const float m_ref = mx == -INFINITY ? 0.f : mx;
-    float a = 0.f, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < DQ_WARPS; ++w) {
-      const float f = ptx::ex2(s_ml[w][h][0] - m_ref);
-      a = fmaf(f, s_acc[w][h][d], a);
-      sum = fmaf(f, s_ml[w][h][1], sum);
-    }
-    if (prm.n_splits == 1) {
-      if (d < D) rope_st(static_cast<ST*>(prm.o) + (bh0 + h) * D + d, len > 0 ? a / sum : 0.f);
-      if (d == 0 && prm.lse != nullptr) prm.lse[bh0 + h] = len > 0 ? (mx + log2f(sum)) * 0.6931471805599453f : -INFINITY;
-    } else {
-      const size_t ps = (bh0 + h) * prm.n_splits + sp;
-      if (d < D) prm.part_o[ps * D + d] = a;
-      if (d == 0) {
-        prm.part_ml[ps * 2] = mx;
-        prm.part_ml[ps * 2 + 1] = sum;
+        for (int mt = 0; mt < MT; ++mt) {
+          out[head * PITCH + 16 * mt + g] = acc[mt][h][e];
+          out[head * PITCH + 16 * mt + g + 8] = acc[mt][h][e + 2];
+        }
       }
+  }
+};
+
+// NG: groups of 32 columns; TERMS: bf16 terms of q (1: bf16 q, two-term P; 3: fp32 q, three-term P); HEADS: query heads of a CTA, 8
+// or, in bf16, 16, which share the operands made of the codes.
+// PLAN_CLUSTER: grid (n_splits, kv_heads * chunks, batch), clusters of n_splits.  PLAN_EVEN: any number of CTAs up to DQ_MAX_CTAS.
+template <int NG, int TERMS, int HEADS, int PLAN>
+__global__ void __launch_bounds__(32 * DQ_WARPS, TERMS == 1 && HEADS == 8 ? 2 : 1)
+fa_decode_q4_kernel(const DecodeQ4Params prm) {
+  using ST = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
+  using S = DecodeQ4Stage<NG>;
+  constexpr int COLS = 32 * NG;
+  using Warp = DecodeQ4Warp<NG, TERMS, HEADS / 8>;
+  static_assert(HEADS * Warp::PITCH * 4 <= S::WARP_BYTES, "a warp's output is left in its ring");
+  extern __shared__ __align__(16) uint8_t dq_smem[];
+  __shared__ float s_ml[DQ_WARPS][HEADS][2];
+  __shared__ int s_scan[DQ_WARPS + 2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int G = prm.H / prm.Hkv, chunks = (G + HEADS - 1) / HEADS, per_b = prm.Hkv * chunks, D = prm.D;
+  uint8_t* ring = dq_smem + warp * S::WARP_BYTES;
+  const uint32_t ring_at = ptx::smem_addr(ring);
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch();
+
+  auto length_of = [&](int b) {
+    const int given = prm.lengths[b], len = min(max(given, 0), prm.max_len);
+    if (given != len) atomicCAS(prm.status, 0, DEV_ERR_CACHE_RANGE);
+    return len;
+  };
+  Warp w;
+  // Keys k_begin .. k_end - 1 of (sequence b, pair p of K/V head and head chunk), by all warps; leaves their results in the rings.
+  auto attend = [&](int b, int p, int k_begin, int k_end) {
+    const int hk = p / chunks, g0 = (p % chunks) * HEADS;
+    const size_t row0 = (static_cast<size_t>(b) * prm.Hkv + hk) * prm.max_len;
+    const int mine = k_begin + warp * DQ_BLOCK, step = DQ_WARPS * DQ_BLOCK;
+    int next = mine;
+    uint32_t put = 0;
+    auto fetch = [&] {   // the warp's next block into the next stage
+      const int k0 = next;
+      if (k0 < k_end) {
+        const uint32_t at = ring_at + put;
+        q4_fetch<NG>(at, at + 2 * S::CODES, prm.k_codes, prm.k_scales, row0 + k0, k_end - k0, lane);
+        q4_fetch<NG>(at + S::CODES, at + 2 * S::CODES + S::SCALES, prm.v_codes, prm.v_scales, row0 + k0, k_end - k0, lane);
+      }
+      cp_async_commit();
+      next += step;
+      put = put == (DQ_STAGES - 1) * S::BYTES ? 0u : put + S::BYTES;
+    };
+    auto lead = [&](const __nv_bfloat16* scales, int k0) {
+      return NG % 2 == 0 ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(scales + (row0 + k0) * NG) & 2) / 2;
+    };
+    fetch();
+    fetch();
+    w.load_q(static_cast<const ST*>(prm.q) + (static_cast<size_t>(b) * prm.H + hk * G + g0) * D, min(HEADS, G - g0), D, prm.scale_log2, g, t);
+    w.begin();
+    uint32_t take = 0;
+    for (int k0 = mine; k0 < k_end; k0 += step) {
+      cp_async_wait<1>();
+      __syncwarp();
+      fetch();
+      uint8_t* stage = ring + take;
+      take = take == (DQ_STAGES - 1) * S::BYTES ? 0u : take + S::BYTES;
+      const int n = k_end - k0, kl = lead(prm.k_scales, k0), vl = lead(prm.v_scales, k0);
+      if (n < DQ_BLOCK) {   // the rows behind the last key keep what was there: scales of zero make them nothing
+        if (lane >= n) {
+          unsigned short* ks = reinterpret_cast<unsigned short*>(stage + 2 * S::CODES) + kl + lane * NG;
+          unsigned short* vs = reinterpret_cast<unsigned short*>(stage + 2 * S::CODES + S::SCALES) + vl + lane * NG;
+#pragma unroll
+          for (int j = 0; j < NG; ++j) ks[j] = vs[j] = 0;
+        }
+        __syncwarp();
+      }
+      w.block(stage, n, kl, vl, g, t);
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+    w.leave(reinterpret_cast<float*>(ring), s_ml[warp], g, t);
+    __syncthreads();
+  };
+  // The warps' results as one: f(head, row of O^T, output, maximum, sum) for each element.
+  auto merged = [&](int heads, auto&& f) {
+    for (int i = threadIdx.x; i < heads * COLS; i += 32 * DQ_WARPS) {
+      const int h = i / COLS, r = i - h * COLS;
+      float mx = s_ml[0][h][0];
+#pragma unroll
+      for (int x = 1; x < DQ_WARPS; ++x) mx = fmaxf(mx, s_ml[x][h][0]);
+      const float m_ref = mx == -INFINITY ? 0.f : mx;
+      float a = 0.f, sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < DQ_WARPS; ++x) {
+        const float e = ptx::ex2(s_ml[x][h][0] - m_ref);
+        a = fmaf(e, reinterpret_cast<const float*>(dq_smem + x * S::WARP_BYTES)[h * Warp::PITCH + r], a);
+        sum = fmaf(e, s_ml[x][h][1], sum);
+      }
+      f(h, r, a, mx, sum);
+    }
+  };
+  auto finish = [&](size_t bh, int r, float a, float mx, float sum, bool some) {
+    const int d = q4_dim_of<NG>(r >> 4, r & 15);
+    if (d < D) rope_st(static_cast<ST*>(prm.o) + bh * D + d, some ? a / sum : 0.f);
+    if (r == 0 && prm.lse != nullptr) prm.lse[bh] = some ? (mx + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+  };
+
+  if constexpr (PLAN == PLAN_CLUSTER) {
+    const int b = blockIdx.z, p = blockIdx.y, sp = blockIdx.x, n = prm.n_splits;
+    const int len = length_of(b), blocks = (len + DQ_BLOCK - 1) / DQ_BLOCK, share = (blocks + n - 1) / n;
+    const int heads = min(HEADS, G - (p % chunks) * HEADS);
+    const size_t bh0 = static_cast<size_t>(b) * prm.H + (p / chunks) * G + (p % chunks) * HEADS;
+    attend(b, p, min(sp * share * DQ_BLOCK, len), min((sp + 1) * share * DQ_BLOCK, len));
+    if (n == 1) {
+      merged(heads, [&](int h, int r, float a, float mx, float sum) { finish(bh0 + h, r, a, mx, sum, len > 0); });
+      return;
+    }
+    // The CTA's result takes the place of its first warp's: element i is read, and then written, by one thread alone.
+    __shared__ float c_ml[HEADS][2];
+    float* c_acc = reinterpret_cast<float*>(dq_smem);
+    merged(heads, [&](int h, int r, float a, float mx, float sum) {
+      c_acc[h * Warp::PITCH + r] = a;
+      if (r == 0) {
+        c_ml[h][0] = mx;
+        c_ml[h][1] = sum;
+      }
+    });
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    for (int i = sp + static_cast<int>(threadIdx.x) * n; i < heads * COLS; i += 32 * DQ_WARPS * n) {
+      const int h = i / COLS, r0 = i - h * COLS;
+      float ms[8], ls[8], as[8], mx = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        ms[r] = -INFINITY;
+        if (r < n) {
+          const float* ml = cluster.map_shared_rank(&c_ml[h][0], r);
+          ms[r] = ml[0];
+          ls[r] = ml[1];
+          as[r] = *cluster.map_shared_rank(c_acc + h * Warp::PITCH + r0, r);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r) mx = fmaxf(mx, ms[r]);
+      const float m_ref = mx == -INFINITY ? 0.f : mx;
+      float a = 0.f, sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < n) {
+          const float e = ptx::ex2(ms[r] - m_ref);
+          a = fmaf(e, as[r], a);
+          sum = fmaf(e, ls[r], sum);
+        }
+      finish(bh0 + h, r0, a, mx, sum, len > 0);
+    }
+    cluster.sync();   // nobody's shared memory goes away while it is read
+  } else {
+    // The work of a pair is its units of 32 keys and DQ_START units for beginning and ending it: without those, a CTA whose
+    // share is many short sequences would be the last by far (32 sequences of up to 2000 positions: 59 us, with them XX).
+    // All CTAs add up the work in front of each sequence, and find the one that their own share begins in.
+    constexpr int threads = 32 * DQ_WARPS;
+    auto work_of = [&](int len) { return len > 0 ? DQ_START + (len + DQ_BLOCK - 1) / DQ_BLOCK : 0; };   // of one pair
+    int total = 0, share = 0, first = 0;
+    const int chunks_b = (prm.B + threads - 1) / threads;
+    for (int pass = chunks_b > 1 ? 0 : 1; pass < 2; ++pass) {   // a batch of more than one chunk is gone through twice
+      int before = 0;
+      for (int c = 0; c < chunks_b; ++c) {
+        const int b = c * threads + static_cast<int>(threadIdx.x);
+        const int work = b < prm.B ? per_b * work_of(length_of(b)) : 0;
+        int incl = work;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, incl, off);
+          if (lane >= off) incl += up;
+        }
+        if (lane == 31) s_scan[warp] = incl;
+        __syncthreads();
+        int at = before + incl - work;
+#pragma unroll
+        for (int x = 0; x < DQ_WARPS; ++x) {
+          if (x < warp) at += s_scan[x];
+          before += s_scan[x];
+        }
+        if (pass == 1) {
+          if (chunks_b == 1) total = before;
+          share = max((total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), DQ_START + DQ_WARPS);
+          first = min(static_cast<int>(blockIdx.x) * share, total);
+          if (b < prm.B) {
+            if (first >= at && first < at + work) {
+              s_scan[DQ_WARPS] = b;
+              s_scan[DQ_WARPS + 1] = at;
+            }
+            if (blockIdx.x == 0) prm.units[b] = at;
+          }
+        }
+        __syncthreads();
+      }
+      total = before;
+    }
+    const int last = min(first + share, total);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      prm.units[prm.B] = total;
+      prm.units[prm.B + 1] = share;
+    }
+    if (first >= last) return;
+    int b = s_scan[DQ_WARPS], at = s_scan[DQ_WARPS + 1];
+    for (int u = first; u < last;) {
+      const int len = min(max(prm.lengths[b], 0), prm.max_len), per_pair = work_of(len);
+      if (u >= at + per_b * per_pair) {
+        at += per_b * per_pair;
+        ++b;
+        continue;
+      }
+      const int p = (u - at) / per_pair, begin = at + p * per_pair + DQ_START, end = begin + per_pair - DQ_START;
+      const int u0 = max(u, begin), u1 = min(last, end);   // of the pair's units of keys begin .. end - 1
+      u = end;
+      if (u0 >= u1) continue;
+      const int heads = min(HEADS, G - (p % chunks) * HEADS);
+      attend(b, p, (u0 - begin) * DQ_BLOCK, min((u1 - begin) * DQ_BLOCK, len));
+      const bool whole = u0 == begin && u1 == end;
+      const size_t bh0 = static_cast<size_t>(b) * prm.H + (p / chunks) * G + (p % chunks) * HEADS;
+      const size_t part = (2 * static_cast<size_t>(blockIdx.x) + (u0 == begin ? 1 : 0)) * HEADS;   // begun here, or in front of it
+      merged(heads, [&](int h, int r, float a, float mx, float sum) {
+        if (whole) {
+          finish(bh0 + h, r, a, mx, sum, true);
+        } else {
+          prm.part_o[(part + h) * COLS + r] = a;
+          if (r == 0) {
+            prm.part_ml[(part + h) * 2] = mx;
+            prm.part_ml[(part + h) * 2 + 1] = sum;
+          }
+        }
+      });
+      __syncthreads();   // the rings are filled again
     }
   }
 }
 
-// One CTA per (batch, head) adds up the splits' parts.  A split without keys has the maximum -inf and the weight 0; a sequence
-// without keys gives zeros, and -inf as its log-sum-exp.
-template <typename ST>
-__global__ void __launch_bounds__(128)
-fa_decode_q4_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ lengths, ST* __restrict__ o,
-                          float* __restrict__ lse, int n_splits, int H, int D) {
-  const size_t bh = blockIdx.x;
+// PLAN_EVEN: one CTA per (batch, head) adds up the parts of a sequence that more than one CTA worked on: a warp takes every eighth
+// part, a lane every 32nd column.  A sequence without keys gives zeros, and -inf as its log-sum-exp.
+template <typename ST, int NG, int HEADS>
+__global__ void __launch_bounds__(32 * DQ_WARPS)
+fa_decode_q4_merge_kernel(const DecodeQ4Params prm) {
+  constexpr int COLS = 32 * NG;
+  __shared__ float s_acc[DQ_WARPS][COLS], s_mx[DQ_WARPS], s_sum[DQ_WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = static_cast<int>(blockIdx.x) / prm.H, head = static_cast<int>(blockIdx.x) % prm.H;
+  const int G = prm.H / prm.Hkv, chunks = (G + HEADS - 1) / HEADS, per_b = prm.Hkv * chunks;
+  const int p = head / G * chunks + head % G / HEADS, h = head % G % HEADS;
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
-  const bool empty = lengths[bh / H] <= 0;
-  const float2* ml = reinterpret_cast<const float2*>(part_ml) + bh * n_splits;
-  float mx = -INFINITY;
-  for (int s = 0; s < n_splits; ++s) mx = fmaxf(mx, ml[s].x);
-  const float m_ref = mx == -INFINITY ? 0.f : mx;
-  float a = 0.f, sum = 0.f;
-  const int d = threadIdx.x;
-  for (int s = 0; s < n_splits; ++s) {
-    const float f = ptx::ex2(ml[s].x - m_ref);
-    sum = fmaf(f, ml[s].y, sum);
-    if (d < D) a = fmaf(f, part_o[(bh * n_splits + s) * D + d], a);
+  const int at = prm.units[b], per_pair = (prm.units[b + 1] - at) / per_b, share = prm.units[prm.B + 1];
+  const int begin = at + p * per_pair + DQ_START, c0 = begin / share, c1 = per_pair > 0 ? (at + (p + 1) * per_pair - 1) / share : c0;
+  const size_t bh = blockIdx.x;
+  ST* o = static_cast<ST*>(prm.o) + bh * prm.D;
+  if (per_pair == 0) {
+    if (threadIdx.x < prm.D) rope_st(o + threadIdx.x, 0.f);
+    if (threadIdx.x == 0 && prm.lse != nullptr) prm.lse[bh] = -INFINITY;
+    return;
   }
-  if (d < D) rope_st(o + bh * D + d, empty ? 0.f : a / sum);
-  if (d == 0 && lse != nullptr) lse[bh] = empty ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
+  if (c0 == c1) return;
+  auto part_of = [&](int c) { return (2 * static_cast<size_t>(c) + (c == c0 ? 1 : 0)) * HEADS + h; };
+  float mx = -INFINITY;
+  for (int c = c0 + static_cast<int>(threadIdx.x); c <= c1; c += 32 * DQ_WARPS) mx = fmaxf(mx, prm.part_ml[part_of(c) * 2]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+  if (lane == 0) s_mx[warp] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < DQ_WARPS; ++x) mx = fmaxf(mx, s_mx[x]);
+  const float m_ref = mx == -INFINITY ? 0.f : mx;
+  float a[NG] = {}, sum = 0.f;
+#pragma unroll 4
+  for (int c = c0 + warp; c <= c1; c += DQ_WARPS) {
+    const size_t part = part_of(c);
+    const float e = ptx::ex2(prm.part_ml[part * 2] - m_ref);
+    sum = fmaf(e, prm.part_ml[part * 2 + 1], sum);
+#pragma unroll
+    for (int j = 0; j < NG; ++j) a[j] = fmaf(e, prm.part_o[part * COLS + 32 * j + lane], a[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < NG; ++j) s_acc[warp][32 * j + lane] = a[j];
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  const int r = threadIdx.x;
+  sum = 0.f;
+#pragma unroll
+  for (int x = 0; x < DQ_WARPS; ++x) sum += s_sum[x];
+  if (r < COLS) {
+    const int d = q4_dim_of<NG>(r >> 4, r & 15);
+    float total = 0.f;
+#pragma unroll
+    for (int x = 0; x < DQ_WARPS; ++x) total += s_acc[x][r];
+    if (d < prm.D) rope_st(o + d, total / sum);
+  }
+  if (r == 0 && prm.lse != nullptr) prm.lse[bh] = (mx + log2f(sum)) * 0.6931471805599453f;
 }
 
 }  // namespace it

@@ -4,6 +4,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
+#include <type_traits>
 
 #include "fa_decode_q4.cuh"
 #include "gemm_i8_sm100.cuh"
@@ -39,6 +41,9 @@ unsigned ctas_of(double threads) {
   const double n = std::ceil(threads / 256.0);
   return n <= 2147483647.0 ? static_cast<unsigned>(n) : 0u;
 }
+
+// Floats of the parts that a persistent attention launch leaves: outputs, then maxima and sums.
+size_t decode_q4_part_floats(int D) { return static_cast<size_t>(2 * it::DQ_MAX_CTAS * 8) * (32 * ((D + 31) / 32) + 2); }
 
 it::KvQ4 half_of(const void* codes, const void* scales) {
   return it::KvQ4{static_cast<uint32_t*>(const_cast<void*>(codes)), static_cast<__nv_bfloat16*>(const_cast<void*>(scales))};
@@ -144,8 +149,7 @@ it_status it_attention_decode_q4_workspace_bytes(int32_t B, int32_t H, int32_t D
   if (out_bytes == nullptr) return fail(IT_ERR_INVALID_ARG, "out_bytes is null");
   if (B < 0 || H < 0) return fail(IT_ERR_INVALID_ARG, "negative dimension");
   if (D < 8 || D > 128 || (D & 7)) return fail(IT_ERR_UNSUPPORTED_SHAPE, "a quantised cache needs head_dim a multiple of 8 in 8..128, got %d", D);
-  const size_t n = static_cast<size_t>(B) * H * it::DQ_MAX_SPLITS * (static_cast<size_t>(D) + 2) * sizeof(float);
-  *out_bytes = (n + 255) / 256 * 256 + 256;
+  *out_bytes = (decode_q4_part_floats(D) + B + 2) * 4 / 256 * 256 + 512;
   return IT_OK;
 }
 
@@ -181,35 +185,53 @@ it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype,
   p.D = D;
   p.max_len = max_len;
   p.scale_log2 = (1.0f / sqrtf(static_cast<float>(D))) * 1.4426950408889634f;
-  // As many shares of a sequence as fill the GPU, none of less than a round of the CTA's warps at max_len
-  const int G = H / Hkv, chunks = (G + it::DQ_HEADS - 1) / it::DQ_HEADS;
-  const long long base = static_cast<long long>(B) * Hkv * chunks, round = it::DQ_WARPS * it::DQ_BLOCK;
-  p.n_splits = static_cast<int>(std::max(1LL, std::min<long long>({(ctx->sm_count + base - 1) / base, (max_len + round - 1) / round, it::DQ_MAX_SPLITS})));
+  p.B = B;
+  const int G = H / Hkv;
+  const bool wide = dtype == IT_BF16 && G > 8;
+  const int heads = wide ? 16 : 8, chunks = (G + heads - 1) / heads;
+  const long long pairs = static_cast<long long>(B) * Hkv * chunks;
+  const int resident = (dtype == IT_BF16 && !wide ? 2 : 1) * ctx->sm_count;
   float* ws = static_cast<float*>(workspace);
   p.part_o = ws;
-  p.part_ml = ws + static_cast<size_t>(B) * H * p.n_splits * D;
-  const dim3 grid(p.n_splits, Hkv * chunks, B);
-  auto launch = [&](auto kernel) -> it_status {
-    IT_CUDA(launch_dependent(kernel, grid, 32 * it::DQ_WARPS, 0, stream->s, p));
-    ctx->launches += 1;
+  p.part_ml = ws + static_cast<size_t>(2 * it::DQ_MAX_CTAS * 8) * (32 * ((D + 31) / 32));
+  p.units = reinterpret_cast<int*>(ws + decode_q4_part_floats(D));
+  const bool even = getenv("DQ_PLAN") ? atoi(getenv("DQ_PLAN")) : pairs * max_len > 1024LL * resident;
+  int n = 1;
+  while (!even && n < 8 && 2 * n * pairs <= resident && max_len > 64 * n) n *= 2;
+  if (getenv("DQ_N")) n = atoi(getenv("DQ_N"));
+  p.n_splits = n;
+  const dim3 grid = even ? dim3(std::min(resident, wide ? it::DQ_MAX_CTAS / 2 : it::DQ_MAX_CTAS)) : dim3(n, Hkv * chunks, B);
+  auto main_launch = [&](auto ng, auto terms, auto hd) -> it_status {
+    constexpr int NG = decltype(ng)::value, TERMS = decltype(terms)::value, HEADS = decltype(hd)::value;
+    constexpr int bytes = it::DecodeQ4Stage<NG>::CTA_BYTES;
+    static std::atomic<bool> attr_set[16];
+    if (!attr_set[ctx->device & 15]) {
+      IT_CUDA(cudaFuncSetAttribute(it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+      IT_CUDA(cudaFuncSetAttribute(it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_EVEN>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+      attr_set[ctx->device & 15] = true;
+    }
+    if (!even) {
+      IT_CUDA(launch_cluster(it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_CLUSTER>, grid, 32 * it::DQ_WARPS, bytes, stream->s, n, p));
+      ctx->launches += 1;
+      return IT_OK;
+    }
+    IT_CUDA(launch_dependent(it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_EVEN>, grid, 32 * it::DQ_WARPS, bytes, stream->s, p));
+    using ST = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
+    IT_CUDA(launch_dependent(it::fa_decode_q4_merge_kernel<ST, NG, HEADS>, static_cast<unsigned>(B * H), 32 * it::DQ_WARPS, 0, stream->s, p));
+    ctx->launches += 2;
     return IT_OK;
   };
-  const int groups = (D + 31) / 32;
-  if (dtype == IT_F32)
-    st = groups == 1 ? launch(it::fa_decode_q4_kernel<1, 3>) : groups == 2 ? launch(it::fa_decode_q4_kernel<2, 3>)
-         : groups == 3 ? launch(it::fa_decode_q4_kernel<3, 3>) : launch(it::fa_decode_q4_kernel<4, 3>);
-  else
-    st = groups == 1 ? launch(it::fa_decode_q4_kernel<1, 1>) : groups == 2 ? launch(it::fa_decode_q4_kernel<2, 1>)
-         : groups == 3 ? launch(it::fa_decode_q4_kernel<3, 1>) : launch(it::fa_decode_q4_kernel<4, 1>);
-  if (st != IT_OK || p.n_splits == 1) return st;
-  auto merge = [&](auto kernel, auto* out) -> it_status {
-    IT_CUDA(launch_dependent(kernel, static_cast<unsigned>(B * H), 128, 0, stream->s, static_cast<const float*>(p.part_o),
-                             static_cast<const float*>(p.part_ml), lengths, out, lse, p.n_splits, H, D));
-    ctx->launches += 1;
-    return IT_OK;
+  auto by_groups = [&](auto terms, auto hd) -> it_status {
+    switch ((D + 31) / 32) {
+      case 1: return main_launch(std::integral_constant<int, 1>{}, terms, hd);
+      case 2: return main_launch(std::integral_constant<int, 2>{}, terms, hd);
+      case 3: return main_launch(std::integral_constant<int, 3>{}, terms, hd);
+      default: return main_launch(std::integral_constant<int, 4>{}, terms, hd);
+    }
   };
-  return dtype == IT_F32 ? merge(it::fa_decode_q4_merge_kernel<float>, static_cast<float*>(o))
-                         : merge(it::fa_decode_q4_merge_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(o));
+  using one = std::integral_constant<int, 1>;
+  if (dtype == IT_F32) return by_groups(std::integral_constant<int, 3>{}, std::integral_constant<int, 8>{});
+  return wide ? by_groups(one{}, std::integral_constant<int, 16>{}) : by_groups(one{}, std::integral_constant<int, 8>{});
 }
 
 it_status it_quantize_rows_i8(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t rows, int32_t cols, const void* x, int8_t* codes,
