@@ -496,11 +496,15 @@ __global__ void __launch_bounds__(32 * DQ_WARPS, TERMS == 1 && HEADS == 8 ? 2 : 
 fa_decode_q4_kernel(const DecodeQ4Params prm) {
   using ST = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
   using S = DecodeQ4Stage<NG>;
-  constexpr int COLS = 32 * NG;
   using Warp = DecodeQ4Warp<NG, TERMS, HEADS / 8>;
-  static_assert(HEADS * Warp::PITCH * 4 <= S::WARP_BYTES, "a warp's output is left in its ring");
+  constexpr int COLS = 32 * NG, STEP = DQ_WARPS * DQ_BLOCK;
+  // A warp leaves its output in the one stage of its ring that is free, while the first keys of the CTA's next stretch are on
+  // their way into the others; 16 heads take the whole ring.
+  constexpr bool AHEAD = HEADS == 8 && PLAN == PLAN_EVEN;
+  static_assert(HEADS * Warp::PITCH * 4 <= (AHEAD ? S::BYTES : S::WARP_BYTES) && S::BYTES % 16 == 0, "room for a warp's output");
   extern __shared__ __align__(16) uint8_t dq_smem[];
-  __shared__ float s_ml[DQ_WARPS][HEADS][2];
+  __shared__ float s_ml[DQ_WARPS][HEADS][2], s_weight[DQ_WARPS][HEADS], s_total[HEADS][2];
+  __shared__ uint32_t s_left[DQ_WARPS];    // where the warps' outputs are
   __shared__ int s_scan[DQ_WARPS + 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int G = prm.H / prm.Hkv, chunks = (G + HEADS - 1) / HEADS, per_b = prm.Hkv * chunks, D = prm.D;
@@ -514,40 +518,61 @@ fa_decode_q4_kernel(const DecodeQ4Params prm) {
     if (given != len) atomicCAS(prm.status, 0, DEV_ERR_CACHE_RANGE);
     return len;
   };
+  // Keys k0 .. k1 - 1 of sequence b and pair p (of K/V head and head chunk).
+  struct Stretch {
+    int b, p, k0, k1;
+  };
+  auto row_of = [&](const Stretch& x) { return (static_cast<size_t>(x.b) * prm.Hkv + x.p / chunks) * prm.max_len; };
+  auto heads_of = [&](const Stretch& x) { return min(HEADS, G - (x.p % chunks) * HEADS); };
+  auto bh_of = [&](const Stretch& x) { return static_cast<size_t>(x.b) * prm.H + (x.p / chunks) * G + (x.p % chunks) * HEADS; };
   Warp w;
-  // Keys k_begin .. k_end - 1 of (sequence b, pair p of K/V head and head chunk), by all warps; leaves their results in the rings.
-  auto attend = [&](int b, int p, int k_begin, int k_end) {
-    const int hk = p / chunks, g0 = (p % chunks) * HEADS;
-    const size_t row0 = (static_cast<size_t>(b) * prm.Hkv + hk) * prm.max_len;
-    const int mine = k_begin + warp * DQ_BLOCK, step = DQ_WARPS * DQ_BLOCK;
-    int next = mine;
-    uint32_t put = 0;
-    auto fetch = [&] {   // the warp's next block into the next stage
-      const int k0 = next;
-      if (k0 < k_end) {
-        const uint32_t at = ring_at + put;
-        q4_fetch<NG>(at, at + 2 * S::CODES, prm.k_codes, prm.k_scales, row0 + k0, k_end - k0, lane);
-        q4_fetch<NG>(at + S::CODES, at + 2 * S::CODES + S::SCALES, prm.v_codes, prm.v_scales, row0 + k0, k_end - k0, lane);
+  // The warp's blocks on their way: of the stretch at hand, or of the one behind it.
+  int fetch_k = 0, fetch_end = 0, on_way = 0;
+  size_t fetch_row = 0;
+  uint32_t put = 0, take = 0;
+  auto next_stage = [](uint32_t at) { return at == (DQ_STAGES - 1) * S::BYTES ? 0u : at + S::BYTES; };
+  auto fetch_from = [&](const Stretch& x) {
+    fetch_k = x.k0 + warp * DQ_BLOCK;
+    fetch_end = x.k1;
+    fetch_row = row_of(x);
+  };
+  auto fetch = [&] {
+    if (!AHEAD && fetch_k >= fetch_end) cp_async_commit();   // an empty group, so that the groups count the steps
+    if (fetch_k >= fetch_end || (AHEAD && on_way == DQ_STAGES)) return;
+    const uint32_t at = ring_at + put;
+    const int n = fetch_end - fetch_k;
+    q4_fetch<NG>(at, at + 2 * S::CODES, prm.k_codes, prm.k_scales, fetch_row + fetch_k, n, lane);
+    q4_fetch<NG>(at + S::CODES, at + 2 * S::CODES + S::SCALES, prm.v_codes, prm.v_scales, fetch_row + fetch_k, n, lane);
+    cp_async_commit();
+    fetch_k += STEP;
+    put = next_stage(put);
+    if (AHEAD) ++on_way;
+  };
+  // Attends to a stretch by all warps and leaves their results in the rings; `next` is what comes behind it (k1 = 0: nothing).
+  // Called with the first blocks on their way, and fetch_k within the stretch.
+  auto attend = [&](const Stretch& x, const Stretch& next) {
+    const size_t row0 = row_of(x);
+    bool behind = false;    // fetch_k is in the next stretch
+    auto fetch_on = [&] {
+      if (AHEAD && !behind && fetch_k >= fetch_end) {
+        fetch_from(next);
+        behind = true;
       }
-      cp_async_commit();
-      next += step;
-      put = put == (DQ_STAGES - 1) * S::BYTES ? 0u : put + S::BYTES;
+      fetch();
     };
     auto lead = [&](const __nv_bfloat16* scales, int k0) {
       return NG % 2 == 0 ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(scales + (row0 + k0) * NG) & 2) / 2;
     };
-    fetch();
-    fetch();
-    w.load_q(static_cast<const ST*>(prm.q) + (static_cast<size_t>(b) * prm.H + hk * G + g0) * D, min(HEADS, G - g0), D, prm.scale_log2, g, t);
+    w.load_q(static_cast<const ST*>(prm.q) + bh_of(x) * D, heads_of(x), D, prm.scale_log2, g, t);
     w.begin();
-    uint32_t take = 0;
-    for (int k0 = mine; k0 < k_end; k0 += step) {
-      cp_async_wait<1>();
-      __syncwarp();
-      fetch();
+    for (int k0 = x.k0 + warp * DQ_BLOCK; k0 < x.k1; k0 += STEP) {
+      if (AHEAD && on_way < 2) fetch_on();
+      if (!AHEAD || on_way > 1) cp_async_wait<1>();
+      else cp_async_wait<0>();
+      __syncwarp();    // the block is there for all lanes, and all have done with the one before it
+      fetch_on();
       uint8_t* stage = ring + take;
-      take = take == (DQ_STAGES - 1) * S::BYTES ? 0u : take + S::BYTES;
-      const int n = k_end - k0, kl = lead(prm.k_scales, k0), vl = lead(prm.v_scales, k0);
+      const int n = x.k1 - k0, kl = lead(prm.k_scales, k0), vl = lead(prm.v_scales, k0);
       if (n < DQ_BLOCK) {   // the rows behind the last key keep what was there: scales of zero make them nothing
         if (lane >= n) {
           unsigned short* ks = reinterpret_cast<unsigned short*>(stage + 2 * S::CODES) + kl + lane * NG;
@@ -558,56 +583,88 @@ fa_decode_q4_kernel(const DecodeQ4Params prm) {
         __syncwarp();
       }
       w.block(stage, n, kl, vl, g, t);
+      take = next_stage(take);
+      if (AHEAD) --on_way;
     }
-    cp_async_wait<0>();
+    if (!AHEAD) {
+      cp_async_wait<0>();
+      put = take = 0;
+    }
     __syncwarp();
-    w.leave(reinterpret_cast<float*>(ring), s_ml[warp], g, t);
+    if (!behind && AHEAD) fetch_from(next);
+    const uint32_t left = AHEAD ? put : 0u;     // on_way < DQ_STAGES here: the stage at `put` is free
+    if (lane == 0) s_left[warp] = warp * S::WARP_BYTES + left;
+    w.leave(reinterpret_cast<float*>(ring + left), s_ml[warp], g, t);
+    __syncthreads();
+    // the warps' results as one: weights, then four rows a thread
+    if (threadIdx.x < DQ_WARPS * HEADS) {
+      const int y = threadIdx.x / HEADS, h = threadIdx.x % HEADS;
+      float mx = s_ml[0][h][0], sum = 0.f;
+#pragma unroll
+      for (int z = 1; z < DQ_WARPS; ++z) mx = fmaxf(mx, s_ml[z][h][0]);
+      const float m_ref = mx == -INFINITY ? 0.f : mx;
+      s_weight[y][h] = ptx::ex2(s_ml[y][h][0] - m_ref);
+      if (y == 0) {
+#pragma unroll
+        for (int z = 0; z < DQ_WARPS; ++z) sum = fmaf(ptx::ex2(s_ml[z][h][0] - m_ref), s_ml[z][h][1], sum);
+        s_total[h][0] = mx;
+        s_total[h][1] = sum;
+      }
+    }
     __syncthreads();
   };
-  // The warps' results as one: f(head, row of O^T, output, maximum, sum) for each element.
+  // f(head, first of four rows of O^T, their outputs) for all of the CTA's result; s_total has the maxima and sums.
   auto merged = [&](int heads, auto&& f) {
-    for (int i = threadIdx.x; i < heads * COLS; i += 32 * DQ_WARPS) {
-      const int h = i / COLS, r = i - h * COLS;
-      float mx = s_ml[0][h][0];
-#pragma unroll
-      for (int x = 1; x < DQ_WARPS; ++x) mx = fmaxf(mx, s_ml[x][h][0]);
-      const float m_ref = mx == -INFINITY ? 0.f : mx;
-      float a = 0.f, sum = 0.f;
+    for (int i = threadIdx.x; i < heads * (COLS / 4); i += 32 * DQ_WARPS) {
+      const int h = i / (COLS / 4), r = 4 * (i % (COLS / 4));
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int x = 0; x < DQ_WARPS; ++x) {
-        const float e = ptx::ex2(s_ml[x][h][0] - m_ref);
-        a = fmaf(e, reinterpret_cast<const float*>(dq_smem + x * S::WARP_BYTES)[h * Warp::PITCH + r], a);
-        sum = fmaf(e, s_ml[x][h][1], sum);
+        const float e = s_weight[x][h];
+        const float4 v = *reinterpret_cast<const float4*>(dq_smem + s_left[x] + (h * Warp::PITCH + r) * 4);
+        a.x = fmaf(e, v.x, a.x);
+        a.y = fmaf(e, v.y, a.y);
+        a.z = fmaf(e, v.z, a.z);
+        a.w = fmaf(e, v.w, a.w);
       }
-      f(h, r, a, mx, sum);
+      f(h, r, a);
     }
   };
-  auto finish = [&](size_t bh, int r, float a, float mx, float sum, bool some) {
+  auto store_o = [&](size_t bh, int r, float x) {
     const int d = q4_dim_of<NG>(r >> 4, r & 15);
-    if (d < D) rope_st(static_cast<ST*>(prm.o) + bh * D + d, some ? a / sum : 0.f);
-    if (r == 0 && prm.lse != nullptr) prm.lse[bh] = some ? (mx + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    if (d < D) rope_st(static_cast<ST*>(prm.o) + bh * D + d, x);
+  };
+  auto store_lse = [&](size_t bh, float mx, float sum, bool some) {
+    if (prm.lse != nullptr) prm.lse[bh] = some ? (mx + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+  };
+  auto finish = [&](size_t bh0, int heads, bool some) {
+    merged(heads, [&](int h, int r, const float4& a) {
+      const float sum = s_total[h][1], inv = some ? 1.f / sum : 0.f;
+      store_o(bh0 + h, r, a.x * inv);
+      store_o(bh0 + h, r + 1, a.y * inv);
+      store_o(bh0 + h, r + 2, a.z * inv);
+      store_o(bh0 + h, r + 3, a.w * inv);
+      if (r == 0) store_lse(bh0 + h, s_total[h][0], sum, some);
+    });
   };
 
   if constexpr (PLAN == PLAN_CLUSTER) {
     const int b = blockIdx.z, p = blockIdx.y, sp = blockIdx.x, n = prm.n_splits;
     const int len = length_of(b), blocks = (len + DQ_BLOCK - 1) / DQ_BLOCK, share = (blocks + n - 1) / n;
-    const int heads = min(HEADS, G - (p % chunks) * HEADS);
-    const size_t bh0 = static_cast<size_t>(b) * prm.H + (p / chunks) * G + (p % chunks) * HEADS;
-    attend(b, p, min(sp * share * DQ_BLOCK, len), min((sp + 1) * share * DQ_BLOCK, len));
+    const Stretch x{b, p, min(sp * share * DQ_BLOCK, len), min((sp + 1) * share * DQ_BLOCK, len)};
+    const int heads = heads_of(x);
+    const size_t bh0 = bh_of(x);
+    fetch_from(x);
+    fetch();
+    fetch();
+    attend(x, Stretch{0, 0, 0, 0});
     if (n == 1) {
-      merged(heads, [&](int h, int r, float a, float mx, float sum) { finish(bh0 + h, r, a, mx, sum, len > 0); });
+      finish(bh0, heads, len > 0);
       return;
     }
-    // The CTA's result takes the place of its first warp's: element i is read, and then written, by one thread alone.
-    __shared__ float c_ml[HEADS][2];
+    // The CTA's result takes the place of its first warp's: four rows are read, and then written, by one thread alone.
     float* c_acc = reinterpret_cast<float*>(dq_smem);
-    merged(heads, [&](int h, int r, float a, float mx, float sum) {
-      c_acc[h * Warp::PITCH + r] = a;
-      if (r == 0) {
-        c_ml[h][0] = mx;
-        c_ml[h][1] = sum;
-      }
-    });
+    merged(heads, [&](int h, int r, const float4& a) { *reinterpret_cast<float4*>(c_acc + h * Warp::PITCH + r) = a; });
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
@@ -618,7 +675,7 @@ fa_decode_q4_kernel(const DecodeQ4Params prm) {
       for (int r = 0; r < 8; ++r) {
         ms[r] = -INFINITY;
         if (r < n) {
-          const float* ml = cluster.map_shared_rank(&c_ml[h][0], r);
+          const float* ml = cluster.map_shared_rank(&s_total[h][0], r);
           ms[r] = ml[0];
           ls[r] = ml[1];
           as[r] = *cluster.map_shared_rank(c_acc + h * Warp::PITCH + r0, r);
@@ -635,12 +692,13 @@ fa_decode_q4_kernel(const DecodeQ4Params prm) {
           a = fmaf(e, as[r], a);
           sum = fmaf(e, ls[r], sum);
         }
-      finish(bh0 + h, r0, a, mx, sum, len > 0);
+      store_o(bh0 + h, r0, len > 0 ? a / sum : 0.f);
+      if (r0 == 0) store_lse(bh0 + h, mx, sum, len > 0);
     }
     cluster.sync();   // nobody's shared memory goes away while it is read
   } else {
     // The work of a pair is its units of 32 keys and DQ_START units for beginning and ending it: without those, a CTA whose
-    // share is many short sequences would be the last by far (32 sequences of up to 2000 positions: 59 us, with them XX).
+    // share is many short sequences would be the last by far (32 sequences of up to 2000 positions: 59 us, with them 24).
     // All CTAs add up the work in front of each sequence, and find the one that their own share begins in.
     constexpr int threads = 32 * DQ_WARPS;
     auto work_of = [&](int len) { return len > 0 ? DQ_START + (len + DQ_BLOCK - 1) / DQ_BLOCK : 0; };   // of one pair
@@ -687,50 +745,69 @@ fa_decode_q4_kernel(const DecodeQ4Params prm) {
       prm.units[prm.B + 1] = share;
     }
     if (first >= last) return;
-    int b = s_scan[DQ_WARPS], at = s_scan[DQ_WARPS + 1];
-    for (int u = first; u < last;) {
-      const int len = min(max(prm.lengths[b], 0), prm.max_len), per_pair = work_of(len);
-      if (u >= at + per_b * per_pair) {
-        at += per_b * per_pair;
-        ++b;
-        continue;
-      }
-      const int p = (u - at) / per_pair, begin = at + p * per_pair + DQ_START, end = begin + per_pair - DQ_START;
-      const int u0 = max(u, begin), u1 = min(last, end);   // of the pair's units of keys begin .. end - 1
-      u = end;
-      if (u0 >= u1) continue;
-      const int heads = min(HEADS, G - (p % chunks) * HEADS);
-      attend(b, p, (u0 - begin) * DQ_BLOCK, min((u1 - begin) * DQ_BLOCK, len));
-      const bool whole = u0 == begin && u1 == end;
-      const size_t bh0 = static_cast<size_t>(b) * prm.H + (p / chunks) * G + (p % chunks) * HEADS;
-      const size_t part = (2 * static_cast<size_t>(blockIdx.x) + (u0 == begin ? 1 : 0)) * HEADS;   // begun here, or in front of it
-      merged(heads, [&](int h, int r, float a, float mx, float sum) {
-        if (whole) {
-          finish(bh0 + h, r, a, mx, sum, true);
-        } else {
-          prm.part_o[(part + h) * COLS + r] = a;
-          if (r == 0) {
-            prm.part_ml[(part + h) * 2] = mx;
-            prm.part_ml[(part + h) * 2 + 1] = sum;
-          }
+    int b = s_scan[DQ_WARPS], at = s_scan[DQ_WARPS + 1], u = first;
+    // The share's next stretch (k1 = 0: none), and whether it is a whole sequence.
+    auto next_stretch = [&](bool* whole) {
+      while (u < last) {
+        const int len = min(max(prm.lengths[b], 0), prm.max_len), per_pair = work_of(len);
+        if (u >= at + per_b * per_pair) {
+          at += per_b * per_pair;
+          ++b;
+          continue;
         }
-      });
+        const int p = (u - at) / per_pair, begin = at + p * per_pair + DQ_START, end = begin + per_pair - DQ_START;
+        const int u0 = max(u, begin), u1 = min(last, end);   // of the pair's units of keys begin .. end - 1
+        u = end;
+        if (u0 >= u1) continue;
+        *whole = u0 == begin && u1 == end;
+        return Stretch{b, p, (u0 - begin) * DQ_BLOCK, min((u1 - begin) * DQ_BLOCK, len)};
+      }
+      return Stretch{0, 0, 0, 0};
+    };
+    bool whole = false, next_whole = false;
+    Stretch x = next_stretch(&whole);
+    fetch_from(x);
+    fetch();
+    fetch();
+    while (x.k1 > 0) {
+      const Stretch next = next_stretch(&next_whole);
+      attend(x, next);
+      const int heads = heads_of(x);
+      if (whole) {
+        finish(bh_of(x), heads, true);
+      } else {
+        const size_t part = (2 * static_cast<size_t>(blockIdx.x) + (x.k0 == 0 ? 1 : 0)) * HEADS;   // begun here, or in front of it
+        merged(heads, [&](int h, int r, const float4& a) {
+          *reinterpret_cast<float4*>(prm.part_o + (part + h) * COLS + r) = a;
+          if (r == 0) {
+            prm.part_ml[(part + h) * 2] = s_total[h][0];
+            prm.part_ml[(part + h) * 2 + 1] = s_total[h][1];
+          }
+        });
+      }
       __syncthreads();   // the rings are filled again
+      if (!AHEAD) fetch_from(next);
+      if (!AHEAD || on_way < 2) fetch();
+      if (!AHEAD || on_way < 2) fetch();
+      x = next;
+      whole = next_whole;
     }
   }
 }
 
-// PLAN_EVEN: one CTA per (batch, head) adds up the parts of a sequence that more than one CTA worked on: a warp takes every eighth
-// part, a lane every 32nd column.  A sequence without keys gives zeros, and -inf as its log-sum-exp.
-template <typename ST, int NG, int HEADS>
+// PLAN_EVEN: adds up the parts of a sequence that more than one CTA worked on.  Grid (batch * heads, 1 or NG): of the NG CTAs of a
+// (batch, head) each takes 32 rows of O^T, where there are few (batch, head).  A warp takes every eighth part.  A sequence without
+// keys gives zeros, and -inf as its log-sum-exp.
+template <typename ST, int NG, int HEADS, int JN>   // JN: groups of 32 rows of a CTA, NG or 1
 __global__ void __launch_bounds__(32 * DQ_WARPS)
 fa_decode_q4_merge_kernel(const DecodeQ4Params prm) {
   constexpr int COLS = 32 * NG;
-  __shared__ float s_acc[DQ_WARPS][COLS], s_mx[DQ_WARPS], s_sum[DQ_WARPS];
+  __shared__ float s_acc[DQ_WARPS][32 * JN], s_e[DQ_MAX_CTAS], s_mx[DQ_WARPS], s_sum[DQ_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = static_cast<int>(blockIdx.x) / prm.H, head = static_cast<int>(blockIdx.x) % prm.H;
   const int G = prm.H / prm.Hkv, chunks = (G + HEADS - 1) / HEADS, per_b = prm.Hkv * chunks;
   const int p = head / G * chunks + head % G / HEADS, h = head % G % HEADS;
+  const int j0 = static_cast<int>(blockIdx.y) * JN;
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
   const int at = prm.units[b], per_pair = (prm.units[b + 1] - at) / per_b, share = prm.units[prm.B + 1];
@@ -738,14 +815,20 @@ fa_decode_q4_merge_kernel(const DecodeQ4Params prm) {
   const size_t bh = blockIdx.x;
   ST* o = static_cast<ST*>(prm.o) + bh * prm.D;
   if (per_pair == 0) {
-    if (threadIdx.x < prm.D) rope_st(o + threadIdx.x, 0.f);
-    if (threadIdx.x == 0 && prm.lse != nullptr) prm.lse[bh] = -INFINITY;
+    if (blockIdx.y == 0 && threadIdx.x < prm.D) rope_st(o + threadIdx.x, 0.f);
+    if (blockIdx.y == 0 && threadIdx.x == 0 && prm.lse != nullptr) prm.lse[bh] = -INFINITY;
     return;
   }
   if (c0 == c1) return;
   auto part_of = [&](int c) { return (2 * static_cast<size_t>(c) + (c == c0 ? 1 : 0)) * HEADS + h; };
-  float mx = -INFINITY;
-  for (int c = c0 + static_cast<int>(threadIdx.x); c <= c1; c += 32 * DQ_WARPS) mx = fmaxf(mx, prm.part_ml[part_of(c) * 2]);
+  float2 ml[2];   // of up to DQ_MAX_CTAS parts
+  float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int c = c0 + i * 32 * DQ_WARPS + static_cast<int>(threadIdx.x);
+    ml[i] = c <= c1 ? *reinterpret_cast<const float2*>(prm.part_ml + part_of(c) * 2) : make_float2(-INFINITY, 0.f);
+    mx = fmaxf(mx, ml[i].x);
+  }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
   if (lane == 0) s_mx[warp] = mx;
@@ -753,28 +836,36 @@ fa_decode_q4_merge_kernel(const DecodeQ4Params prm) {
 #pragma unroll
   for (int x = 0; x < DQ_WARPS; ++x) mx = fmaxf(mx, s_mx[x]);
   const float m_ref = mx == -INFINITY ? 0.f : mx;
-  float a[NG] = {}, sum = 0.f;
-#pragma unroll 4
-  for (int c = c0 + warp; c <= c1; c += DQ_WARPS) {
-    const size_t part = part_of(c);
-    const float e = ptx::ex2(prm.part_ml[part * 2] - m_ref);
-    sum = fmaf(e, prm.part_ml[part * 2 + 1], sum);
 #pragma unroll
-    for (int j = 0; j < NG; ++j) a[j] = fmaf(e, prm.part_o[part * COLS + 32 * j + lane], a[j]);
+  for (int i = 0; i < 2; ++i) {
+    const float e = ptx::ex2(ml[i].x - m_ref);
+    s_e[i * 32 * DQ_WARPS + threadIdx.x] = e;
+    sum = fmaf(e, ml[i].y, sum);
   }
 #pragma unroll
-  for (int j = 0; j < NG; ++j) s_acc[warp][32 * j + lane] = a[j];
+  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   if (lane == 0) s_sum[warp] = sum;
   __syncthreads();
-  const int r = threadIdx.x;
   sum = 0.f;
 #pragma unroll
   for (int x = 0; x < DQ_WARPS; ++x) sum += s_sum[x];
-  if (r < COLS) {
+  float a[JN] = {};
+#pragma unroll 4
+  for (int c = c0 + warp; c <= c1; c += DQ_WARPS) {
+    const float e = s_e[c - c0];
+    const float* src = prm.part_o + part_of(c) * COLS + 32 * j0 + lane;
+#pragma unroll
+    for (int j = 0; j < JN; ++j) a[j] = fmaf(e, src[32 * j], a[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < JN; ++j) s_acc[warp][32 * j + lane] = a[j];
+  __syncthreads();
+  const int r = 32 * j0 + static_cast<int>(threadIdx.x);
+  if (threadIdx.x < 32 * JN) {
     const int d = q4_dim_of<NG>(r >> 4, r & 15);
     float total = 0.f;
 #pragma unroll
-    for (int x = 0; x < DQ_WARPS; ++x) total += s_acc[x][r];
+    for (int x = 0; x < DQ_WARPS; ++x) total += s_acc[x][threadIdx.x];
     if (d < prm.D) rope_st(o + d, total / sum);
   }
   if (r == 0 && prm.lse != nullptr) prm.lse[bh] = (mx + log2f(sum)) * 0.6931471805599453f;

@@ -42,6 +42,54 @@ unsigned ctas_of(double threads) {
   return n <= 2147483647.0 ? static_cast<unsigned>(n) : 0u;
 }
 
+// How many clusters of `size` CTAs of a kernel are resident at once (asked once per kernel, device and size).
+template <typename Kernel>
+int clusters_at_once(Kernel kernel, int size, int smem_bytes, std::atomic<int>& known) {
+  if (known == 0) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(32 * it::DQ_WARPS);
+    cfg.dynamicSmemBytes = smem_bytes;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(size);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = 1;
+    }
+    known = n;
+  }
+  return known;
+}
+
+// How 4-bit attention shares out its work (see fa_decode_q4.cuh): clusters of 1, 2, 4 or 8 CTAs a pair, or even shares.  The lengths are
+// on the device, so this goes by max_len.  In us, measured: a launch of clusters is 4.5, 0.3 for each doubling of the cluster and a
+// round of 256 keys 1.25 for a CTA that has an SM for itself, 2.2 for two on one, at head_dim 128 (B8 H32/8, 4000 positions: 16.5
+// in clusters of two or four, 24.9 alone; B1 H32/8, 16000, clusters of eight: 15.6; 1000 positions of B4 H16/4: 8.5, 7.1, 5.9 and
+// 6.4 with 1, 2, 4 and 8).  An even launch is 16 and its rounds (one sequence of 131000, H16/2: 26, in clusters 88; B32 H32/8
+// ragged to 8190: 53, in clusters 64 and 55; 64 pairs of 4000: 24 and 16.5).  Batches are counted as three quarters full there, because
+// in clusters the longest sequence decides.
+template <typename AtOnce>
+void choose_decode_q4_plan(long long pairs, int B, int max_len, int sm_count, int per_sm, int groups, AtOnce&& at_once, int* n_splits, bool* even) {
+  const double width = 0.35 + 0.65 * groups / 4, two = 2.2 * width, one = per_sm == 1 ? two : 1.25 * width;
+  double best = 1e30;
+  for (int n = 1; n <= 8; n *= 2) {
+    const long long rounds = (static_cast<long long>(max_len) + 256LL * n - 1) / (256LL * n), resident = std::max(1, at_once(n));
+    const double round = pairs * n > sm_count ? two : one;
+    const double t = 4.5 + 0.3 * (n >= 8 ? 3 : n / 2) + static_cast<double>((pairs + resident - 1) / resident) * rounds * round;
+    if (t < best) {
+      best = t;
+      *n_splits = n;
+    }
+  }
+  const double rounds = static_cast<double>(pairs) * (max_len + 32.0 * it::DQ_START) / (256.0 * per_sm * sm_count);
+  *even = 16.0 + (B > 1 ? 0.75 : 1.0) * rounds * two < best;
+}
+
 // Floats of the parts that a persistent attention launch leaves: outputs, then maxima and sums.
 size_t decode_q4_part_floats(int D) { return static_cast<size_t>(2 * it::DQ_MAX_CTAS * 8) * (32 * ((D + 31) / 32) + 2); }
 
@@ -195,12 +243,8 @@ it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype,
   p.part_o = ws;
   p.part_ml = ws + static_cast<size_t>(2 * it::DQ_MAX_CTAS * 8) * (32 * ((D + 31) / 32));
   p.units = reinterpret_cast<int*>(ws + decode_q4_part_floats(D));
-  const bool even = getenv("DQ_PLAN") ? atoi(getenv("DQ_PLAN")) : pairs * max_len > 1024LL * resident;
   int n = 1;
-  while (!even && n < 8 && 2 * n * pairs <= resident && max_len > 64 * n) n *= 2;
-  if (getenv("DQ_N")) n = atoi(getenv("DQ_N"));
-  p.n_splits = n;
-  const dim3 grid = even ? dim3(std::min(resident, wide ? it::DQ_MAX_CTAS / 2 : it::DQ_MAX_CTAS)) : dim3(n, Hkv * chunks, B);
+  bool even = false;
   auto main_launch = [&](auto ng, auto terms, auto hd) -> it_status {
     constexpr int NG = decltype(ng)::value, TERMS = decltype(terms)::value, HEADS = decltype(hd)::value;
     constexpr int bytes = it::DecodeQ4Stage<NG>::CTA_BYTES;
@@ -210,14 +254,24 @@ it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype,
       IT_CUDA(cudaFuncSetAttribute(it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_EVEN>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
       attr_set[ctx->device & 15] = true;
     }
+    const auto in_clusters = it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_CLUSTER>;
+    static std::atomic<int> at_once[16][9];
+    choose_decode_q4_plan(pairs, B, max_len, ctx->sm_count, resident / ctx->sm_count, NG,
+                          [&](int size) { return clusters_at_once(in_clusters, size, bytes, at_once[ctx->device & 15][size]); }, &n, &even);
+    if (getenv("DQ_PLAN")) even = atoi(getenv("DQ_PLAN"));
+    if (getenv("DQ_N")) n = atoi(getenv("DQ_N"));
+    p.n_splits = n;
+    const dim3 grid = even ? dim3(std::min(resident, wide ? it::DQ_MAX_CTAS / 2 : it::DQ_MAX_CTAS)) : dim3(n, Hkv * chunks, B);
     if (!even) {
-      IT_CUDA(launch_cluster(it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_CLUSTER>, grid, 32 * it::DQ_WARPS, bytes, stream->s, n, p));
+      IT_CUDA(launch_cluster(in_clusters, grid, 32 * it::DQ_WARPS, bytes, stream->s, n, p));
       ctx->launches += 1;
       return IT_OK;
     }
     IT_CUDA(launch_dependent(it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_EVEN>, grid, 32 * it::DQ_WARPS, bytes, stream->s, p));
     using ST = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
-    IT_CUDA(launch_dependent(it::fa_decode_q4_merge_kernel<ST, NG, HEADS>, static_cast<unsigned>(B * H), 32 * it::DQ_WARPS, 0, stream->s, p));
+    const bool few = B * H < ctx->sm_count;
+    IT_CUDA(launch_dependent(few ? it::fa_decode_q4_merge_kernel<ST, NG, HEADS, 1> : it::fa_decode_q4_merge_kernel<ST, NG, HEADS, NG>,
+                             dim3(B * H, few ? NG : 1), 32 * it::DQ_WARPS, 0, stream->s, p));
     ctx->launches += 2;
     return IT_OK;
   };

@@ -36,12 +36,12 @@ def cache_of(k, v, max_len, junk=True):
     import torch
     B, L, Hkv, D = k.shape
     g = -(-D // 32)
-    codes = np.full((2, B, Hkv, max_len, 16 * g), 0xFF if junk else 0x88, np.uint8)
-    scales = np.full((2, B, Hkv, max_len, g), np.nan if junk else 0.0)
+    codes = torch.full((2, B, Hkv, max_len, 16 * g), 0xFF if junk else 0x88, dtype=torch.uint8, device="cuda")
+    scales = torch.full((2, B, Hkv, max_len, g), math.nan if junk else 0.0, dtype=torch.bfloat16, device="cuda")
     for i, x in enumerate((k, v)):
         c, s = qr.q4(x.transpose(0, 2, 1, 3))
-        codes[i, :, :, :L], scales[i, :, :, :L] = qr.q4_bytes(c), s
-    return QuantizedCache(torch.from_numpy(codes).cuda(), torch.from_numpy(scales).to(torch.bfloat16).cuda(), D)
+        codes[i, :, :, :L], scales[i, :, :, :L] = torch.from_numpy(qr.q4_bytes(c)).cuda(), torch.from_numpy(s).cuda()
+    return QuantizedCache(codes, scales, D)
 
 
 def host(cache):
@@ -181,6 +181,31 @@ def test_decode_at_every_sequences_own_length(it_ctx, precision, H, Hkv, D, leng
     q = values(rng, (B, H, D), precision)
     k, v = values(rng, (B, L, Hkv, D), FP32), values(rng, (B, L, Hkv, D), FP32)
     check_decode(it_ctx, precision, q, k, v, lengths, max_len)
+
+
+@pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("H,Hkv,D,max_len,lengths", [
+    (8, 2, 128, 1 << 17, [3000, 1, 0, 900, 33]), (12, 1, 64, 1 << 18, [5000, 0, 31]), (4, 4, 32, 1 << 17, [2050, 700]), (6, 2, 96, 1 << 17, [0, 1500, 1]),
+    (32, 2, 80, 1 << 17, [0, 2000]), (5, 1, 16, 1 << 19, [1025]), (2, 2, 48, 1 << 18, [0, 0]),
+])
+def test_decode_in_even_shares(it_ctx, precision, H, Hkv, D, max_len, lengths):
+    """Room for long sequences: the persistent launch, whose CTAs share out what the lengths turn out to be."""
+    rng = np.random.default_rng(D + H)
+    B, L = len(lengths), max(max(lengths), 1)
+    q = values(rng, (B, H, D), precision)
+    k, v = values(rng, (B, L, Hkv, D), FP32), values(rng, (B, L, Hkv, D), FP32)
+    check_decode(it_ctx, precision, q, k, v, lengths, max_len)
+
+
+def test_decode_of_many_sequences_in_even_shares(it_ctx):
+    """More sequences than a CTA has threads."""
+    rng = np.random.default_rng(19)
+    B, H, D = 700, 2, 64
+    lengths = rng.integers(0, 70, B)
+    lengths[[0, 255, 256, 699]] = [0, 69, 1, 40]
+    q, k, v = values(rng, (B, H, D), BF16), values(rng, (B, 69, 1, D), FP32), values(rng, (B, 69, 1, D), FP32)
+    check_decode(it_ctx, BF16, q, k, v, lengths, 2048)
+    check_decode(it_ctx, BF16, q, k, v, np.zeros(B, int), 2048)
 
 
 @pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
