@@ -36,8 +36,12 @@
 
 namespace it {
 
-constexpr int DQ_WARPS = 8, DQ_BLOCK = 32, DQ_STAGES = 3, DQ_MAX_CTAS = 512, DQ_START = 12;
+constexpr int DQ_BLOCK = 32, DQ_STAGES = 3, DQ_MAX_CTAS = 512, DQ_START = 12;
 enum : int { PLAN_CLUSTER = 0, PLAN_EVEN = 1 };
+// Warps of a CTA: eight, or six in the persistent launches of which two CTAs are on an SM: 168 registers a thread, which the loop needs
+// more than it needs a fourth warp on each scheduler with 128 and some of them in memory (B32 H32/8 D128 ragged to 8190: 52.7 -> 50.0 us).
+__host__ __device__ constexpr int dq_warps(int terms, int heads, int plan) { return plan == PLAN_EVEN && terms == 1 && heads == 8 ? 6 : 8; }
+constexpr int DQ_MERGE_WARPS = 8;
 
 struct DecodeQ4Params {
   const void* q;            // [batch, heads, D]
@@ -127,7 +131,6 @@ struct DecodeQ4Stage {
   static constexpr int SCALES = (DQ_BLOCK * 2 * NG + 2 + 15) / 16 * 16;     // and up to two bytes in front of them
   static constexpr int BYTES = 2 * CODES + 2 * SCALES;
   static constexpr int WARP_BYTES = DQ_STAGES * BYTES;
-  static constexpr int CTA_BYTES = DQ_WARPS * WARP_BYTES;
 };
 
 // Position in the block of a score's column: the n-th of 8 is key n / 2 (n even) or 4 + (n / 2 ^ X).  With the V operand's
@@ -492,12 +495,12 @@ struct DecodeQ4Warp {
 // or, in bf16, 16, which share the operands made of the codes.
 // PLAN_CLUSTER: grid (n_splits, kv_heads * chunks, batch), clusters of n_splits.  PLAN_EVEN: any number of CTAs up to DQ_MAX_CTAS.
 template <int NG, int TERMS, int HEADS, int PLAN>
-__global__ void __launch_bounds__(32 * DQ_WARPS, TERMS == 1 && HEADS == 8 ? 2 : 1)
+__global__ void __launch_bounds__(32 * dq_warps(TERMS, HEADS, PLAN), TERMS == 1 && HEADS == 8 ? 2 : 1)
 fa_decode_q4_kernel(const DecodeQ4Params prm) {
   using ST = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
   using S = DecodeQ4Stage<NG>;
   using Warp = DecodeQ4Warp<NG, TERMS, HEADS / 8>;
-  constexpr int COLS = 32 * NG, STEP = DQ_WARPS * DQ_BLOCK;
+  constexpr int DQ_WARPS = dq_warps(TERMS, HEADS, PLAN), COLS = 32 * NG, STEP = DQ_WARPS * DQ_BLOCK;
   // A warp leaves its output in the one stage of its ring that is free, while the first keys of the CTA's next stretch are on
   // their way into the others; 16 heads take the whole ring.
   constexpr bool AHEAD = HEADS == 8 && PLAN == PLAN_EVEN;
@@ -799,10 +802,10 @@ fa_decode_q4_kernel(const DecodeQ4Params prm) {
 // (batch, head) each takes 32 rows of O^T, where there are few (batch, head).  A warp takes every eighth part.  A sequence without
 // keys gives zeros, and -inf as its log-sum-exp.
 template <typename ST, int NG, int HEADS, int JN>   // JN: groups of 32 rows of a CTA, NG or 1
-__global__ void __launch_bounds__(32 * DQ_WARPS)
+__global__ void __launch_bounds__(32 * DQ_MERGE_WARPS)
 fa_decode_q4_merge_kernel(const DecodeQ4Params prm) {
   constexpr int COLS = 32 * NG;
-  __shared__ float s_acc[DQ_WARPS][32 * JN], s_e[DQ_MAX_CTAS], s_mx[DQ_WARPS], s_sum[DQ_WARPS];
+  __shared__ float s_acc[DQ_MERGE_WARPS][32 * JN], s_e[DQ_MAX_CTAS], s_mx[DQ_MERGE_WARPS], s_sum[DQ_MERGE_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = static_cast<int>(blockIdx.x) / prm.H, head = static_cast<int>(blockIdx.x) % prm.H;
   const int G = prm.H / prm.Hkv, chunks = (G + HEADS - 1) / HEADS, per_b = prm.Hkv * chunks;
@@ -825,7 +828,7 @@ fa_decode_q4_merge_kernel(const DecodeQ4Params prm) {
   float mx = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int c = c0 + i * 32 * DQ_WARPS + static_cast<int>(threadIdx.x);
+    const int c = c0 + i * 32 * DQ_MERGE_WARPS + static_cast<int>(threadIdx.x);
     ml[i] = c <= c1 ? *reinterpret_cast<const float2*>(prm.part_ml + part_of(c) * 2) : make_float2(-INFINITY, 0.f);
     mx = fmaxf(mx, ml[i].x);
   }
@@ -834,12 +837,12 @@ fa_decode_q4_merge_kernel(const DecodeQ4Params prm) {
   if (lane == 0) s_mx[warp] = mx;
   __syncthreads();
 #pragma unroll
-  for (int x = 0; x < DQ_WARPS; ++x) mx = fmaxf(mx, s_mx[x]);
+  for (int x = 0; x < DQ_MERGE_WARPS; ++x) mx = fmaxf(mx, s_mx[x]);
   const float m_ref = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float e = ptx::ex2(ml[i].x - m_ref);
-    s_e[i * 32 * DQ_WARPS + threadIdx.x] = e;
+    s_e[i * 32 * DQ_MERGE_WARPS + threadIdx.x] = e;
     sum = fmaf(e, ml[i].y, sum);
   }
 #pragma unroll
@@ -848,10 +851,10 @@ fa_decode_q4_merge_kernel(const DecodeQ4Params prm) {
   __syncthreads();
   sum = 0.f;
 #pragma unroll
-  for (int x = 0; x < DQ_WARPS; ++x) sum += s_sum[x];
+  for (int x = 0; x < DQ_MERGE_WARPS; ++x) sum += s_sum[x];
   float a[JN] = {};
 #pragma unroll 4
-  for (int c = c0 + warp; c <= c1; c += DQ_WARPS) {
+  for (int c = c0 + warp; c <= c1; c += DQ_MERGE_WARPS) {
     const float e = s_e[c - c0];
     const float* src = prm.part_o + part_of(c) * COLS + 32 * j0 + lane;
 #pragma unroll
@@ -865,7 +868,7 @@ fa_decode_q4_merge_kernel(const DecodeQ4Params prm) {
     const int d = q4_dim_of<NG>(r >> 4, r & 15);
     float total = 0.f;
 #pragma unroll
-    for (int x = 0; x < DQ_WARPS; ++x) total += s_acc[x][threadIdx.x];
+    for (int x = 0; x < DQ_MERGE_WARPS; ++x) total += s_acc[x][threadIdx.x];
     if (d < prm.D) rope_st(o + d, total / sum);
   }
   if (r == 0 && prm.lse != nullptr) prm.lse[bh] = (mx + log2f(sum)) * 0.6931471805599453f;

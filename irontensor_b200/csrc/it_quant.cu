@@ -44,11 +44,11 @@ unsigned ctas_of(double threads) {
 
 // How many clusters of `size` CTAs of a kernel are resident at once (asked once per kernel, device and size).
 template <typename Kernel>
-int clusters_at_once(Kernel kernel, int size, int smem_bytes, std::atomic<int>& known) {
+int clusters_at_once(Kernel kernel, int size, int threads, int smem_bytes, std::atomic<int>& known) {
   if (known == 0) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(size);
-    cfg.blockDim = dim3(32 * it::DQ_WARPS);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem_bytes;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -247,31 +247,32 @@ it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype,
   bool even = false;
   auto main_launch = [&](auto ng, auto terms, auto hd) -> it_status {
     constexpr int NG = decltype(ng)::value, TERMS = decltype(terms)::value, HEADS = decltype(hd)::value;
-    constexpr int bytes = it::DecodeQ4Stage<NG>::CTA_BYTES;
+    constexpr int warps = it::dq_warps(TERMS, HEADS, it::PLAN_CLUSTER), even_warps = it::dq_warps(TERMS, HEADS, it::PLAN_EVEN);
+    constexpr int bytes = warps * it::DecodeQ4Stage<NG>::WARP_BYTES, even_bytes = even_warps * it::DecodeQ4Stage<NG>::WARP_BYTES;
     static std::atomic<bool> attr_set[16];
     if (!attr_set[ctx->device & 15]) {
       IT_CUDA(cudaFuncSetAttribute(it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-      IT_CUDA(cudaFuncSetAttribute(it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_EVEN>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+      IT_CUDA(cudaFuncSetAttribute(it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_EVEN>, cudaFuncAttributeMaxDynamicSharedMemorySize, even_bytes));
       attr_set[ctx->device & 15] = true;
     }
     const auto in_clusters = it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_CLUSTER>;
     static std::atomic<int> at_once[16][9];
     choose_decode_q4_plan(pairs, B, max_len, ctx->sm_count, resident / ctx->sm_count, NG,
-                          [&](int size) { return clusters_at_once(in_clusters, size, bytes, at_once[ctx->device & 15][size]); }, &n, &even);
+                          [&](int size) { return clusters_at_once(in_clusters, size, 32 * warps, bytes, at_once[ctx->device & 15][size]); }, &n, &even);
     if (getenv("DQ_PLAN")) even = atoi(getenv("DQ_PLAN"));
     if (getenv("DQ_N")) n = atoi(getenv("DQ_N"));
     p.n_splits = n;
     const dim3 grid = even ? dim3(std::min(resident, wide ? it::DQ_MAX_CTAS / 2 : it::DQ_MAX_CTAS)) : dim3(n, Hkv * chunks, B);
     if (!even) {
-      IT_CUDA(launch_cluster(in_clusters, grid, 32 * it::DQ_WARPS, bytes, stream->s, n, p));
+      IT_CUDA(launch_cluster(in_clusters, grid, 32 * warps, bytes, stream->s, n, p));
       ctx->launches += 1;
       return IT_OK;
     }
-    IT_CUDA(launch_dependent(it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_EVEN>, grid, 32 * it::DQ_WARPS, bytes, stream->s, p));
+    IT_CUDA(launch_dependent(it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_EVEN>, grid, 32 * even_warps, even_bytes, stream->s, p));
     using ST = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
     const bool few = B * H < ctx->sm_count;
     IT_CUDA(launch_dependent(few ? it::fa_decode_q4_merge_kernel<ST, NG, HEADS, 1> : it::fa_decode_q4_merge_kernel<ST, NG, HEADS, NG>,
-                             dim3(B * H, few ? NG : 1), 32 * it::DQ_WARPS, 0, stream->s, p));
+                             dim3(B * H, few ? NG : 1), 32 * it::DQ_MERGE_WARPS, 0, stream->s, p));
     ctx->launches += 2;
     return IT_OK;
   };
@@ -379,5 +380,10 @@ extern "C" it_status it_linear_i8_fwd(it_ctx* ctx, it_stream* stream, it_dtype o
   p.N = out_dim;
   p.K = in_dim;
   p.status = ctx->d_status;
+  const int bn = getenv("I8_TILE") ? atoi(getenv("I8_TILE")) : 128;
+  if (bn == 512) return launch_gemm_i8<256, 2>(ctx, stream->s, x_codes, w_codes, p);
+  if (bn == 384) return launch_gemm_i8<128, 2>(ctx, stream->s, x_codes, w_codes, p);
+  if (bn == 256) return launch_gemm_i8<256, 1>(ctx, stream->s, x_codes, w_codes, p);
+  if (bn == 64) return launch_gemm_i8<64, 1>(ctx, stream->s, x_codes, w_codes, p);
   return launch_gemm_i8<128, 1>(ctx, stream->s, x_codes, w_codes, p);
 }
