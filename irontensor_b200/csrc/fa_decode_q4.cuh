@@ -57,37 +57,6 @@ struct DecodeQ4Params {
   float scale_log2;         // 1/sqrt(D) * log2(e)
 };
 
-__device__ __forceinline__ uint32_t q4_fma2(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-__device__ __forceinline__ uint32_t q4_mul2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-// (x & MASK) | magic in one instruction.  It takes one constant in itself and no second one, so `magic` comes in a register; left to
-// itself the compiler makes two instructions of it, and this unit is what the kernel waits for.
-template <uint32_t MASK>
-__device__ __forceinline__ uint32_t q4_and_or(uint32_t x, uint32_t magic) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "n"(MASK), "r"(magic));
-  return d;
-}
-__device__ __forceinline__ uint32_t q4_constant(uint32_t c) {   // one that the compiler does not see through
-  uint32_t d;
-  asm volatile("mov.b32 %0, %1;" : "=r"(d) : "r"(c));
-  return d;
-}
-// Nibble I of both halves of w as the values (16 + u) s - 24 s.
-template <int I>
-__device__ __forceinline__ uint32_t q4_pair(uint32_t w, uint32_t s2, uint32_t bias2, uint32_t magic) {
-  const uint32_t at3 = I == 0 ? w << 3 : w >> (4 * I - 3);
-  return q4_fma2(q4_and_or<0x00780078u>(at3, magic), s2, bias2);
-}
-constexpr uint32_t Q4_MAGIC = 0x41804180u;      // 16 in both halves
-
 // D = A B + C in fp16 with fp32 sums.
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
                                               float c0, float c1, float c2, float c3) {
@@ -101,7 +70,6 @@ __device__ __forceinline__ uint32_t q4_add2_f16(uint32_t a, uint32_t b) {
   asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-constexpr uint32_t Q4_MINUS_24 = 0xC1C0C1C0u;   // -24 in both halves
 
 // Which column of a head is row r (0 .. 15) of O^T's m-tile mt (see the V operand below).
 template <int NG>

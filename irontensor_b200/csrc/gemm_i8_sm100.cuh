@@ -16,92 +16,130 @@
 
 namespace it {
 
-// x [rows, cols] -> codes [rows, cols], scales [rows].  A CTA per row, which keeps what it can of the row in registers between
-// finding the largest magnitude and dividing: 8 columns a thread and step.
-template <typename ST>
+// x [rows, cols] -> codes [rows, cols], scales [rows].  WARPS warps a row, which keep what they can of it (16 bytes a lane and step,
+// KEEP steps) in registers between finding the largest magnitude and dividing, and read the rest again.  Bound by memory where
+// there are many rows, and by two trips to it where there are few.
+template <typename ST, int WARPS>
 __global__ void __launch_bounds__(256)
-quantize_rows_kernel(const ST* __restrict__ x, int8_t* __restrict__ codes, float* __restrict__ scales, int cols) {
-  constexpr int KEEP = 4;
+quantize_rows_kernel(const ST* __restrict__ x, int8_t* __restrict__ codes, float* __restrict__ scales, int rows, int cols) {
+  constexpr int KEEP = 8, VEC = 16 / sizeof(ST), STEP = 32 * WARPS * VEC, ROWS = 8 / WARPS;
   __shared__ uint32_t s_most[8];
-  const size_t row = blockIdx.x;
-  const ST* src = x + row * cols;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row = static_cast<long long>(blockIdx.x) * ROWS + warp / WARPS;
+  const int first = ((warp % WARPS) * 32 + lane) * VEC;
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
-  float keep[KEEP][8];
+  if (WARPS == 1 && row >= rows) return;   // a row of more warps is a whole CTA's, or half of one: all stay for the barrier
+  const ST* src = x + (row < rows ? row : 0) * cols;
+  auto bits = [](const uint4& v, uint32_t most) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (sizeof(ST) == 4) most = max(most, w[i] & 0x7FFFFFFFu);
+      else most = max(most, max((w[i] << 16) & 0x7FFFFFFFu, w[i] & 0x7FFF0000u));
+    }
+    return most;
+  };
+  uint4 keep[KEEP];
   uint32_t most = 0;
 #pragma unroll
   for (int u = 0; u < KEEP; ++u) {
-    const int c = (u * 256 + static_cast<int>(threadIdx.x)) * 8;
-    if (c < cols) {
-      q4_load8(src + c, keep[u]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(keep[u][e]) & 0x7FFFFFFFu);
-    }
+    keep[u] = make_uint4(0u, 0u, 0u, 0u);
+    if (first + u * STEP < cols) keep[u] = __ldg(reinterpret_cast<const uint4*>(src + first + u * STEP));
   }
-  for (int c = (KEEP * 256 + static_cast<int>(threadIdx.x)) * 8; c < cols; c += 2048) {
-    float v[8];
-    q4_load8(src + c, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(v[e]) & 0x7FFFFFFFu);
-  }
+  for (int u = 0; u < KEEP; ++u) most = bits(keep[u], most);
+  for (int c = first + KEEP * STEP; c < cols; c += STEP) most = bits(__ldg(reinterpret_cast<const uint4*>(src + c)), most);
   most = __reduce_max_sync(0xffffffffu, most);
-  if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = most;
-  __syncthreads();
+  if (WARPS > 1) {
+    if (lane == 0) s_most[warp] = most;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; ++w) most = max(most, s_most[w]);
+    for (int w = 0; w < WARPS; ++w) most = max(most, s_most[warp / WARPS * WARPS + w]);
+    if (row >= rows) return;
+  }
   const float s = quant_scale<127, 8>(most);
-  const bool some = s > 0.f;
+  const bool some = s > 0.f;   // false: zeros, or not numbers
   const float inv = some ? __frcp_rn(s) : 0.f;
-  if (threadIdx.x == 0) scales[row] = s;
-  auto store = [&](int c, const float (&v)[8]) {
-    uint32_t w[2] = {0u, 0u};
+  if (first == 0) scales[row] = s;
+  auto store = [&](int c, const uint4& v) {
+    float f[VEC];
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e >> 2] |= (static_cast<uint32_t>(some ? quant_code<127>(v[e], s, inv) : 0) & 0xFFu) << (8 * (e & 3));
-    *reinterpret_cast<uint2*>(codes + row * cols + c) = make_uint2(w[0], w[1]);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(ST) == 4) {
+        f[i] = __uint_as_float(w[i]);
+      } else {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+    }
+    uint32_t b[VEC] = {};
+    if (some) quant_codes(f, s, inv, b);
+    uint32_t out[VEC / 4];
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i)
+      out[i] = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x0040), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x0040), 0x5410);
+    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(codes + row * cols + c) = make_uint2(out[0], out[1]);
+    else *reinterpret_cast<uint32_t*>(codes + row * cols + c) = out[0];
   };
 #pragma unroll
-  for (int u = 0; u < KEEP; ++u) {
-    const int c = (u * 256 + static_cast<int>(threadIdx.x)) * 8;
-    if (c < cols) store(c, keep[u]);
-  }
-  for (int c = (KEEP * 256 + static_cast<int>(threadIdx.x)) * 8; c < cols; c += 2048) {
-    float v[8];
-    q4_load8(src + c, v);
-    store(c, v);
-  }
+  for (int u = 0; u < KEEP; ++u)
+    if (first + u * STEP < cols) store(first + u * STEP, keep[u]);
+  for (int c = first + KEEP * STEP; c < cols; c += STEP) store(c, __ldg(reinterpret_cast<const uint4*>(src + c)));
 }
 
 // Where the columns of the product go: up to three column ranges, each a tensor [n, width] of its own.
 struct I8Out {
   void* ptr[3];
   int end[3];      // first column behind the range
-  int is_f32;
 };
 struct GemmI8Params {
+  const int8_t *x, *w;
   const float *sx, *sw;
   I8Out out;
   int M, N, K;
   int* status;
 };
+struct GemmI8Maps {   // x and w as bytes, and the results: boxes of 128 bytes by 32 rows, 128-byte swizzle
+  CUtensorMap a, b, out[3];
+};
 
+__device__ __forceinline__ int i8_range_of(const I8Out& o, int col) { return col < o.end[0] ? 0 : col < o.end[1] ? 1 : 2; }
+__device__ __forceinline__ int i8_range_begin(const I8Out& o, int r) { return r == 0 ? 0 : o.end[r - 1]; }
 // 8 columns from `col` (a multiple of 8, as are the ranges' ends) of row `row`.
+template <typename OT>
 __device__ __forceinline__ void i8_store8(const I8Out& o, size_t row, int col, const float (&y)[8]) {
-  const int r = col < o.end[0] ? 0 : col < o.end[1] ? 1 : 2;
-  const int begin = r == 0 ? 0 : o.end[r - 1];
-  const size_t at = row * (o.end[r] - begin) + (col - begin);
-  if (o.is_f32) q4_store8(static_cast<float*>(o.ptr[r]) + at, y);
-  else q4_store8(static_cast<__nv_bfloat16*>(o.ptr[r]) + at, y);
+  const int r = i8_range_of(o, col), begin = i8_range_begin(o, r);
+  q4_store8(static_cast<OT*>(o.ptr[r]) + row * (o.end[r] - begin) + (col - begin), y);
 }
+
+template <int BN_, int CG>
+struct GemmI8Traits {
+  static constexpr int BM = 128, BK = 128, B_ROWS = BN_ / CG;
+  static constexpr int A_BYTES = BM * BK, B_BYTES = B_ROWS * BK, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = B_ROWS == 256 ? 4 : B_ROWS == 128 ? 6 : 8;
+  static constexpr int OUT_BYTES = 32 * 128;                  // a warp's piece of the result, two a warp
+  static constexpr int SMEM_OUT = STAGES * STAGE_BYTES;
+  static constexpr int SMEM_BAR = SMEM_OUT + 8 * OUT_BYTES;
+  static constexpr int SMEM_MISC = SMEM_BAR + (2 * STAGES + 4) * 8;
+  static constexpr int SMEM_BYTES = SMEM_MISC + 16;
+  static constexpr int THREADS = 256;
+  static constexpr uint32_t TMEM_COLS = 2 * BN_;              // two accumulators
+};
 
 // The pipeline of gemm_bf16_sm100_kernel (y = x W^T) on bytes: a 128-byte row of a stage is 128 columns of K, an instruction of
 // kind::i8 takes 32 of them, and tensor memory holds 32-bit integers.  Persistent CTAs (or pairs, CG = 2) of
 //   warp 0: TMA loads   warp 1: tcgen05.mma   warp 2: tensor memory   warps 4-7: epilogue, a thread per row.
-template <int BN, int CG>
+// At twice bf16's rate a tile has half the time for its epilogue.  Stored from registers, 16 bytes of 32 rows at a time, results of
+// 2999 x 2048 -> 6144 took 71 us in fp32; so a warp turns pieces of 32 rows by 128 bytes round in shared memory and stores them
+// by TMA: whole lines, and no instructions of the epilogue's (XX us).
+template <int BN, int CG, typename OT>
 __global__ void __launch_bounds__(256, 1)
-gemm_i8_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const GemmI8Params prm) {
-  using T = GemmTraits<BN, CG>;
+gemm_i8_sm100_kernel(const __grid_constant__ GemmI8Maps maps, const GemmI8Params prm) {
+  using T = GemmI8Traits<BN, CG>;
   using namespace ptx;
-  constexpr int BK = 128;   // bytes
+  constexpr int BK = T::BK;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + T::SMEM_BAR);
   uint64_t* full = bars;
@@ -131,7 +169,7 @@ gemm_i8_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], CG == 2 ? 8 : 128);
+      mbar_init(&acc_empty[i], CG == 2 ? 8 : 4);   // one arrival per epilogue warp, of a pair of both CTAs
     }
     fence_mbar_init();
     fence_proxy_async_smem();
@@ -158,8 +196,8 @@ gemm_i8_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
     // nothing to do
   } else if (warp == 0) {
     if (elect_one()) {
-      prefetch_tensormap(&tmap_a);
-      prefetch_tensormap(&tmap_b);
+      prefetch_tensormap(&maps.a);
+      prefetch_tensormap(&maps.b);
       int it = 0;
       bool ok = true;
       for (int tile = first_tile; tile < n_tiles && ok; tile += tile_step) {
@@ -175,12 +213,12 @@ gemm_i8_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
           if (CG == 2) {   // the even CTA expects both CTAs' bytes
             if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * T::STAGE_BYTES);
             const uint32_t bar = cluster_addr(&full[st], 0);
-            tma_load_4d_2cta(sa, &tmap_a, bar, kb * BK, m0, 0, 0);
-            tma_load_4d_2cta(sb, &tmap_b, bar, kb * BK, n0, 0, 0);
+            tma_load_4d_2cta(sa, &maps.a, bar, kb * BK, m0, 0, 0);
+            tma_load_4d_2cta(sb, &maps.b, bar, kb * BK, n0, 0, 0);
           } else {
             mbar_arrive_expect_tx(&full[st], T::STAGE_BYTES);
-            tma_load_4d(sa, &tmap_a, &full[st], kb * BK, m0, 0, 0);
-            tma_load_4d(sb, &tmap_b, &full[st], kb * BK, n0, 0, 0);
+            tma_load_4d(sa, &maps.a, &full[st], kb * BK, m0, 0, 0);
+            tma_load_4d(sb, &maps.b, &full[st], kb * BK, n0, 0, 0);
           }
         }
       }
@@ -224,11 +262,12 @@ gemm_i8_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       }
     }
   } else if (warp >= 4) {
+    constexpr int W = 128 / sizeof(OT);      // columns of a piece
     const int row_in_tile = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    int t = 0;
+    uint8_t* pieces = smem + T::SMEM_OUT + (warp & 3) * 2 * T::OUT_BYTES;
+    int t = 0, piece = 0;
     bool ok = true;
-    uint32_t r[32];
     for (int tile = first_tile; tile < n_tiles && ok; tile += tile_step, ++t) {
       const int buf = t & 1;
       int tm, tn;
@@ -239,30 +278,68 @@ gemm_i8_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
+      if (m0 + (warp & 3) * 32 < prm.M) {
 #pragma unroll 1
-      for (int c = 0; c < BN / 32; ++c) {
-        tmem_ld_x32(t_lane + buf * BN + c * 32, r);
-        tmem_wait_ld();
+        for (int c = 0; c < BN / W; ++c) {
+          const int col0 = n0 + c * W;
+          if (col0 >= prm.N) break;
+          // a piece that lies in one range (what is behind the range's last column is cut off) goes through shared memory
+          const int range = i8_range_of(prm.out, col0), begin = i8_range_begin(prm.out, range);
+          const bool whole = min(col0 + W, prm.N) <= prm.out.end[range];
+          uint8_t* dst = pieces + (piece & 1) * T::OUT_BYTES + lane * 128;
+          if (whole) {
+            if (lane == 0) bulk_wait_group_read<1>();   // the piece before the last has left this buffer
+            __syncwarp();
+          }
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int col = n0 + c * 32 + v * 8;
-          if (row < prm.M && col < prm.N) {
-            float y[8], sw[8];
-            q4_load8(prm.sw + col, sw);
+          for (int half = 0; half < W / 32; ++half) {
+            uint32_t r[32];
+            tmem_ld_x32(t_lane + buf * BN + c * W + half * 32, r);
+            float4 sw[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = static_cast<float>(static_cast<int>(r[v * 8 + e])) * (sx * sw[e]);
-            i8_store8(prm.out, row, col, y);
+            for (int v = 0; v < 8; ++v) {
+              const int col = col0 + half * 32 + v * 4;
+              sw[v] = col < prm.N ? __ldg(reinterpret_cast<const float4*>(prm.sw + col)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            tmem_wait_ld();
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              const float f[8] = {sw[2 * v].x, sw[2 * v].y, sw[2 * v].z, sw[2 * v].w, sw[2 * v + 1].x, sw[2 * v + 1].y, sw[2 * v + 1].z, sw[2 * v + 1].w};
+              float y[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) y[e] = static_cast<float>(static_cast<int>(r[v * 8 + e])) * (sx * f[e]);
+              if (!whole) {
+                const int col = col0 + half * 32 + v * 8;
+                if (row < prm.M && col < prm.N) i8_store8<OT>(prm.out, row, col, y);
+              } else if constexpr (sizeof(OT) == 4) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                  *reinterpret_cast<float4*>(dst + (((2 * v + q) ^ (lane & 7)) << 4)) = make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+              } else {
+                *reinterpret_cast<uint4*>(dst + (((half * 4 + v) ^ (lane & 7)) << 4)) =
+                    make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+              }
+            }
+          }
+          if (whole) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_4d(&maps.out[range], pieces + (piece & 1) * T::OUT_BYTES, col0 - begin, m0 + (warp & 3) * 32, 0, 0);
+              bulk_commit_group();
+            }
+            ++piece;
           }
         }
       }
       tc_fence_before();
-      if (CG == 2) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(cluster_addr(&acc_empty[buf], 0));
-      } else {
-        mbar_arrive(&acc_empty[buf]);
+      __syncwarp();
+      if (lane == 0) {
+        if (CG == 2) mbar_arrive_cluster(cluster_addr(&acc_empty[buf], 0));
+        else mbar_arrive(&acc_empty[buf]);
       }
     }
+    if (lane == 0) bulk_wait_group_all();
   }
 
   __syncwarp();
@@ -281,6 +358,82 @@ gemm_i8_sm100_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_co
   } else if (warp == 2) {
     tc_fence_after();
     tmem_dealloc(tmem_base, T::TMEM_COLS);
+  }
+}
+
+__device__ __forceinline__ void mma_s8_16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// A handful of tokens: every SM streams weights, as gemm_skinny_kernel does for bf16 and for the same reason.  A CTA owns 16 channels,
+// its eight warps split K, a lane reads 16 bytes of a row at a time; the four lanes of a quad hold 64 consecutive k, in the same
+// order for channels and tokens.  NT: groups of 8 tokens.
+template <int NT, typename OT>
+__global__ void __launch_bounds__(256)
+gemm_i8_skinny_kernel(const GemmI8Params p) {
+  constexpr int WARPS = 8, U = NT <= 2 ? 4 : 2, TOK = NT * 8, ROWS = 16;
+  __shared__ int part[WARPS][ROWS][TOK + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int r0 = blockIdx.x * ROWS;
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch();
+  int acc[NT][4];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[j][e] = 0;
+  const int steps = (p.K + 63) >> 6;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  for (int s0 = warp * U; s0 < steps; s0 += WARPS * U) {
+    uint4 a[U][2], b[U][NT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = (s0 + u) * 64 + t * 16;
+      const bool ok = k < p.K;    // K is a multiple of 16
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = r0 + h * 8 + g;
+        a[u][h] = (ok && row < p.N) ? __ldg(reinterpret_cast<const uint4*>(p.w + static_cast<size_t>(row) * p.K + k)) : zero;
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int tok = j * 8 + g;
+        b[u][j] = (ok && tok < p.M) ? *reinterpret_cast<const uint4*>(p.x + static_cast<size_t>(tok) * p.K + k) : zero;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        mma_s8_16832(acc[j], a[u][0].x, a[u][1].x, a[u][0].y, a[u][1].y, b[u][j].x, b[u][j].y);
+        mma_s8_16832(acc[j], a[u][0].z, a[u][1].z, a[u][0].w, a[u][1].w, b[u][j].z, b[u][j].w);
+      }
+  }
+  // c0, c1: row g, tokens 2t, 2t + 1; c2, c3: row g + 8
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[warp][(e >> 1) * 8 + g][j * 8 + t * 2 + (e & 1)] = acc[j][e];
+  __syncthreads();
+  // a thread finishes pairs of neighbouring columns of y, which lie in one range
+  for (int idx = threadIdx.x; idx < TOK * (ROWS / 2); idx += 256) {
+    const int tok = idx / (ROWS / 2), pr = idx - tok * (ROWS / 2);
+    const int col = r0 + 2 * pr;
+    if (tok >= p.M || col >= p.N) continue;
+    int v0 = 0, v1 = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      v0 += part[w][2 * pr][tok];
+      v1 += part[w][2 * pr + 1][tok];
+    }
+    const float sx = p.sx[tok], y0 = static_cast<float>(v0) * (sx * p.sw[col]), y1 = static_cast<float>(v1) * (sx * p.sw[col + 1]);
+    const int r = i8_range_of(p.out, col), begin = i8_range_begin(p.out, r);
+    OT* dst = static_cast<OT*>(p.out.ptr[r]) + static_cast<size_t>(tok) * (p.out.end[r] - begin) + (col - begin);
+    if constexpr (sizeof(OT) == 4) *reinterpret_cast<float2*>(dst) = make_float2(y0, y1);
+    else *reinterpret_cast<uint32_t*>(dst) = ptx::pack_bf16(y0, y1);
   }
 }
 

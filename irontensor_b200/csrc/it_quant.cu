@@ -4,7 +4,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 #include <type_traits>
 
 #include "fa_decode_q4.cuh"
@@ -36,10 +35,23 @@ it_status check_cache(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t B,
   return IT_OK;
 }
 
-// CTAs of 256 threads for so many threads; 0 where a launch does not hold them.
-unsigned ctas_of(double threads) {
-  const double n = std::ceil(threads / 256.0);
-  return n <= 2147483647.0 ? static_cast<unsigned>(n) : 0u;
+// The grid of the kernels that write and read a cache (kv_q4.cuh).
+it_status cache_grid(int B, int tokens, int Hkv, int D, dim3* grid) {
+  const int64_t rows = static_cast<int64_t>(tokens) * Hkv, per_cta = 256 / (4 * ((D + 31) / 32));
+  if (rows > 0x7fffffffLL - per_cta) return fail(IT_ERR_UNSUPPORTED_SHAPE, "tokens * kv_heads must be below 2^31");
+  *grid = dim3(static_cast<unsigned>((rows + per_cta - 1) / per_cta), std::min(B, 65535), 2);
+  return IT_OK;
+}
+
+// f(groups of 32 columns as a constant)
+template <typename F>
+it_status by_groups(int D, F&& f) {
+  switch ((D + 31) / 32) {
+    case 1: return f(std::integral_constant<int, 1>{});
+    case 2: return f(std::integral_constant<int, 2>{});
+    case 3: return f(std::integral_constant<int, 3>{});
+    default: return f(std::integral_constant<int, 4>{});
+  }
 }
 
 // How many clusters of `size` CTAs of a kernel are resident at once (asked once per kernel, device and size).
@@ -159,18 +171,20 @@ it_status it_kv_cache_q4_append(it_ctx* ctx, it_stream* stream, it_dtype dtype, 
   if (lengths == new_lengths || counts == new_lengths) return fail(IT_ERR_INVALID_ARG, "new_lengths must be another array than lengths and counts");
   if (T > 0 && (k == nullptr || v == nullptr)) return fail(IT_ERR_INVALID_ARG, "null tensor");
   if (!aligned16(k) || !aligned16(v)) return fail(IT_ERR_ALIGNMENT, "k and v must be 16-byte aligned");
-  const int lanes = 4 * ((D + 31) / 32);
-  const unsigned ctas = ctas_of(std::max(2.0 * B * T * Hkv * lanes, static_cast<double>(B)));
-  if (ctas == 0) return fail(IT_ERR_UNSUPPORTED_SHAPE, "too many tokens");
+  dim3 grid;
+  if ((st = cache_grid(B, std::max(T, 1), Hkv, D, &grid)) != IT_OK) return st;
   IT_CUDA(cudaSetDevice(ctx->device));
   auto launch = [&](auto kernel, auto* kk, auto* vv) -> it_status {
-    IT_CUDA(launch_dependent(kernel, ctas, 256, 0, stream->s, kk, vv, half_of(k_codes, k_scales), half_of(v_codes, v_scales), lengths, counts,
+    IT_CUDA(launch_dependent(kernel, grid, 256, 0, stream->s, kk, vv, half_of(k_codes, k_scales), half_of(v_codes, v_scales), lengths, counts,
                              new_lengths, B, T, Hkv, D, max_len, ctx->d_status));
     ctx->launches += 1;
     return IT_OK;
   };
-  return dtype == IT_F32 ? launch(it::kv_q4_append_kernel<float>, static_cast<const float*>(k), static_cast<const float*>(v))
-                         : launch(it::kv_q4_append_kernel<__nv_bfloat16>, static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v));
+  return by_groups(D, [&](auto ng) {
+    constexpr int NG = decltype(ng)::value;
+    return dtype == IT_F32 ? launch(it::kv_q4_append_kernel<float, NG>, static_cast<const float*>(k), static_cast<const float*>(v))
+                           : launch(it::kv_q4_append_kernel<__nv_bfloat16, NG>, static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v));
+  });
 }
 
 it_status it_kv_cache_q4_read(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t B, int32_t T, int32_t Hkv, int32_t D, int32_t max_len,
@@ -180,17 +194,20 @@ it_status it_kv_cache_q4_read(it_ctx* ctx, it_stream* stream, it_dtype dtype, in
   if (st != IT_OK || B == 0 || T == 0) return st;
   if (k == nullptr || v == nullptr) return fail(IT_ERR_INVALID_ARG, "null tensor");
   if (!aligned16(k) || !aligned16(v)) return fail(IT_ERR_ALIGNMENT, "k and v must be 16-byte aligned");
-  const unsigned ctas = ctas_of(2.0 * B * T * Hkv * (D / 8));
-  if (ctas == 0) return fail(IT_ERR_UNSUPPORTED_SHAPE, "too many tokens");
+  dim3 grid;
+  if ((st = cache_grid(B, T, Hkv, D, &grid)) != IT_OK) return st;
   IT_CUDA(cudaSetDevice(ctx->device));
   auto launch = [&](auto kernel, auto* kk, auto* vv) -> it_status {
-    IT_CUDA(launch_dependent(kernel, ctas, 256, 0, stream->s, kk, vv, half_of(k_codes, k_scales), half_of(v_codes, v_scales), starts, lengths, B, T,
+    IT_CUDA(launch_dependent(kernel, grid, 256, 0, stream->s, kk, vv, half_of(k_codes, k_scales), half_of(v_codes, v_scales), starts, lengths, B, T,
                              Hkv, D, max_len));
     ctx->launches += 1;
     return IT_OK;
   };
-  return dtype == IT_F32 ? launch(it::kv_q4_read_kernel<float>, static_cast<float*>(k), static_cast<float*>(v))
-                         : launch(it::kv_q4_read_kernel<__nv_bfloat16>, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v));
+  return by_groups(D, [&](auto ng) {
+    constexpr int NG = decltype(ng)::value;
+    return dtype == IT_F32 ? launch(it::kv_q4_read_kernel<float, NG>, static_cast<float*>(k), static_cast<float*>(v))
+                           : launch(it::kv_q4_read_kernel<__nv_bfloat16, NG>, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v));
+  });
 }
 
 it_status it_attention_decode_q4_workspace_bytes(int32_t B, int32_t H, int32_t D, size_t* out_bytes) {
@@ -259,8 +276,6 @@ it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype,
     static std::atomic<int> at_once[16][9];
     choose_decode_q4_plan(pairs, B, max_len, ctx->sm_count, resident / ctx->sm_count, NG,
                           [&](int size) { return clusters_at_once(in_clusters, size, 32 * warps, bytes, at_once[ctx->device & 15][size]); }, &n, &even);
-    if (getenv("DQ_PLAN")) even = atoi(getenv("DQ_PLAN"));
-    if (getenv("DQ_N")) n = atoi(getenv("DQ_N"));
     p.n_splits = n;
     const dim3 grid = even ? dim3(std::min(resident, wide ? it::DQ_MAX_CTAS / 2 : it::DQ_MAX_CTAS)) : dim3(n, Hkv * chunks, B);
     if (!even) {
@@ -276,17 +291,13 @@ it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype,
     ctx->launches += 2;
     return IT_OK;
   };
-  auto by_groups = [&](auto terms, auto hd) -> it_status {
-    switch ((D + 31) / 32) {
-      case 1: return main_launch(std::integral_constant<int, 1>{}, terms, hd);
-      case 2: return main_launch(std::integral_constant<int, 2>{}, terms, hd);
-      case 3: return main_launch(std::integral_constant<int, 3>{}, terms, hd);
-      default: return main_launch(std::integral_constant<int, 4>{}, terms, hd);
-    }
-  };
   using one = std::integral_constant<int, 1>;
-  if (dtype == IT_F32) return by_groups(std::integral_constant<int, 3>{}, std::integral_constant<int, 8>{});
-  return wide ? by_groups(one{}, std::integral_constant<int, 16>{}) : by_groups(one{}, std::integral_constant<int, 8>{});
+  using three = std::integral_constant<int, 3>;
+  using eight = std::integral_constant<int, 8>;
+  return by_groups(D, [&](auto ng) {
+    if (dtype == IT_F32) return main_launch(ng, three{}, eight{});
+    return wide ? main_launch(ng, one{}, std::integral_constant<int, 16>{}) : main_launch(ng, one{}, eight{});
+  });
 }
 
 it_status it_quantize_rows_i8(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t rows, int32_t cols, const void* x, int8_t* codes,
@@ -299,46 +310,86 @@ it_status it_quantize_rows_i8(it_ctx* ctx, it_stream* stream, it_dtype dtype, in
   if (x == nullptr || codes == nullptr || scales == nullptr) return fail(IT_ERR_INVALID_ARG, "null tensor");
   if (!aligned16(x) || !aligned16(codes)) return fail(IT_ERR_ALIGNMENT, "x and codes must be 16-byte aligned");
   IT_CUDA(cudaSetDevice(ctx->device));
+  // Warps of a row: one where that makes as many warps as keep the memory busy, and as many as a short row has work for
+  const int vec = dtype == IT_F32 ? 4 : 8;
+  int warps = 1;
+  while (warps < 8 && (static_cast<int64_t>(rows) * warps < 16LL * ctx->sm_count || cols > 8 * 32 * vec * warps) && cols > 32 * vec * warps) warps *= 2;
   auto launch = [&](auto kernel, auto* src) -> it_status {
-    IT_CUDA(launch_dependent(kernel, static_cast<unsigned>(rows), 256, 0, stream->s, src, codes, scales, cols));
+    IT_CUDA(launch_dependent(kernel, static_cast<unsigned>((static_cast<int64_t>(rows) * warps + 7) / 8), 256, 0, stream->s, src, codes, scales, rows,
+                             cols));
     ctx->launches += 1;
     return IT_OK;
   };
-  return dtype == IT_F32 ? launch(it::quantize_rows_kernel<float>, static_cast<const float*>(x))
-                         : launch(it::quantize_rows_kernel<__nv_bfloat16>, static_cast<const __nv_bfloat16*>(x));
+  auto by_warps = [&](auto* src) -> it_status {
+    using ST = std::remove_const_t<std::remove_pointer_t<decltype(src)>>;
+    return warps == 1 ? launch(it::quantize_rows_kernel<ST, 1>, src) : warps == 2 ? launch(it::quantize_rows_kernel<ST, 2>, src)
+           : warps == 4 ? launch(it::quantize_rows_kernel<ST, 4>, src) : launch(it::quantize_rows_kernel<ST, 8>, src);
+  };
+  return dtype == IT_F32 ? by_warps(static_cast<const float*>(x)) : by_warps(static_cast<const __nv_bfloat16*>(x));
 }
 
 }  // extern "C"
 
 namespace {
 
-// [rows, K] bytes as TMA sees them: boxes of 128 columns by `box_rows` rows, 128-byte swizzle, zeros outside.
-it_status make_bytes_map(it_ctx* ctx, CUtensorMap* map, const void* base, int rows, int K, int box_rows) {
-  const cuuint64_t n = static_cast<cuuint64_t>(rows), k = static_cast<cuuint64_t>(K);
-  const cuuint64_t dims[4] = {k, n, 1, 1}, strides[3] = {k, k * n, k * n};
-  const cuuint32_t box[4] = {128, static_cast<cuuint32_t>(box_rows), 1, 1}, estr[4] = {1, 1, 1, 1};
-  const CUresult r = ctx->encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, estr,
-                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+// [rows, cols] as TMA sees them: boxes of 128 bytes by `box_rows` rows, 128-byte swizzle, zeros outside.
+it_status make_rows_map(it_ctx* ctx, CUtensorMap* map, CUtensorMapDataType type, int bytes, const void* base, int rows, int cols, int box_rows) {
+  const cuuint64_t n = static_cast<cuuint64_t>(rows), c = static_cast<cuuint64_t>(cols);
+  const cuuint64_t dims[4] = {c, n, 1, 1}, strides[3] = {c * bytes, c * n * bytes, c * n * bytes};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(128 / bytes), static_cast<cuuint32_t>(box_rows), 1, 1}, estr[4] = {1, 1, 1, 1};
+  const CUresult r = ctx->encode(map, type, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? IT_OK : fail(IT_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", static_cast<int>(r));
 }
 
-template <int BN, int CG>
-it_status launch_gemm_i8(it_ctx* ctx, cudaStream_t s, const int8_t* x, const int8_t* w, it::GemmI8Params p) {
-  using T = it::GemmTraits<BN, CG>;
-  CUtensorMap ma, mb;
+template <int BN, int CG, typename OT>
+it_status launch_gemm_i8(it_ctx* ctx, cudaStream_t s, const it::GemmI8Params& p) {
+  using T = it::GemmI8Traits<BN, CG>;
+  it::GemmI8Maps maps;
   it_status st;
-  if ((st = make_bytes_map(ctx, &ma, x, p.M, p.K, T::BM)) != IT_OK || (st = make_bytes_map(ctx, &mb, w, p.N, p.K, T::B_ROWS)) != IT_OK) return st;
+  if ((st = make_rows_map(ctx, &maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.x, p.M, p.K, T::BM)) != IT_OK) return st;
+  if ((st = make_rows_map(ctx, &maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.N, p.K, T::B_ROWS)) != IT_OK) return st;
+  const auto type = sizeof(OT) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  for (int r = 2; r >= 0; --r) {
+    const int width = p.out.end[r] - (r > 0 ? p.out.end[r - 1] : 0);
+    if (width > 0 && (st = make_rows_map(ctx, &maps.out[r], type, sizeof(OT), p.out.ptr[r], p.M, width, 32)) != IT_OK) return st;
+    if (width == 0) maps.out[r] = maps.a;   // never used
+  }
   static std::atomic<bool> attr_set[16];
   if (!attr_set[ctx->device & 15]) {
-    IT_CUDA(cudaFuncSetAttribute(it::gemm_i8_sm100_kernel<BN, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM_BYTES));
+    IT_CUDA(cudaFuncSetAttribute(it::gemm_i8_sm100_kernel<BN, CG, OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM_BYTES));
     attr_set[ctx->device & 15] = true;
   }
   const long long tiles = static_cast<long long>((p.M + CG * T::BM - 1) / (CG * T::BM)) * ((p.N + BN - 1) / BN);
   const int grid = static_cast<int>(std::min<long long>(tiles, ctx->sm_count / CG)) * CG;
-  IT_CUDA(launch_cluster(it::gemm_i8_sm100_kernel<BN, CG>, grid, T::THREADS, T::SMEM_BYTES, s, CG, ma, mb, p));
+  IT_CUDA(launch_cluster(it::gemm_i8_sm100_kernel<BN, CG, OT>, grid, T::THREADS, T::SMEM_BYTES, s, CG, maps, p));
   ctx->launches += 1;
   return IT_OK;
+}
+
+// Up to 16 tokens stream the weights (gemm_i8_skinny_kernel; 16 x 4096 -> 12288: 17.6 us, in 128-column tiles 20.6; 32 x 4096 -> 4096:
+// 10.8 and, in 64-column tiles, 8.8).  Above that the tile is the one with the least 4 + waves * (a + b K / 1024) us, fitted to
+// 300 x 4096 -> 12288 (27, 21, 23 and 29 us with 64, 128 and 256 columns and pairs of CTAs of 256 x 256), 512 x 4096 -> 4096 (15, 12, 17
+// and 17), 2999 x 2048 -> 6144 (52, 35, 31 and 33), 8192 x 4096 -> 12288 (488, 338, 306 and 249: 3.3 POP/s), 8192 x 512 -> 1536 (20, 20,
+// 18 and 20).
+template <typename OT>
+it_status launch_linear_i8(it_ctx* ctx, cudaStream_t s, const it::GemmI8Params& p) {
+  if (p.M <= 16) {
+    const auto kernel = p.M <= 8 ? it::gemm_i8_skinny_kernel<1, OT> : it::gemm_i8_skinny_kernel<2, OT>;
+    IT_CUDA(launch_dependent(kernel, static_cast<unsigned>((p.N + 15) / 16), 256, 0, s, p));
+    ctx->launches += 1;
+    return IT_OK;
+  }
+  auto cost = [&](int rows, int columns, int at_once, double a, double b) {
+    const long long tiles = static_cast<long long>((p.M + rows - 1) / rows) * ((p.N + columns - 1) / columns);
+    return static_cast<double>((tiles + at_once - 1) / at_once) * (a + b * p.K / 1024.0);
+  };
+  const double c64 = cost(128, 64, ctx->sm_count, 1.0, 1.1), c128 = cost(128, 128, ctx->sm_count, 2.0, 1.45), c256 = cost(128, 256, ctx->sm_count, 3.6, 2.6);
+  const double c_pair = cost(256, 256, std::max(1, ctx->sm_count / 2), 4.5, 1.9), best = std::min(std::min(c64, c128), std::min(c256, c_pair));
+  if (best == c64) return launch_gemm_i8<64, 1, OT>(ctx, s, p);
+  if (best == c128) return launch_gemm_i8<128, 1, OT>(ctx, s, p);
+  if (best == c256) return launch_gemm_i8<256, 1, OT>(ctx, s, p);
+  return launch_gemm_i8<256, 2, OT>(ctx, s, p);
 }
 
 }  // namespace
@@ -373,17 +424,13 @@ extern "C" it_status it_linear_i8_fwd(it_ctx* ctx, it_stream* stream, it_dtype o
   if (!aligned16(x_codes) || !aligned16(w_codes) || !aligned16(w_scales))
     return fail(IT_ERR_ALIGNMENT, "codes and weight scales must be 16-byte aligned");
   IT_CUDA(cudaSetDevice(ctx->device));
+  p.x = x_codes;
+  p.w = w_codes;
   p.sx = x_scales;
   p.sw = w_scales;
-  p.out.is_f32 = out_dtype == IT_F32;
   p.M = n;
   p.N = out_dim;
   p.K = in_dim;
   p.status = ctx->d_status;
-  const int bn = getenv("I8_TILE") ? atoi(getenv("I8_TILE")) : 128;
-  if (bn == 512) return launch_gemm_i8<256, 2>(ctx, stream->s, x_codes, w_codes, p);
-  if (bn == 384) return launch_gemm_i8<128, 2>(ctx, stream->s, x_codes, w_codes, p);
-  if (bn == 256) return launch_gemm_i8<256, 1>(ctx, stream->s, x_codes, w_codes, p);
-  if (bn == 64) return launch_gemm_i8<64, 1>(ctx, stream->s, x_codes, w_codes, p);
-  return launch_gemm_i8<128, 1>(ctx, stream->s, x_codes, w_codes, p);
+  return out_dtype == IT_F32 ? launch_linear_i8<float>(ctx, stream->s, p) : launch_linear_i8<__nv_bfloat16>(ctx, stream->s, p);
 }

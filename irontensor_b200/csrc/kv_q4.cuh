@@ -41,17 +41,61 @@ __device__ __forceinline__ float quant_scale(uint32_t largest_bits) {
   return __uint_as_float(base + (up ? MASK + 1u : 0u));
 }
 
-// round(x / s), ties to even, for s of at most 8 significant bits; inv = 1 / s.  x * inv may be a step off next to the middle of
-// two whole numbers; x - q s is exact there (at most 24 bits above the last place of x) and says which is nearer.
-template <int MOST>
-__device__ __forceinline__ int quant_code(float x, float s, float inv) {
-  float q = rintf(x * inv);
-  const float r = fmaf(-q, s, x), half = 0.5f * s;
-  const bool odd = static_cast<int>(q) & 1;
-  if (r > half || (r == half && odd)) q += 1.f;
-  else if (r < -half || (r == -half && odd)) q -= 1.f;
-  return static_cast<int>(fminf(fmaxf(q, -static_cast<float>(MOST)), static_cast<float>(MOST)));
+// round(x / s), ties to even, in the low byte of each c, for s of at most 8 significant bits and quotients of less than 127.5; inv =
+// 1 / s.  The whole number q comes out of the low bits of a sum with 1.5 * 2^23, rounded once.  x * inv may be off by a last
+// place, which matters next to the middle of two whole numbers: there x - q s, exact (at most 24 bits above the last place of x),
+// says which is nearer.  That is rare, and asked once for all N.
+template <int N>
+__device__ __forceinline__ void quant_codes(const float (&x)[N], float s, float inv, uint32_t (&c)[N]) {
+  constexpr float MAGIC = 12582912.f;
+  const float half = 0.5f * s;
+  bool close = false;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float y = fmaf(x[e], inv, MAGIC);
+    c[e] = __float_as_uint(y);
+    close |= fabsf(fmaf(-(y - MAGIC), s, x[e])) >= half;
+  }
+  if (close) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float r = fmaf(-(__uint_as_float(c[e]) - MAGIC), s, x[e]);
+      if (fabsf(r) > half || (fabsf(r) == half && (c[e] & 1u))) c[e] += r > 0.f ? 1u : 0xFFFFFFFFu;
+    }
+  }
 }
+
+__device__ __forceinline__ uint32_t q4_fma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t q4_mul2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// (x & MASK) | magic in one instruction.  It takes one constant in itself and no second one, so `magic` comes in a register; left to
+// itself the compiler makes two instructions of it, and attention waits for the unit that executes them.
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t q4_and_or(uint32_t x, uint32_t magic) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "n"(MASK), "r"(magic));
+  return d;
+}
+__device__ __forceinline__ uint32_t q4_constant(uint32_t c) {   // one that the compiler does not see through
+  uint32_t d;
+  asm volatile("mov.b32 %0, %1;" : "=r"(d) : "r"(c));
+  return d;
+}
+// Nibble I of both halves of w as the values (16 + u) s - 24 s.
+template <int I>
+__device__ __forceinline__ uint32_t q4_pair(uint32_t w, uint32_t s2, uint32_t bias2, uint32_t magic) {
+  const uint32_t at3 = I == 0 ? w << 3 : w >> (4 * I - 3);
+  return q4_fma2(q4_and_or<0x00780078u>(at3, magic), s2, bias2);
+}
+constexpr uint32_t Q4_MAGIC = 0x41804180u;       // 16 in both halves
+constexpr uint32_t Q4_MINUS_24 = 0xC1C0C1C0u;
 
 constexpr float Q4_MOST_SCALE = 0x1p122f;   // 24 * s, which attention's operands are made with, stays finite
 
@@ -83,92 +127,111 @@ __device__ __forceinline__ void q4_store8(float* p, const float (&x)[8]) {
   *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
 }
 
-// New tokens k, v [batch, T, kv_heads, head_dim] into the cache behind the lengths[b] positions that are there; of sequence b the
-// first counts[b] tokens (null: all T).  new_lengths[b] = what is there afterwards.  A thread takes 8 columns, the quad that shares
-// a group finds its largest magnitude by two shuffles.  Positions outside the cache are not written, and reported.
-// Reads 2 * 8 or 4 * 8 bytes a thread and writes 4.5: bound by memory, and for single tokens by the launch.
-template <typename ST>
-__global__ void __launch_bounds__(256)
-kv_q4_append_kernel(const ST* __restrict__ k, const ST* __restrict__ v, KvQ4 ck, KvQ4 cv, const int* __restrict__ lengths,
-                    const int* __restrict__ counts, int* __restrict__ new_lengths, int B, int T, int Hkv, int D, int max_len, int* status) {
-  const int groups = (D + 31) >> 5, lanes = 4 * groups;   // threads of a row
-  ptx::grid_dep_wait();
-  ptx::grid_dep_launch();
-  const long long rows = static_cast<long long>(B) * T * Hkv, total = 2 * rows * lanes;
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (i < B) {
-    const int have = lengths[i], want = counts != nullptr ? counts[i] : T, add = min(max(want, 0), T);
-    const long long end = static_cast<long long>(have) + add;
-    if (have < 0 || end > max_len || add != want) atomicCAS(status, 0, DEV_ERR_CACHE_RANGE);
-    new_lengths[i] = static_cast<int>(min(max(end, 0LL), static_cast<long long>(max_len)));
-  }
-  const bool live = i < total;   // a quad is live as a whole; its warp stays together for the shuffles
-  const long long at = live ? i : 0;
-  const bool is_v = at >= rows * lanes;
-  const long long in_half = is_v ? at - rows * lanes : at;
-  const long long row = in_half / lanes;
-  const int lane = static_cast<int>(in_half - row * lanes), j = lane >> 2, t = lane & 3;
-  const int h = static_cast<int>(row % Hkv);
-  const long long bt = row / Hkv;
-  const int b = static_cast<int>(bt / T), tok = static_cast<int>(bt - static_cast<long long>(b) * T);
-  const int d0 = 32 * j + 8 * t;
-  float x[8] = {};
-  if (live && d0 < D) q4_load8((is_v ? v : k) + row * D + d0, x);
+// What 8 columns of a thread become: the word of their codes, and the group's scale.  The threads of a quad hold a group.
+__device__ __forceinline__ uint32_t q4_quantise(const float (&x)[8], float* scale) {
   uint32_t largest = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) largest = max(largest, __float_as_uint(x[e]) & 0x7FFFFFFFu);
   largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
   largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
   float s = quant_scale<7, 5>(largest);
-  if (s > Q4_MOST_SCALE) s = Q4_MOST_SCALE;
-  const bool some = s > 0.f;   // false for NaN too
-  const float inv = some ? __frcp_rn(s) : 0.f;
-  uint32_t word = 0;
+  const bool saturates = s > Q4_MOST_SCALE;
+  if (saturates) s = Q4_MOST_SCALE;
+  *scale = s;
+  if (!(s > 0.f)) return 0x88888888u;   // zeros, or not numbers
+  const float inv = __frcp_rn(s);
+  float y[8];
+  uint32_t c[8], word = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int c = some ? quant_code<7>(x[e], s, inv) : 0;
-    word |= static_cast<uint32_t>(c + 8) << (4 * (e >> 1) + 16 * (e & 1));
+  for (int e = 0; e < 8; ++e) y[e] = saturates ? fminf(fmaxf(x[e], -7.f * s), 7.f * s) : x[e];
+  quant_codes(y, s, inv, c);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) word |= ((c[e] + 8u) & 15u) << (4 * (e >> 1) + 16 * (e & 1));
+  return word;
+}
+
+// New tokens k, v [batch, T, kv_heads, head_dim] into the cache behind the lengths[b] positions that are there; of sequence b the
+// first counts[b] tokens (null: all T).  new_lengths[b] = what is there afterwards.  Grid (rows, batch, keys or values); a
+// thread takes 8 columns.  Positions outside the cache are not written, and reported.
+// Reads 2 * 8 or 4 * 8 bytes a thread and writes 4.5: bound by memory, and for single tokens by the launch.
+template <typename ST, int NG>
+__global__ void __launch_bounds__(256)
+kv_q4_append_kernel(const ST* __restrict__ k, const ST* __restrict__ v, KvQ4 ck, KvQ4 cv, const int* __restrict__ lengths,
+                    const int* __restrict__ counts, int* __restrict__ new_lengths, int B, int T, int Hkv, int D, int max_len, int* status) {
+  constexpr int LANES = 4 * NG, ROWS = 256 / LANES;   // threads of a row, rows of a CTA
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch();
+  const int in_cta = static_cast<int>(threadIdx.x) / LANES, lane = static_cast<int>(threadIdx.x) % LANES, j = lane >> 2, t = lane & 3;
+  const uint32_t row = blockIdx.x * ROWS + in_cta;    // of the sequence: token and head
+  const int tok = static_cast<int>(row / static_cast<uint32_t>(Hkv)), h = static_cast<int>(row - static_cast<uint32_t>(tok) * Hkv);
+  const int d0 = 32 * j + 8 * t;
+  const ST* src = blockIdx.z ? v : k;
+  const KvQ4& c = blockIdx.z ? cv : ck;
+  for (int b = blockIdx.y; b < B; b += static_cast<int>(gridDim.y)) {
+    const int have = lengths[b], want = counts != nullptr ? counts[b] : T, add = min(max(want, 0), T);
+    if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) {
+      const long long end = static_cast<long long>(have) + add;
+      if (have < 0 || end > max_len || add != want) atomicCAS(status, 0, DEV_ERR_CACHE_RANGE);
+      new_lengths[b] = static_cast<int>(min(max(end, 0LL), static_cast<long long>(max_len)));
+    }
+    const long long pos = static_cast<long long>(have) + tok;
+    const bool live = in_cta < ROWS && tok < add && pos >= 0 && pos < max_len;
+    if (!__any_sync(0xffffffffu, live)) continue;
+    float x[8] = {};
+    if (live && d0 < D) q4_load8(src + ((static_cast<size_t>(b) * T + tok) * Hkv + h) * D + d0, x);
+    float s;
+    const uint32_t word = q4_quantise(x, &s);
+    if (live) {
+      const size_t crow = (static_cast<size_t>(b) * Hkv + h) * max_len + pos;
+      c.codes[crow * LANES + t * NG + j] = word;
+      if (t == 0) c.scales[crow * NG + j] = __float2bfloat16_rn(s);
+    }
   }
-  if (!live || tok >= (counts != nullptr ? counts[b] : T)) return;
-  const long long pos = static_cast<long long>(lengths[b]) + tok;
-  if (pos < 0 || pos >= max_len) return;
-  const long long crow = (static_cast<long long>(b) * Hkv + h) * max_len + pos;
-  const KvQ4& c = is_v ? cv : ck;
-  c.codes[crow * lanes + t * groups + j] = word;
-  if (t == 0) c.scales[crow * groups + j] = __float2bfloat16_rn(s);
 }
 
 // Positions starts[b] + t, t < T, of the cache (null: from 0) as keys and values [batch, T, kv_heads, head_dim]; zeros outside
-// 0 <= position < min(lengths[b], max_len) (null: max_len).  A thread writes 8 columns.  Bound by the bytes that it writes.
-template <typename ST>
+// 0 <= position < min(lengths[b], max_len) (null: max_len).  Grid as above; a thread writes 8 columns.  Bound by the bytes that it
+// writes.
+template <typename ST, int NG>
 __global__ void __launch_bounds__(256)
 kv_q4_read_kernel(ST* __restrict__ k, ST* __restrict__ v, KvQ4 ck, KvQ4 cv, const int* __restrict__ starts, const int* __restrict__ lengths,
                   int B, int T, int Hkv, int D, int max_len) {
-  const int groups = (D + 31) >> 5, per_row = D >> 3;   // threads of a row: none for a padded group's empty columns
+  constexpr int LANES = 4 * NG, ROWS = 256 / LANES;
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
-  const long long rows = static_cast<long long>(B) * T * Hkv, total = 2 * rows * per_row;
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= total) return;
-  const bool is_v = i >= rows * per_row;
-  const long long in_half = is_v ? i - rows * per_row : i;
-  const long long row = in_half / per_row;
-  const int oct = static_cast<int>(in_half - row * per_row), j = oct >> 2, t = oct & 3;
-  const int h = static_cast<int>(row % Hkv);
-  const long long bt = row / Hkv;
-  const int b = static_cast<int>(bt / T), tok = static_cast<int>(bt - static_cast<long long>(b) * T);
-  const long long pos = static_cast<long long>(starts != nullptr ? starts[b] : 0) + tok;
-  const int end = lengths != nullptr ? min(lengths[b], max_len) : max_len;
-  float x[8] = {};
-  if (pos >= 0 && pos < end) {
-    const long long crow = (static_cast<long long>(b) * Hkv + h) * max_len + pos;
-    const KvQ4& c = is_v ? cv : ck;
-    const uint32_t w = __ldg(c.codes + crow * 4 * groups + t * groups + j);
-    const float s = __bfloat162float(c.scales[crow * groups + j]);
+  const int in_cta = static_cast<int>(threadIdx.x) / LANES, lane = static_cast<int>(threadIdx.x) % LANES, j = lane >> 2, t = lane & 3;
+  const uint32_t row = blockIdx.x * ROWS + in_cta;
+  const int tok = static_cast<int>(row / static_cast<uint32_t>(Hkv)), h = static_cast<int>(row - static_cast<uint32_t>(tok) * Hkv);
+  const int d0 = 32 * j + 8 * t;
+  if (in_cta >= ROWS || tok >= T || d0 >= D) return;
+  ST* dst = blockIdx.z ? v : k;
+  const KvQ4& c = blockIdx.z ? cv : ck;
+  for (int b = blockIdx.y; b < B; b += static_cast<int>(gridDim.y)) {
+    const long long pos = static_cast<long long>(starts != nullptr ? starts[b] : 0) + tok;
+    const int end = lengths != nullptr ? min(lengths[b], max_len) : max_len;
+    uint32_t x[4] = {0u, 0u, 0u, 0u};   // pairs of neighbouring columns
+    if (pos >= 0 && pos < end) {
+      const size_t crow = (static_cast<size_t>(b) * Hkv + h) * max_len + pos;
+      const uint32_t w = __ldg(c.codes + crow * LANES + t * NG + j);
+      const uint32_t s2 = __byte_perm(*reinterpret_cast<const unsigned short*>(c.scales + crow * NG + j), 0, 0x1010), bias2 = q4_mul2(s2, Q4_MINUS_24);
+      x[0] = q4_pair<0>(w, s2, bias2, Q4_MAGIC);
+      x[1] = q4_pair<1>(w, s2, bias2, Q4_MAGIC);
+      x[2] = q4_pair<2>(w, s2, bias2, Q4_MAGIC);
+      x[3] = q4_pair<3>(w, s2, bias2, Q4_MAGIC);
+    }
+    ST* at = dst + ((static_cast<size_t>(b) * T + tok) * Hkv + h) * D + d0;
+    if constexpr (sizeof(ST) == 2) {
+      *reinterpret_cast<uint4*>(at) = make_uint4(x[0], x[1], x[2], x[3]);
+    } else {
+      float f[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = s * static_cast<float>(static_cast<int>((w >> (4 * (e >> 1) + 16 * (e & 1))) & 15u) - 8);
+      for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(x[i] << 16);
+        f[2 * i + 1] = __uint_as_float(x[i] & 0xFFFF0000u);
+      }
+      q4_store8(at, f);
+    }
   }
-  q4_store8((is_v ? v : k) + row * D + 8 * oct, x);
 }
 
 }  // namespace it
