@@ -60,7 +60,7 @@ quantize_rows_kernel(const ST* __restrict__ x, int8_t* __restrict__ codes, float
   }
   const float s = quant_scale<127, 8>(most);
   const bool some = s > 0.f;   // false: zeros, or not numbers
-  const float inv = some ? __frcp_rn(s) : 0.f;
+  const float inv = quant_inverse(s);
   if (first == 0) scales[row] = s;
   auto store = [&](int c, const uint4& v) {
     float f[VEC];
@@ -75,7 +75,7 @@ quantize_rows_kernel(const ST* __restrict__ x, int8_t* __restrict__ codes, float
       }
     }
     uint32_t b[VEC] = {};
-    if (some) quant_codes(f, s, inv, b);
+    if (some) quant_codes<0>(f, s, inv, b);
     uint32_t out[VEC / 4];
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i)
@@ -119,23 +119,24 @@ struct GemmI8Traits {
   static constexpr int BM = 128, BK = 128, B_ROWS = BN_ / CG;
   static constexpr int A_BYTES = BM * BK, B_BYTES = B_ROWS * BK, STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int STAGES = B_ROWS == 256 ? 4 : B_ROWS == 128 ? 6 : 8;
-  static constexpr int OUT_BYTES = 32 * 128;                  // a warp's piece of the result, two a warp
+  static constexpr int OUT_BYTES = 32 * 128;                  // a warp's piece of the result
+  static constexpr int OUT_WARPS = 8;
   static constexpr int SMEM_OUT = STAGES * STAGE_BYTES;
-  static constexpr int SMEM_BAR = SMEM_OUT + 8 * OUT_BYTES;
+  static constexpr int SMEM_BAR = SMEM_OUT + OUT_WARPS * OUT_BYTES;
   static constexpr int SMEM_MISC = SMEM_BAR + (2 * STAGES + 4) * 8;
   static constexpr int SMEM_BYTES = SMEM_MISC + 16;
-  static constexpr int THREADS = 256;
+  static constexpr int THREADS = 128 + 32 * OUT_WARPS;
   static constexpr uint32_t TMEM_COLS = 2 * BN_;              // two accumulators
 };
 
 // The pipeline of gemm_bf16_sm100_kernel (y = x W^T) on bytes: a 128-byte row of a stage is 128 columns of K, an instruction of
 // kind::i8 takes 32 of them, and tensor memory holds 32-bit integers.  Persistent CTAs (or pairs, CG = 2) of
-//   warp 0: TMA loads   warp 1: tcgen05.mma   warp 2: tensor memory   warps 4-7: epilogue, a thread per row.
+//   warp 0: TMA loads   warp 1: tcgen05.mma   warp 2: tensor memory   warps 4-11: epilogue, two warps for 32 rows.
 // At twice bf16's rate a tile has half the time for its epilogue.  Stored from registers, 16 bytes of 32 rows at a time, results of
 // 2999 x 2048 -> 6144 took 71 us in fp32; so a warp turns pieces of 32 rows by 128 bytes round in shared memory and stores them
 // by TMA: whole lines, and no instructions of the epilogue's (XX us).
 template <int BN, int CG, typename OT>
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(384, 1)
 gemm_i8_sm100_kernel(const __grid_constant__ GemmI8Maps maps, const GemmI8Params prm) {
   using T = GemmI8Traits<BN, CG>;
   using namespace ptx;
@@ -169,7 +170,7 @@ gemm_i8_sm100_kernel(const __grid_constant__ GemmI8Maps maps, const GemmI8Params
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], CG == 2 ? 8 : 4);   // one arrival per epilogue warp, of a pair of both CTAs
+      mbar_init(&acc_empty[i], CG * T::OUT_WARPS);   // one arrival per epilogue warp, of a pair of both CTAs
     }
     fence_mbar_init();
     fence_proxy_async_smem();
@@ -265,8 +266,8 @@ gemm_i8_sm100_kernel(const __grid_constant__ GemmI8Maps maps, const GemmI8Params
     constexpr int W = 128 / sizeof(OT);      // columns of a piece
     const int row_in_tile = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    uint8_t* pieces = smem + T::SMEM_OUT + (warp & 3) * 2 * T::OUT_BYTES;
-    int t = 0, piece = 0;
+    uint8_t* piece = smem + T::SMEM_OUT + (warp - 4) * T::OUT_BYTES;
+    int t = 0;
     bool ok = true;
     for (int tile = first_tile; tile < n_tiles && ok; tile += tile_step, ++t) {
       const int buf = t & 1;
@@ -280,17 +281,13 @@ gemm_i8_sm100_kernel(const __grid_constant__ GemmI8Maps maps, const GemmI8Params
       tc_fence_after();
       if (m0 + (warp & 3) * 32 < prm.M) {
 #pragma unroll 1
-        for (int c = 0; c < BN / W; ++c) {
+        for (int c = (warp - 4) >> 2; c < BN / W; c += 2) {
           const int col0 = n0 + c * W;
           if (col0 >= prm.N) break;
           // a piece that lies in one range (what is behind the range's last column is cut off) goes through shared memory
           const int range = i8_range_of(prm.out, col0), begin = i8_range_begin(prm.out, range);
           const bool whole = min(col0 + W, prm.N) <= prm.out.end[range];
-          uint8_t* dst = pieces + (piece & 1) * T::OUT_BYTES + lane * 128;
-          if (whole) {
-            if (lane == 0) bulk_wait_group_read<1>();   // the piece before the last has left this buffer
-            __syncwarp();
-          }
+          uint32_t out[32];   // the row's 128 bytes
 #pragma unroll
           for (int half = 0; half < W / 32; ++half) {
             uint32_t r[32];
@@ -311,24 +308,28 @@ gemm_i8_sm100_kernel(const __grid_constant__ GemmI8Maps maps, const GemmI8Params
               if (!whole) {
                 const int col = col0 + half * 32 + v * 8;
                 if (row < prm.M && col < prm.N) i8_store8<OT>(prm.out, row, col, y);
-              } else if constexpr (sizeof(OT) == 4) {
+              }
+              if constexpr (sizeof(OT) == 4) {
 #pragma unroll
-                for (int q = 0; q < 2; ++q)
-                  *reinterpret_cast<float4*>(dst + (((2 * v + q) ^ (lane & 7)) << 4)) = make_float4(y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+                for (int e = 0; e < 8; ++e) out[v * 8 + e] = __float_as_uint(y[e]);
               } else {
-                *reinterpret_cast<uint4*>(dst + (((half * 4 + v) ^ (lane & 7)) << 4)) =
-                    make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) out[half * 16 + v * 4 + e] = pack_bf16(y[2 * e], y[2 * e + 1]);
               }
             }
           }
           if (whole) {
+            if (lane == 0) bulk_wait_group_read<0>();   // the piece before has left the buffer
+            __syncwarp();
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              *reinterpret_cast<uint4*>(piece + lane * 128 + ((v ^ (lane & 7)) << 4)) = make_uint4(out[4 * v], out[4 * v + 1], out[4 * v + 2], out[4 * v + 3]);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tma_store_4d(&maps.out[range], pieces + (piece & 1) * T::OUT_BYTES, col0 - begin, m0 + (warp & 3) * 32, 0, 0);
+              tma_store_4d(&maps.out[range], piece, col0 - begin, m0 + (warp & 3) * 32, 0, 0);
               bulk_commit_group();
             }
-            ++piece;
           }
         }
       }

@@ -35,9 +35,36 @@ it_status check_cache(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t B,
   return IT_OK;
 }
 
+// Frequencies and axes of the dimension pairs.  64 powers in 64 bits take as long as the launch: the last ones are kept, by value.
+const it::RopeAxes& rope_axes(int D, float base, int n_axes, const int32_t* sections, int per_axis) {
+  struct Last {
+    int D = 0, n_axes = 0, per_axis = 0;
+    int32_t sections[4] = {};
+    float base = 0.f;
+    it::RopeAxes axes;
+  };
+  thread_local Last last;
+  const bool same = last.D == D && last.n_axes == n_axes && last.per_axis == (per_axis != 0) && last.base == base &&
+                    std::equal(sections, sections + n_axes, last.sections);
+  if (same) return last.axes;
+  last.D = D;
+  last.n_axes = n_axes;
+  last.per_axis = per_axis != 0;
+  last.base = base;
+  std::copy(sections, sections + n_axes, last.sections);
+  int pair = 0;
+  for (int a = 0; a < n_axes; ++a)
+    for (int j = 0; j < sections[a]; ++j, ++pair) {
+      last.axes.freq[pair] = std::pow(static_cast<double>(base), per_axis ? -static_cast<double>(j) / sections[a] : -2.0 * pair / D);
+      last.axes.axis[pair] = static_cast<uint8_t>(a);
+    }
+  for (; pair < 64; ++pair) last.axes.freq[pair] = last.axes.axis[pair] = 0;
+  return last.axes;
+}
+
 // The grid of the kernels that write and read a cache (kv_q4.cuh).
 it_status cache_grid(int B, int tokens, int Hkv, int D, dim3* grid) {
-  const int64_t rows = static_cast<int64_t>(tokens) * Hkv, per_cta = 256 / (4 * ((D + 31) / 32));
+  const int64_t rows = static_cast<int64_t>(tokens) * Hkv, per_cta = 256 / (4 * ((D + 31) / 32)) * it::KV_ROWS_A_THREAD;
   if (rows > 0x7fffffffLL - per_cta) return fail(IT_ERR_UNSUPPORTED_SHAPE, "tokens * kv_heads must be below 2^31");
   *grid = dim3(static_cast<unsigned>((rows + per_cta - 1) / per_cta), std::min(B, 65535), 2);
   return IT_OK;
@@ -122,16 +149,12 @@ it_status it_rope_positions(it_ctx* ctx, it_stream* stream, it_dtype dtype, int3
   if (D < 2 || D > 128 || (D & 1)) return fail(IT_ERR_UNSUPPORTED_SHAPE, "rotary embedding needs an even head_dim in 2..128, got %d", D);
   if (!(rope_base > 0.f) || !std::isfinite(rope_base)) return fail(IT_ERR_INVALID_ARG, "rotary base must be positive and finite");
   if (n_axes < 1 || n_axes > 4 || sections == nullptr) return fail(IT_ERR_INVALID_ARG, "1 to 4 axes with a section each, got %d", n_axes);
-  it::RopeAxes axes{};
-  int pair = 0;
+  int pairs = 0;
   for (int a = 0; a < n_axes; ++a) {
-    if (sections[a] < 0 || sections[a] > D / 2 - pair) return fail(IT_ERR_INVALID_ARG, "sections must add up to head_dim / 2 = %d", D / 2);
-    for (int j = 0; j < sections[a]; ++j, ++pair) {
-      axes.freq[pair] = std::pow(static_cast<double>(rope_base), per_axis ? -static_cast<double>(j) / sections[a] : -2.0 * pair / D);
-      axes.axis[pair] = static_cast<uint8_t>(a);
-    }
+    if (sections[a] < 0 || sections[a] > D / 2 - pairs) return fail(IT_ERR_INVALID_ARG, "sections must add up to head_dim / 2 = %d", D / 2);
+    pairs += sections[a];
   }
-  if (pair != D / 2) return fail(IT_ERR_INVALID_ARG, "sections must add up to head_dim / 2 = %d", D / 2);
+  if (pairs != D / 2) return fail(IT_ERR_INVALID_ARG, "sections must add up to head_dim / 2 = %d", D / 2);
   const int64_t rows = static_cast<int64_t>(B) * S;
   if (rows == 0 || (H == 0 && Hkv == 0)) return IT_OK;
   if (static_cast<int64_t>(H) + Hkv > 65535) return fail(IT_ERR_UNSUPPORTED_SHAPE, "heads + kv_heads must be at most 65535");
@@ -139,13 +162,16 @@ it_status it_rope_positions(it_ctx* ctx, it_stream* stream, it_dtype dtype, int3
   if (H > 0 && (q_in == nullptr || q_out == nullptr)) return fail(IT_ERR_INVALID_ARG, "null q tensor");
   if (Hkv > 0 && (k_in == nullptr || k_out == nullptr)) return fail(IT_ERR_INVALID_ARG, "null k tensor");
   IT_CUDA(cudaSetDevice(ctx->device));
+  const it::RopeAxes& axes = rope_axes(D, rope_base, n_axes, sections, per_axis);
   const int half = D / 2, elem = dtype == IT_F32 ? 4 : 2;
   const bool chunks = (D * elem) % 16 == 0 && aligned16(q_in) && aligned16(q_out) && aligned16(k_in) && aligned16(k_out);
   const uintptr_t pair_mask = 2 * elem - 1;
   if (!chunks && ((reinterpret_cast<uintptr_t>(q_in) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k_in) |
                    reinterpret_cast<uintptr_t>(k_out)) & pair_mask))
     return fail(IT_ERR_ALIGNMENT, "q and k must be aligned to a pair of elements");
-  const int n_pos = static_cast<int>(std::clamp<int64_t>(rows / (4LL * ctx->sm_count), 1, 256 / half));
+  // as many tokens a CTA as have one sine per thread and four chunks, all in flight together, as long as that leaves four CTAs per SM
+  const int token_chunks = (H + Hkv) * (chunks ? D * elem / 16 : half);
+  const int n_pos = static_cast<int>(std::clamp<int64_t>(rows / (4LL * ctx->sm_count), 1, std::clamp(1024 / token_chunks, 1, 256 / half)));
   const int64_t ctas = (rows + n_pos - 1) / n_pos;
   if (ctas > 2147483647LL) return fail(IT_ERR_UNSUPPORTED_SHAPE, "too many tokens");
   auto launch = [&](auto kernel, auto* q, auto* k, auto* qo, auto* ko) -> it_status {

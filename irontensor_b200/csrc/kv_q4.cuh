@@ -25,29 +25,27 @@
 namespace it {
 
 // largest / MOST rounded to BITS significant bits, ties to even; NaN for a NaN or infinite `largest`, given by the bits of its
-// magnitude.  The fp32 quotient is right but where it is rounded onto the middle between two results: there the sign of the
-// remainder largest - MOST * quotient, exact in one fma, decides.
+// magnitude.  The product with 1 / MOST is right but for its last places; which side of the middle between two results the quotient
+// is on is what largest and MOST * middle say, both exact.
 template <int MOST, int BITS>
 __device__ __forceinline__ float quant_scale(uint32_t largest_bits) {
-  if (largest_bits >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
-  const float largest = __uint_as_float(largest_bits);
-  if (largest < 0x1p-100f) return 0.f;
   constexpr int DROP = 24 - BITS;
   constexpr uint32_t MASK = (1u << DROP) - 1u, HALF = 1u << (DROP - 1);
-  const float t = __fdiv_rn(largest, static_cast<float>(MOST));
-  const float rest = fmaf(-static_cast<float>(MOST), t, largest);
-  const uint32_t bits = __float_as_uint(t), low = bits & MASK, base = bits & ~MASK;
-  const bool up = low > HALF || (low == HALF && (rest > 0.f || (rest == 0.f && ((base >> DROP) & 1u))));
-  return __uint_as_float(base + (up ? MASK + 1u : 0u));
+  const float largest = __uint_as_float(largest_bits);
+  const uint32_t base = __float_as_uint(largest * (1.f / MOST)) & ~MASK;
+  const float middle = static_cast<float>(MOST) * __uint_as_float(base | HALF);
+  const bool up = largest > middle || (largest == middle && ((base >> DROP) & 1u));
+  const float s = __uint_as_float(base + (up ? MASK + 1u : 0u));
+  return largest_bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : largest < 0x1p-100f ? 0.f : s;
 }
 
-// round(x / s), ties to even, in the low byte of each c, for s of at most 8 significant bits and quotients of less than 127.5; inv =
-// 1 / s.  The whole number q comes out of the low bits of a sum with 1.5 * 2^23, rounded once.  x * inv may be off by a last
-// place, which matters next to the middle of two whole numbers: there x - q s, exact (at most 24 bits above the last place of x),
-// says which is nearer.  That is rare, and asked once for all N.
-template <int N>
+// round(x / s), ties to even, plus BIAS in the low 16 bits of each c, for s of at most 8 significant bits and quotients of less than
+// 127.5; inv = 1 / s to 22 bits.  The whole number q comes out of the low bits of a sum with 1.5 * 2^23, rounded once.  x * inv may be
+// off by a few last places, which matters next to the middle of two whole numbers: there x - q s, exact (at most 24 bits above the
+// last place of x), says which is nearer.  That is rare, and asked once for all N.
+template <int BIAS, int N>
 __device__ __forceinline__ void quant_codes(const float (&x)[N], float s, float inv, uint32_t (&c)[N]) {
-  constexpr float MAGIC = 12582912.f;
+  constexpr float MAGIC = 12582912.f + BIAS;
   const float half = 0.5f * s;
   bool close = false;
 #pragma unroll
@@ -60,9 +58,14 @@ __device__ __forceinline__ void quant_codes(const float (&x)[N], float s, float 
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       const float r = fmaf(-(__uint_as_float(c[e]) - MAGIC), s, x[e]);
-      if (fabsf(r) > half || (fabsf(r) == half && (c[e] & 1u))) c[e] += r > 0.f ? 1u : 0xFFFFFFFFu;
+      if (fabsf(r) > half || (fabsf(r) == half && ((c[e] - BIAS) & 1u))) c[e] += r > 0.f ? 1u : 0xFFFFFFFFu;
     }
   }
+}
+__device__ __forceinline__ float quant_inverse(float s) {
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  return inv;
 }
 
 __device__ __forceinline__ uint32_t q4_fma2(uint32_t a, uint32_t b, uint32_t c) {
@@ -127,46 +130,105 @@ __device__ __forceinline__ void q4_store8(float* p, const float (&x)[8]) {
   *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
 }
 
-// What 8 columns of a thread become: the word of their codes, and the group's scale.  The threads of a quad hold a group.
-__device__ __forceinline__ uint32_t q4_quantise(const float (&x)[8], float* scale) {
-  uint32_t largest = 0;
+// Eight columns as they are loaded, and the largest of their magnitudes by its bits as fp32.
+template <typename ST>
+struct Raw8;
+template <>
+struct Raw8<__nv_bfloat16> {
+  uint4 v;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ uint32_t largest() const {
+    auto max2 = [](uint32_t a, uint32_t b) {
+      uint32_t d;
+      asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+      return d;
+    };
+    const uint32_t m = max2(max2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), max2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+    return max(m & 0xFFFF0000u, m << 16);
+  }
+  __device__ __forceinline__ void to(float (&x)[8]) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) largest = max(largest, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+};
+template <>
+struct Raw8<float> {
+  uint4 v, w;
+  __device__ __forceinline__ void load(const float* p) {
+    v = __ldg(reinterpret_cast<const uint4*>(p));
+    w = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+  }
+  __device__ __forceinline__ uint32_t largest() const {
+    constexpr uint32_t M = 0x7FFFFFFFu;
+    return max(max(max(v.x & M, v.y & M), max(v.z & M, v.w & M)), max(max(w.x & M, w.y & M), max(w.z & M, w.w & M)));
+  }
+  __device__ __forceinline__ void to(float (&x)[8]) const {
+    const uint32_t b[8] = {v.x, v.y, v.z, v.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(b[i]);
+  }
+};
+
+// What 8 columns of a thread become: the word of their codes, and the group's scale.  The threads of a quad hold a group.
+template <typename ST>
+__device__ __forceinline__ uint32_t q4_quantise(const Raw8<ST>& raw, float* scale) {
+  uint32_t largest = raw.largest();
   largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
   largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-  float s = quant_scale<7, 5>(largest);
-  const bool saturates = s > Q4_MOST_SCALE;
-  if (saturates) s = Q4_MOST_SCALE;
+  float s = quant_scale<7, 5>(largest), x[8];
+  raw.to(x);
+  if (s > Q4_MOST_SCALE) {
+    s = Q4_MOST_SCALE;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = fminf(fmaxf(x[e], -7.f * s), 7.f * s);
+  }
   *scale = s;
   if (!(s > 0.f)) return 0x88888888u;   // zeros, or not numbers
-  const float inv = __frcp_rn(s);
-  float y[8];
-  uint32_t c[8], word = 0;
+  uint32_t c[8], p[4];
+  quant_codes<8>(x, s, quant_inverse(s), c);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = saturates ? fminf(fmaxf(x[e], -7.f * s), 7.f * s) : x[e];
-  quant_codes(y, s, inv, c);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) word |= ((c[e] + 8u) & 15u) << (4 * (e >> 1) + 16 * (e & 1));
-  return word;
+  for (int i = 0; i < 4; ++i) p[i] = __byte_perm(c[2 * i], c[2 * i + 1], 0x5410);
+  return (p[0] + 16u * p[1]) + 256u * (p[2] + 16u * p[3]);
 }
 
+constexpr int KV_ROWS_A_THREAD = 4;   // whose loads are in flight together
+
+// Where a thread of the two kernels below is: 8 columns, and rows (token and head of a sequence) `row`, `row` + ROWS, ...
+template <int NG>
+struct KvLane {
+  static constexpr int LANES = 4 * NG, ROWS = 256 / LANES;   // threads of a row, rows of a CTA at a time
+  int in_cta, j, t;
+  uint32_t row;
+  __device__ __forceinline__ KvLane() {
+    in_cta = static_cast<int>(threadIdx.x) / LANES;
+    j = static_cast<int>(threadIdx.x) % LANES >> 2;
+    t = static_cast<int>(threadIdx.x) & 3;
+    row = blockIdx.x * (ROWS * KV_ROWS_A_THREAD) + in_cta;
+  }
+};
+
 // New tokens k, v [batch, T, kv_heads, head_dim] into the cache behind the lengths[b] positions that are there; of sequence b the
-// first counts[b] tokens (null: all T).  new_lengths[b] = what is there afterwards.  Grid (rows, batch, keys or values); a
-// thread takes 8 columns.  Positions outside the cache are not written, and reported.
-// Reads 2 * 8 or 4 * 8 bytes a thread and writes 4.5: bound by memory, and for single tokens by the launch.
+// first counts[b] tokens (null: all T).  new_lengths[b] = what is there afterwards.  Grid (rows, batch, keys or values).  Positions
+// outside the cache are not written, and reported.
+// Bound by memory, 2 or 4 bytes read and 0.56 written a value, and for single tokens by the launch.
 template <typename ST, int NG>
 __global__ void __launch_bounds__(256)
 kv_q4_append_kernel(const ST* __restrict__ k, const ST* __restrict__ v, KvQ4 ck, KvQ4 cv, const int* __restrict__ lengths,
                     const int* __restrict__ counts, int* __restrict__ new_lengths, int B, int T, int Hkv, int D, int max_len, int* status) {
-  constexpr int LANES = 4 * NG, ROWS = 256 / LANES;   // threads of a row, rows of a CTA
+  using L = KvLane<NG>;
+  constexpr int U = KV_ROWS_A_THREAD;
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
-  const int in_cta = static_cast<int>(threadIdx.x) / LANES, lane = static_cast<int>(threadIdx.x) % LANES, j = lane >> 2, t = lane & 3;
-  const uint32_t row = blockIdx.x * ROWS + in_cta;    // of the sequence: token and head
-  const int tok = static_cast<int>(row / static_cast<uint32_t>(Hkv)), h = static_cast<int>(row - static_cast<uint32_t>(tok) * Hkv);
-  const int d0 = 32 * j + 8 * t;
+  const L at;
+  const int d0 = 32 * at.j + 8 * at.t;
   const ST* src = blockIdx.z ? v : k;
   const KvQ4& c = blockIdx.z ? cv : ck;
+  const int step_tok = L::ROWS / Hkv, step_h = L::ROWS - step_tok * Hkv;
+  const int first_tok = static_cast<int>(at.row / static_cast<uint32_t>(Hkv)), first_h = static_cast<int>(at.row - static_cast<uint32_t>(first_tok) * Hkv);
   for (int b = blockIdx.y; b < B; b += static_cast<int>(gridDim.y)) {
     const int have = lengths[b], want = counts != nullptr ? counts[b] : T, add = min(max(want, 0), T);
     if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) {
@@ -174,62 +236,104 @@ kv_q4_append_kernel(const ST* __restrict__ k, const ST* __restrict__ v, KvQ4 ck,
       if (have < 0 || end > max_len || add != want) atomicCAS(status, 0, DEV_ERR_CACHE_RANGE);
       new_lengths[b] = static_cast<int>(min(max(end, 0LL), static_cast<long long>(max_len)));
     }
-    const long long pos = static_cast<long long>(have) + tok;
-    const bool live = in_cta < ROWS && tok < add && pos >= 0 && pos < max_len;
-    if (!__any_sync(0xffffffffu, live)) continue;
-    float x[8] = {};
-    if (live && d0 < D) q4_load8(src + ((static_cast<size_t>(b) * T + tok) * Hkv + h) * D + d0, x);
-    float s;
-    const uint32_t word = q4_quantise(x, &s);
-    if (live) {
-      const size_t crow = (static_cast<size_t>(b) * Hkv + h) * max_len + pos;
-      c.codes[crow * LANES + t * NG + j] = word;
-      if (t == 0) c.scales[crow * NG + j] = __float2bfloat16_rn(s);
+    Raw8<ST> x[U] = {};
+    bool live[U];
+    size_t crow[U];
+    int tok = first_tok, h = first_h;
+    const ST* from = src + (static_cast<size_t>(b) * T * Hkv + at.row) * D + d0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long pos = static_cast<long long>(have) + tok;
+      live[u] = at.in_cta < L::ROWS && tok < add && pos >= 0 && pos < max_len;
+      crow[u] = (static_cast<size_t>(b) * Hkv + h) * max_len + pos;
+      if (live[u] && d0 < D) x[u].load(from + static_cast<size_t>(u) * L::ROWS * D);
+      tok += step_tok;
+      h += step_h;
+      if (h >= Hkv) {
+        h -= Hkv;
+        ++tok;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!__any_sync(0xffffffffu, live[u])) continue;
+      float s;
+      const uint32_t word = q4_quantise(x[u], &s);
+      if (live[u]) {
+        c.codes[crow[u] * L::LANES + at.t * NG + at.j] = word;
+        if (at.t == 0) c.scales[crow[u] * NG + at.j] = __float2bfloat16_rn(s);
+      }
     }
   }
 }
 
 // Positions starts[b] + t, t < T, of the cache (null: from 0) as keys and values [batch, T, kv_heads, head_dim]; zeros outside
-// 0 <= position < min(lengths[b], max_len) (null: max_len).  Grid as above; a thread writes 8 columns.  Bound by the bytes that it
-// writes.
+// 0 <= position < min(lengths[b], max_len) (null: max_len).  Grid as above.  Bound by the bytes that it writes.
 template <typename ST, int NG>
 __global__ void __launch_bounds__(256)
 kv_q4_read_kernel(ST* __restrict__ k, ST* __restrict__ v, KvQ4 ck, KvQ4 cv, const int* __restrict__ starts, const int* __restrict__ lengths,
                   int B, int T, int Hkv, int D, int max_len) {
-  constexpr int LANES = 4 * NG, ROWS = 256 / LANES;
+  using L = KvLane<NG>;
+  constexpr int U = KV_ROWS_A_THREAD;
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
-  const int in_cta = static_cast<int>(threadIdx.x) / LANES, lane = static_cast<int>(threadIdx.x) % LANES, j = lane >> 2, t = lane & 3;
-  const uint32_t row = blockIdx.x * ROWS + in_cta;
-  const int tok = static_cast<int>(row / static_cast<uint32_t>(Hkv)), h = static_cast<int>(row - static_cast<uint32_t>(tok) * Hkv);
-  const int d0 = 32 * j + 8 * t;
-  if (in_cta >= ROWS || tok >= T || d0 >= D) return;
+  const L at;
+  const int d0 = 32 * at.j + 8 * at.t;
+  const bool none = at.in_cta >= L::ROWS || d0 >= D;   // columns that only pad a group; they stay for the exchange below
   ST* dst = blockIdx.z ? v : k;
   const KvQ4& c = blockIdx.z ? cv : ck;
+  const int step_tok = L::ROWS / Hkv, step_h = L::ROWS - step_tok * Hkv;
+  const int first_tok = static_cast<int>(at.row / static_cast<uint32_t>(Hkv)), first_h = static_cast<int>(at.row - static_cast<uint32_t>(first_tok) * Hkv);
   for (int b = blockIdx.y; b < B; b += static_cast<int>(gridDim.y)) {
-    const long long pos = static_cast<long long>(starts != nullptr ? starts[b] : 0) + tok;
+    const long long start = starts != nullptr ? starts[b] : 0;
     const int end = lengths != nullptr ? min(lengths[b], max_len) : max_len;
-    uint32_t x[4] = {0u, 0u, 0u, 0u};   // pairs of neighbouring columns
-    if (pos >= 0 && pos < end) {
-      const size_t crow = (static_cast<size_t>(b) * Hkv + h) * max_len + pos;
-      const uint32_t w = __ldg(c.codes + crow * LANES + t * NG + j);
-      const uint32_t s2 = __byte_perm(*reinterpret_cast<const unsigned short*>(c.scales + crow * NG + j), 0, 0x1010), bias2 = q4_mul2(s2, Q4_MINUS_24);
-      x[0] = q4_pair<0>(w, s2, bias2, Q4_MAGIC);
-      x[1] = q4_pair<1>(w, s2, bias2, Q4_MAGIC);
-      x[2] = q4_pair<2>(w, s2, bias2, Q4_MAGIC);
-      x[3] = q4_pair<3>(w, s2, bias2, Q4_MAGIC);
-    }
-    ST* at = dst + ((static_cast<size_t>(b) * T + tok) * Hkv + h) * D + d0;
-    if constexpr (sizeof(ST) == 2) {
-      *reinterpret_cast<uint4*>(at) = make_uint4(x[0], x[1], x[2], x[3]);
-    } else {
-      float f[8];
+    uint32_t w[U], s2[U];
+    int tok = first_tok, h = first_h;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f[2 * i] = __uint_as_float(x[i] << 16);
-        f[2 * i + 1] = __uint_as_float(x[i] & 0xFFFF0000u);
+    for (int u = 0; u < U; ++u) {
+      const long long pos = start + tok;
+      w[u] = 0x88888888u;
+      s2[u] = 0u;
+      if (!none && tok < T && pos >= 0 && pos < end) {
+        const size_t crow = (static_cast<size_t>(b) * Hkv + h) * max_len + pos;
+        w[u] = __ldg(c.codes + crow * L::LANES + at.t * NG + at.j);
+        s2[u] = __ldg(reinterpret_cast<const unsigned short*>(c.scales) + crow * NG + at.j);
       }
-      q4_store8(at, f);
+      tok += step_tok;
+      h += step_h;
+      if (h >= Hkv) {
+        h -= Hkv;
+        ++tok;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t row = at.row + u * L::ROWS;
+      const bool there = !none && row < static_cast<uint32_t>(T) * Hkv;
+      const uint32_t s = __byte_perm(s2[u], 0, 0x1010), bias = q4_mul2(s, Q4_MINUS_24);
+      const uint32_t x[4] = {q4_pair<0>(w[u], s, bias, Q4_MAGIC), q4_pair<1>(w[u], s, bias, Q4_MAGIC), q4_pair<2>(w[u], s, bias, Q4_MAGIC),
+                             q4_pair<3>(w[u], s, bias, Q4_MAGIC)};   // pairs of neighbouring columns
+      ST* out = dst + (static_cast<size_t>(b) * T * Hkv + row) * D + d0;
+      if constexpr (sizeof(ST) == 2) {
+        if (there) *reinterpret_cast<uint4*>(out) = make_uint4(x[0], x[1], x[2], x[3]);
+      } else {
+        // A thread has 32 bytes and stores 16 at a time: as they lie, every store would fill half of each 32-byte sector.  So two
+        // neighbours store together, first the 32 bytes of the even one and then those of the odd one.
+        uint32_t f[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f[2 * i] = x[i] << 16;
+          f[2 * i + 1] = x[i] & 0xFFFF0000u;
+        }
+        const bool odd = threadIdx.x & 1;
+        uint32_t got[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) got[i] = __shfl_xor_sync(0xffffffffu, odd ? f[i] : f[4 + i], 1);
+        const bool other = __shfl_xor_sync(0xffffffffu, static_cast<int>(there), 1) != 0;
+        ST* even_at = out - (odd ? 8 : 0);   // the even thread's columns
+        if (odd ? other : there) *reinterpret_cast<uint4*>(even_at + (odd ? 4 : 0)) = odd ? make_uint4(got[0], got[1], got[2], got[3]) : make_uint4(f[0], f[1], f[2], f[3]);
+        if (odd ? there : other) *reinterpret_cast<uint4*>(even_at + 8 + (odd ? 4 : 0)) = odd ? make_uint4(f[4], f[5], f[6], f[7]) : make_uint4(got[0], got[1], got[2], got[3]);
+      }
     }
   }
 }

@@ -33,41 +33,63 @@ __device__ __forceinline__ float2 rope_turn(int position, double freq) {
   return make_float2(c, s);
 }
 
-// A CTA owns n_pos tokens: one sine per thread into shared memory, then the heads of q and k in 16-byte chunks (see
-// rope_qk_chunks_kernel).  VEC: elements of a chunk; 2 where rows are not whole chunks.
+// A CTA owns n_pos tokens: one sine per thread into shared memory, then the heads of q and k in chunks of VEC elements (16 bytes; 2
+// elements where rows are not whole chunks), of which a thread has four in flight, the first four before the sines.  A thread stays
+// with one chunk of a head, `half` / (VEC / 2) threads a head, and steps over the (token, head) rows.
 template <typename ST, int VEC>
 __global__ void __launch_bounds__(256)
 rope_positions_kernel(const ST* q_in, const ST* k_in, ST* q_out, ST* k_out, const int* __restrict__ positions, long long rows, int n_pos,
                       int H, int Hkv, int D, int inverse, const __grid_constant__ RopeAxes axes) {
+  constexpr int U = 4;
   __shared__ float2 tab[256];
   struct alignas(VEC * sizeof(ST)) Chunk { ST e[VEC]; };
   const int half = D >> 1, per_head = D / VEC, n_heads = H + Hkv;
   const long long row0 = static_cast<long long>(blockIdx.x) * n_pos;
   const int n_rows = static_cast<int>(min(static_cast<long long>(n_pos), rows - row0));
-  const int n_chunks = n_rows * n_heads * per_head;
+  const int step = 256 / per_head, mine = static_cast<int>(threadIdx.x) / per_head, d = (static_cast<int>(threadIdx.x) - mine * per_head) * VEC;
+  const int step_r = step / n_heads, step_h = step - step_r * n_heads;
+  int r = mine < step ? mine / n_heads : n_rows, h = mine < step ? mine - r * n_heads : 0;   // the threads behind the last whole head: none
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
-  for (int t = static_cast<int>(threadIdx.x); t < n_rows * half; t += 256) {
-    const int r = t / half, pair = t - r * half;
-    float2 cs = rope_turn(positions[axes.axis[pair] * rows + row0 + r], axes.freq[pair]);
-    if (inverse) cs.y = -cs.y;
-    tab[t] = cs;
-  }
-  __syncthreads();
-  for (int i = static_cast<int>(threadIdx.x); i < n_chunks; i += 256) {
-    const int head_row = i / per_head, d = (i - head_row * per_head) * VEC;
-    const int r = head_row / n_heads, hh = head_row - r * n_heads;
-    const bool is_q = hh < H;
-    const long long off = (is_q ? (row0 + r) * H + hh : (row0 + r) * Hkv + (hh - H)) * D + d;
-    Chunk x = *reinterpret_cast<const Chunk*>((is_q ? q_in : k_in) + off);
-    const float2* cs = &tab[r * half + (d >> 1)];
+  auto offset = [&](int rr, int hh) { return (hh < H ? (row0 + rr) * H + hh : (row0 + rr) * Hkv + (hh - H)) * D + d; };
+  bool first = true;
+  while (first || r < n_rows) {
+    Chunk x[U];
+    int rr[U], hh[U];
 #pragma unroll
-    for (int p = 0; p < VEC / 2; ++p) {
-      const float x0 = rope_ld(&x.e[2 * p]), x1 = rope_ld(&x.e[2 * p + 1]);
-      rope_st(&x.e[2 * p], x0 * cs[p].x - x1 * cs[p].y);
-      rope_st(&x.e[2 * p + 1], x0 * cs[p].y + x1 * cs[p].x);
+    for (int u = 0; u < U; ++u) {
+      rr[u] = r;
+      hh[u] = h;
+      if (r < n_rows) x[u] = *reinterpret_cast<const Chunk*>((h < H ? q_in : k_in) + offset(r, h));
+      r += step_r;
+      h += step_h;
+      if (h >= n_heads) {
+        h -= n_heads;
+        ++r;
+      }
     }
-    *reinterpret_cast<Chunk*>((is_q ? q_out : k_out) + off) = x;
+    if (first) {   // every thread passes here once
+      for (int i = static_cast<int>(threadIdx.x); i < n_rows * half; i += 256) {
+        const int tr = i / half, pair = i - tr * half;
+        float2 cs = rope_turn(positions[axes.axis[pair] * rows + row0 + tr], axes.freq[pair]);
+        if (inverse) cs.y = -cs.y;
+        tab[i] = cs;
+      }
+      __syncthreads();
+      first = false;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (rr[u] >= n_rows) break;
+      const float2* cs = &tab[rr[u] * half + (d >> 1)];
+#pragma unroll
+      for (int p = 0; p < VEC / 2; ++p) {
+        const float x0 = rope_ld(&x[u].e[2 * p]), x1 = rope_ld(&x[u].e[2 * p + 1]);
+        rope_st(&x[u].e[2 * p], x0 * cs[p].x - x1 * cs[p].y);
+        rope_st(&x[u].e[2 * p + 1], x0 * cs[p].y + x1 * cs[p].x);
+      }
+      *reinterpret_cast<Chunk*>((hh[u] < H ? q_out : k_out) + offset(rr[u], hh[u])) = x[u];
+    }
   }
 }
 
