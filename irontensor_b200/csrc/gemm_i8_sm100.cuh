@@ -75,7 +75,7 @@ quantize_rows_kernel(const ST* __restrict__ x, int8_t* __restrict__ codes, float
       }
     }
     uint32_t b[VEC] = {};
-    if (some) quant_codes<0>(f, s, inv, b);
+    if (some) quant_codes<0, sizeof(ST) == 2>(f, s, inv, b);
     uint32_t out[VEC / 4];
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i)

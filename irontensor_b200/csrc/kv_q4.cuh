@@ -40,12 +40,22 @@ __device__ __forceinline__ float quant_scale(uint32_t largest_bits) {
 }
 
 // round(x / s), ties to even, plus BIAS in the low 16 bits of each c, for s of at most 8 significant bits and quotients of less than
-// 127.5; inv = 1 / s to 22 bits.  The whole number q comes out of the low bits of a sum with 1.5 * 2^23, rounded once.  x * inv may be
-// off by a few last places, which matters next to the middle of two whole numbers: there x - q s, exact (at most 24 bits above the
-// last place of x), says which is nearer.  That is rare, and asked once for all N.
-template <int BIAS, int N>
+// 127.5; inv = 1 / s to 22 bits.  The whole number comes out of the low bits of a sum with 1.5 * 2^23, rounded once.
+// SHORT: x of 8 significant bits, where ties are common.  A quotient that is no tie is 2^-16 away from one and more, so the quotient
+// rounded to fp32 decides; one step of refinement with the exact remainder gives it, and ties exactly.
+// Otherwise x * inv may be off by a few last places, which matters next to the middle of two whole numbers: there x - q s, exact (at
+// most 24 bits above the last place of x), says which is nearer.  That is rare, and asked once for all N.
+template <int BIAS, bool SHORT, int N>
 __device__ __forceinline__ void quant_codes(const float (&x)[N], float s, float inv, uint32_t (&c)[N]) {
   constexpr float MAGIC = 12582912.f + BIAS;
+  if constexpr (SHORT) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float q = x[e] * inv;
+      c[e] = __float_as_uint(fmaf(fmaf(-q, s, x[e]), inv, q) + MAGIC);
+    }
+    return;
+  }
   const float half = 0.5f * s;
   bool close = false;
 #pragma unroll
@@ -189,7 +199,7 @@ __device__ __forceinline__ uint32_t q4_quantise(const Raw8<ST>& raw, float* scal
   *scale = s;
   if (!(s > 0.f)) return 0x88888888u;   // zeros, or not numbers
   uint32_t c[8], p[4];
-  quant_codes<8>(x, s, quant_inverse(s), c);
+  quant_codes<8, sizeof(ST) == 2>(x, s, quant_inverse(s), c);
 #pragma unroll
   for (int i = 0; i < 4; ++i) p[i] = __byte_perm(c[2 * i], c[2 * i + 1], 0x5410);
   return (p[0] + 16u * p[1]) + 256u * (p[2] + 16u * p[3]);

@@ -37,7 +37,7 @@ __device__ __forceinline__ float2 rope_turn(int position, double freq) {
 // elements where rows are not whole chunks), of which a thread has four in flight, the first four before the sines.  A thread stays
 // with one chunk of a head, `half` / (VEC / 2) threads a head, and steps over the (token, head) rows.
 template <typename ST, int VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 rope_positions_kernel(const ST* q_in, const ST* k_in, ST* q_out, ST* k_out, const int* __restrict__ positions, long long rows, int n_pos,
                       int H, int Hkv, int D, int inverse, const __grid_constant__ RopeAxes axes) {
   constexpr int U = 4;
@@ -51,16 +51,16 @@ rope_positions_kernel(const ST* q_in, const ST* k_in, ST* q_out, ST* k_out, cons
   int r = mine < step ? mine / n_heads : n_rows, h = mine < step ? mine - r * n_heads : 0;   // the threads behind the last whole head: none
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
-  auto offset = [&](int rr, int hh) { return (hh < H ? (row0 + rr) * H + hh : (row0 + rr) * Hkv + (hh - H)) * D + d; };
+  const long long q_at = row0 * H * D + d, k_at = row0 * Hkv * D + d;
   bool first = true;
   while (first || r < n_rows) {
     Chunk x[U];
-    int rr[U], hh[U];
+    int rr[U], off[U];   // token; place in the CTA's q, or, negative, in its k
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       rr[u] = r;
-      hh[u] = h;
-      if (r < n_rows) x[u] = *reinterpret_cast<const Chunk*>((h < H ? q_in : k_in) + offset(r, h));
+      off[u] = h < H ? (r * H + h) * D : ~((r * Hkv + h - H) * D);
+      if (r < n_rows) x[u] = *reinterpret_cast<const Chunk*>(off[u] >= 0 ? q_in + q_at + off[u] : k_in + k_at + ~off[u]);
       r += step_r;
       h += step_h;
       if (h >= n_heads) {
@@ -88,7 +88,7 @@ rope_positions_kernel(const ST* q_in, const ST* k_in, ST* q_out, ST* k_out, cons
         rope_st(&x[u].e[2 * p], x0 * cs[p].x - x1 * cs[p].y);
         rope_st(&x[u].e[2 * p + 1], x0 * cs[p].y + x1 * cs[p].x);
       }
-      *reinterpret_cast<Chunk*>((hh[u] < H ? q_out : k_out) + offset(rr[u], hh[u])) = x[u];
+      *reinterpret_cast<Chunk*>(off[u] >= 0 ? q_out + q_at + off[u] : k_out + k_at + ~off[u]) = x[u];
     }
   }
 }
