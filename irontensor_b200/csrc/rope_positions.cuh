@@ -5,7 +5,7 @@
 // The inverse turns back and is the gradient.  The pairs of a head are cut into one section per axis; f(i) and axis(i) come from
 // the host.
 // Angles are in 64 bits: at position 200000 an angle in 32 bits, as rope.cuh has it, is off by up to 0.01, which is 2^-7 of a
-// result; here the whole turns are taken off in 64 bits and the rest of at most pi, then rounded to 32, is off by 2^-24 of itself.
+// result; here whole quarter turns are taken off in 64 bits and the rest, rounded to 32, is off by 2^-24 of itself.
 #pragma once
 #include <cuda_bf16.h>
 
@@ -21,17 +21,42 @@ struct RopeAxes {
   uint8_t axis[64];
 };
 
-// (cos, sin) of position * freq.  |position| < 2^31 and freq is at most a few: up to 2^30 whole turns, so the turn is given in two
-// parts and the product with its first is exact in the fma.
+// (cos, sin) of position * freq.  Quarter turns are taken off in 64 bits: |position| < 2^31 and freq is at most a few, so there are up
+// to 2^32 of them, and pi / 2 is given in two parts, the product with the first of which is exact in the fma.  What is left, at most
+// pi / 4, goes through the Taylor series in 32 bits (their next terms are below 2^-29 there), and the quarter says which is which.
 __device__ __forceinline__ float2 rope_turn(int position, double freq) {
   const double a = static_cast<double>(position) * freq;
-  const double n = rint(a * 0.15915494309189535);            // 1 / (2 pi)
-  double r = fma(-n, 6.283185307179586, a);
-  r = fma(-n, 2.4492935982947064e-16, r);                    // 2 pi - its first part
-  float s, c;
-  sincosf(static_cast<float>(r), &s, &c);
-  return make_float2(c, s);
+  const double n = rint(a * 0.6366197723675814);             // 2 / pi
+  double r = fma(-n, 1.5707963267948966, a);
+  r = fma(-n, 6.123233995736766e-17, r);                     // pi / 2 - its first part
+  const float x = static_cast<float>(r), z = x * x;
+  const float s = fmaf(x * z, fmaf(z, fmaf(z, fmaf(z, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f), x);
+  const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1.f / 3628800.f, 1.f / 40320.f), -1.f / 720.f), 1.f / 24.f), -0.5f), 1.f);
+  const unsigned quarter = static_cast<unsigned>(static_cast<long long>(n)) & 3u;
+  const float ca = quarter & 1u ? s : c, sa = quarter & 1u ? c : s;
+  return make_float2((quarter + 1u) & 2u ? -ca : ca, quarter & 2u ? -sa : sa);
 }
+
+// A chunk of VEC elements in 32-bit words, and its pairs turned.
+template <typename ST, int VEC>
+struct alignas(VEC * sizeof(ST)) RopeChunk {
+  static constexpr int WORDS = VEC * sizeof(ST) / 4;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void turn(const float2* cs) {
+#pragma unroll
+    for (int p = 0; p < VEC / 2; ++p) {
+      const float2 t = cs[p];
+      if constexpr (sizeof(ST) == 2) {
+        const float x0 = __uint_as_float(w[p] << 16), x1 = __uint_as_float(w[p] & 0xFFFF0000u);
+        w[p] = ptx::pack_bf16(x0 * t.x - x1 * t.y, x0 * t.y + x1 * t.x);
+      } else {
+        const float x0 = __uint_as_float(w[2 * p]), x1 = __uint_as_float(w[2 * p + 1]);
+        w[2 * p] = __float_as_uint(x0 * t.x - x1 * t.y);
+        w[2 * p + 1] = __float_as_uint(x0 * t.y + x1 * t.x);
+      }
+    }
+  }
+};
 
 // A CTA owns n_pos tokens: one sine per thread into shared memory, then the heads of q and k in chunks of VEC elements (16 bytes; 2
 // elements where rows are not whole chunks), of which a thread has four in flight, the first four before the sines.  A thread stays
@@ -42,7 +67,7 @@ rope_positions_kernel(const ST* q_in, const ST* k_in, ST* q_out, ST* k_out, cons
                       int H, int Hkv, int D, int inverse, const __grid_constant__ RopeAxes axes) {
   constexpr int U = 4;
   __shared__ float2 tab[256];
-  struct alignas(VEC * sizeof(ST)) Chunk { ST e[VEC]; };
+  using Chunk = RopeChunk<ST, VEC>;
   const int half = D >> 1, per_head = D / VEC, n_heads = H + Hkv;
   const long long row0 = static_cast<long long>(blockIdx.x) * n_pos;
   const int n_rows = static_cast<int>(min(static_cast<long long>(n_pos), rows - row0));
@@ -81,13 +106,7 @@ rope_positions_kernel(const ST* q_in, const ST* k_in, ST* q_out, ST* k_out, cons
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (rr[u] >= n_rows) break;
-      const float2* cs = &tab[rr[u] * half + (d >> 1)];
-#pragma unroll
-      for (int p = 0; p < VEC / 2; ++p) {
-        const float x0 = rope_ld(&x[u].e[2 * p]), x1 = rope_ld(&x[u].e[2 * p + 1]);
-        rope_st(&x[u].e[2 * p], x0 * cs[p].x - x1 * cs[p].y);
-        rope_st(&x[u].e[2 * p + 1], x0 * cs[p].y + x1 * cs[p].x);
-      }
+      x[u].turn(&tab[rr[u] * half + (d >> 1)]);
       *reinterpret_cast<Chunk*>(off[u] >= 0 ? q_out + q_at + off[u] : k_out + k_at + ~off[u]) = x[u];
     }
   }
