@@ -62,11 +62,15 @@ const it::RopeAxes& rope_axes(int D, float base, int n_axes, const int32_t* sect
   return last.axes;
 }
 
-// The grid of the kernels that write and read a cache (kv_q4.cuh).
-it_status cache_grid(int B, int tokens, int Hkv, int D, dim3* grid) {
-  const int64_t rows = static_cast<int64_t>(tokens) * Hkv, per_cta = 256 / (4 * ((D + 31) / 32)) * it::KV_ROWS_A_THREAD;
-  if (rows > 0x7fffffffLL - per_cta) return fail(IT_ERR_UNSUPPORTED_SHAPE, "tokens * kv_heads must be below 2^31");
-  *grid = dim3(static_cast<unsigned>((rows + per_cta - 1) / per_cta), std::min(B, 65535), 2);
+// The grid of the kernels that write and read a cache, and the tokens that a CTA takes at a time (kv_q4.cuh).
+it_status cache_grid(int B, int tokens, int Hkv, int D, dim3* grid, int* at_once) {
+  const int rows = 256 / (4 * ((D + 31) / 32));
+  *at_once = std::clamp(tokens, 1, rows);
+  const int per_cta = *at_once * it::KV_ROWS_A_THREAD, heads = rows / *at_once;
+  const int64_t pairs = static_cast<int64_t>(B) * Hkv;
+  if (pairs > 0x7fffffffLL - 65535 * 64) return fail(IT_ERR_UNSUPPORTED_SHAPE, "batch * kv_heads must be below 2^31");
+  if (tokens > 0x7fffffff - per_cta) return fail(IT_ERR_UNSUPPORTED_SHAPE, "too many tokens");
+  *grid = dim3(static_cast<unsigned>(std::max(1, (tokens + per_cta - 1) / per_cta)), static_cast<unsigned>(std::min<int64_t>((pairs + heads - 1) / heads, 65535)), 2);
   return IT_OK;
 }
 
@@ -198,18 +202,23 @@ it_status it_kv_cache_q4_append(it_ctx* ctx, it_stream* stream, it_dtype dtype, 
   if (T > 0 && (k == nullptr || v == nullptr)) return fail(IT_ERR_INVALID_ARG, "null tensor");
   if (!aligned16(k) || !aligned16(v)) return fail(IT_ERR_ALIGNMENT, "k and v must be 16-byte aligned");
   dim3 grid;
-  if ((st = cache_grid(B, std::max(T, 1), Hkv, D, &grid)) != IT_OK) return st;
+  int at_once;
+  if ((st = cache_grid(B, T, Hkv, D, &grid, &at_once)) != IT_OK) return st;
   IT_CUDA(cudaSetDevice(ctx->device));
   auto launch = [&](auto kernel, auto* kk, auto* vv) -> it_status {
     IT_CUDA(launch_dependent(kernel, grid, 256, 0, stream->s, kk, vv, half_of(k_codes, k_scales), half_of(v_codes, v_scales), lengths, counts,
-                             new_lengths, B, T, Hkv, D, max_len, ctx->d_status));
+                             new_lengths, B, T, Hkv, D, max_len, at_once, ctx->d_status));
     ctx->launches += 1;
     return IT_OK;
   };
   return by_groups(D, [&](auto ng) {
     constexpr int NG = decltype(ng)::value;
-    return dtype == IT_F32 ? launch(it::kv_q4_append_kernel<float, NG>, static_cast<const float*>(k), static_cast<const float*>(v))
-                           : launch(it::kv_q4_append_kernel<__nv_bfloat16, NG>, static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v));
+    const bool full = at_once == 256 / (4 * NG);
+    using BF = __nv_bfloat16;
+    return dtype == IT_F32 ? launch(full ? it::kv_q4_append_kernel<float, NG, true> : it::kv_q4_append_kernel<float, NG, false>,
+                                    static_cast<const float*>(k), static_cast<const float*>(v))
+                           : launch(full ? it::kv_q4_append_kernel<BF, NG, true> : it::kv_q4_append_kernel<BF, NG, false>,
+                                    static_cast<const BF*>(k), static_cast<const BF*>(v));
   });
 }
 
@@ -221,18 +230,20 @@ it_status it_kv_cache_q4_read(it_ctx* ctx, it_stream* stream, it_dtype dtype, in
   if (k == nullptr || v == nullptr) return fail(IT_ERR_INVALID_ARG, "null tensor");
   if (!aligned16(k) || !aligned16(v)) return fail(IT_ERR_ALIGNMENT, "k and v must be 16-byte aligned");
   dim3 grid;
-  if ((st = cache_grid(B, T, Hkv, D, &grid)) != IT_OK) return st;
+  int at_once;
+  if ((st = cache_grid(B, T, Hkv, D, &grid, &at_once)) != IT_OK) return st;
   IT_CUDA(cudaSetDevice(ctx->device));
   auto launch = [&](auto kernel, auto* kk, auto* vv) -> it_status {
     IT_CUDA(launch_dependent(kernel, grid, 256, 0, stream->s, kk, vv, half_of(k_codes, k_scales), half_of(v_codes, v_scales), starts, lengths, B, T,
-                             Hkv, D, max_len));
+                             Hkv, D, max_len, at_once));
     ctx->launches += 1;
     return IT_OK;
   };
   return by_groups(D, [&](auto ng) {
     constexpr int NG = decltype(ng)::value;
+    using BF = __nv_bfloat16;
     return dtype == IT_F32 ? launch(it::kv_q4_read_kernel<float, NG>, static_cast<float*>(k), static_cast<float*>(v))
-                           : launch(it::kv_q4_read_kernel<__nv_bfloat16, NG>, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v));
+                           : launch(it::kv_q4_read_kernel<BF, NG>, static_cast<BF*>(k), static_cast<BF*>(v));
   });
 }
 
