@@ -9,7 +9,9 @@
 //   O^T = V^T P^T A: 16 columns by 16 keys.  A register holds one column of two keys, so two keys' words are interleaved by
 //                 halves first (four byte permutes for 32 codes); B: P of 16 keys and 8 heads, S^T transposed in 8 x 8 tiles
 // with the codes as the larger operand, so that an instruction's 16 rows are all in use whatever the number of heads.
-// P goes in as two bf16 terms, 16 bits; an fp32 q as three terms, as does its P.
+// P goes in as two bf16 terms, 16 bits; an fp32 q as three terms, as does its P.  Where a K/V head has up to four query heads, these are
+// there twice among the instruction's eight columns, and P's terms are its columns 0-3 and 4-7: half the instructions for O (PAIRED; B32 H32/8 D128 ragged to 8190:
+// 51 -> 48.5 us).
 // Which key is which row of S^T, and which column of V is which row of O^T, is free as long as both products agree: the order
 // is the one in which the words lie (q4_dim_of, q4_key_of).
 //
@@ -146,9 +148,12 @@ __device__ __forceinline__ void q4_fetch(uint32_t codes_at, uint32_t scales_at, 
   }
 }
 
-// The running softmax and output of one warp, of 8 R query heads.
-template <int NG, int TERMS, int R>
+// The running softmax and output of one warp, of 8 R query heads; PAIRED: of four, columns h and h + 4 being the upper and the lower
+// term of head h.
+template <int NG, int TERMS, int R, bool PAIRED>
 struct DecodeQ4Warp {
+  static_assert(!PAIRED || (TERMS == 1 && R == 1), "two terms of P, eight columns");
+  static constexpr int PT = PAIRED ? 1 : TERMS == 1 ? 2 : 3;   // instructions for P's terms
   static constexpr int MT = 2 * NG;
   float acc[MT][R][4];   // of m-tile, 8 heads: rows g and g + 8 by heads 2t and 2t + 1
   // Of heads 2t and 2t + 1: what p is relative to, the score above which that is renewed, and this lane's keys' share of the sum.
@@ -190,8 +195,9 @@ struct DecodeQ4Warp {
   __device__ __forceinline__ void load_q(const ST* q, int heads, int D, float scale_log2, int g, int t) {
 #pragma unroll
     for (int h = 0; h < R; ++h) {
-      const bool live = 8 * h + g < heads;
-      const ST* row = q + (8 * h + g) * D;
+      const int head = PAIRED ? g & 3 : 8 * h + g;
+      const bool live = head < heads;
+      const ST* row = q + head * D;
       if constexpr (F16) {
         uint32_t largest = 0;
 #pragma unroll
@@ -329,7 +335,7 @@ struct DecodeQ4Warp {
             for (int h = 0; h < R; ++h) s[i][h][e] = -INFINITY;
     }
     // online softmax; a lane holds 4 of the 32 keys of each of its two heads
-    uint32_t p[TERMS == 1 ? 2 : 3][R][4];   // terms of P, transposed: register x of keys 8x .. 8x + 7
+    uint32_t p[PT][R][4];   // terms of P, transposed: register x of keys 8x .. 8x + 7
 #pragma unroll
     for (int h = 0; h < R; ++h) {
       float mx[2], m_ref[2];
@@ -361,12 +367,18 @@ struct DecodeQ4Warp {
         float p1 = ptx::ex2(fmaf(s[x >> 1][h][2 * (x & 1) + 1], scale[h][1], -m_ref[1]));
         l[h][0] += p0;
         l[h][1] += p1;
+        if constexpr (PAIRED) {
+          const uint32_t upper = ptx::pack_bf16(p0, p1);
+          const uint32_t lower = ptx::pack_bf16(p0 - __uint_as_float(upper << 16), p1 - __uint_as_float(upper & 0xFFFF0000u));
+          p[0][h][x] = transposed_8x8(t < 2 ? upper : lower);
+        } else {
 #pragma unroll
-        for (int y = 0; y < (TERMS == 1 ? 2 : 3); ++y) {
-          const uint32_t term = ptx::pack_bf16(p0, p1);
-          p0 -= __uint_as_float(term << 16);
-          p1 -= __uint_as_float(term & 0xFFFF0000u);
-          p[y][h][x] = transposed_8x8(term);
+          for (int y = 0; y < PT; ++y) {
+            const uint32_t term = ptx::pack_bf16(p0, p1);
+            p0 -= __uint_as_float(term << 16);
+            p1 -= __uint_as_float(term & 0xFFFF0000u);
+            p[y][h][x] = transposed_8x8(term);
+          }
         }
       }
     }
@@ -417,7 +429,7 @@ struct DecodeQ4Warp {
 #pragma unroll
           for (int h = 0; h < R; ++h)
 #pragma unroll
-            for (int y = (TERMS == 1 ? 1 : 2); y >= 0; --y) mma_bf16_16816(acc[mt][h], a0, a1, a2, a3, p[y][h][2 * i], p[y][h][2 * i + 1]);
+            for (int y = PT - 1; y >= 0; --y) mma_bf16_16816(acc[mt][h], a0, a1, a2, a3, p[y][h][2 * i], p[y][h][2 * i + 1]);
         };
         product(4 * f, q4_pair<0>(lo[0], s2[0], bias2[0], magic), q4_pair<0>(hi[0], s2[0], bias2[0], magic), q4_pair<0>(lo[1], s2[1], bias2[1], magic),
                 q4_pair<0>(hi[1], s2[1], bias2[1], magic));
@@ -452,22 +464,28 @@ struct DecodeQ4Warp {
         }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          out[head * PITCH + 16 * mt + g] = acc[mt][h][e];
-          out[head * PITCH + 16 * mt + g + 8] = acc[mt][h][e + 2];
+          float upper = acc[mt][h][e], lower = acc[mt][h][e + 2];   // rows g and g + 8
+          if constexpr (PAIRED) {
+            upper += __shfl_xor_sync(0xffffffffu, upper, 2);
+            lower += __shfl_xor_sync(0xffffffffu, lower, 2);
+            if (t >= 2) continue;
+          }
+          out[head * PITCH + 16 * mt + g] = upper;
+          out[head * PITCH + 16 * mt + g + 8] = lower;
         }
       }
   }
 };
 
 // NG: groups of 32 columns; TERMS: bf16 terms of q (1: bf16 q, two-term P; 3: fp32 q, three-term P); HEADS: query heads of a CTA, 8
-// or, in bf16, 16, which share the operands made of the codes.
+// or, in bf16, 16, which share the operands made of the codes; PAIRED: there are four at most.
 // PLAN_CLUSTER: grid (n_splits, kv_heads * chunks, batch), clusters of n_splits.  PLAN_EVEN: any number of CTAs up to DQ_MAX_CTAS.
-template <int NG, int TERMS, int HEADS, int PLAN>
+template <int NG, int TERMS, int HEADS, bool PAIRED, int PLAN>
 __global__ void __launch_bounds__(32 * dq_warps(TERMS, HEADS, PLAN), TERMS == 1 && HEADS == 8 ? 2 : 1)
 fa_decode_q4_kernel(const DecodeQ4Params prm) {
   using ST = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
   using S = DecodeQ4Stage<NG>;
-  using Warp = DecodeQ4Warp<NG, TERMS, HEADS / 8>;
+  using Warp = DecodeQ4Warp<NG, TERMS, HEADS / 8, PAIRED>;
   constexpr int DQ_WARPS = dq_warps(TERMS, HEADS, PLAN), COLS = 32 * NG, STEP = DQ_WARPS * DQ_BLOCK;
   // A warp leaves its output in the one stage of its ring that is free, while the first keys of the CTA's next stretch are on
   // their way into the others; 16 heads take the whole ring.
@@ -792,6 +810,18 @@ fa_decode_q4_merge_kernel(const DecodeQ4Params prm) {
   }
   if (c0 == c1) return;
   auto part_of = [&](int c) { return (2 * static_cast<size_t>(c) + (c == c0 ? 1 : 0)) * HEADS + h; };
+  // The warp's parts are loaded some at a time, the first of them along with the maxima (one sequence of 131000, 148 parts a pair: 24.6 ->
+  // 21.8 us in all; an even share of the work there is 10 us of it, the scan 0.8, a stretch's end 1.3, this kernel 2.5).
+  constexpr int AT_ONCE = JN == 1 ? 20 : 4;
+  float v[AT_ONCE][JN];
+  auto load = [&](int c) {
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+      for (int j = 0; j < JN; ++j)
+        v[i][j] = c + i * DQ_MERGE_WARPS <= c1 ? prm.part_o[part_of(c + i * DQ_MERGE_WARPS) * COLS + 32 * (j0 + j) + lane] : 0.f;
+  };
+  load(c0 + warp);
   float2 ml[2];   // of up to DQ_MAX_CTAS parts
   float mx = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -821,12 +851,14 @@ fa_decode_q4_merge_kernel(const DecodeQ4Params prm) {
 #pragma unroll
   for (int x = 0; x < DQ_MERGE_WARPS; ++x) sum += s_sum[x];
   float a[JN] = {};
-#pragma unroll 4
-  for (int c = c0 + warp; c <= c1; c += DQ_MERGE_WARPS) {
-    const float e = s_e[c - c0];
-    const float* src = prm.part_o + part_of(c) * COLS + 32 * j0 + lane;
+  for (int c = c0 + warp; c <= c1; c += AT_ONCE * DQ_MERGE_WARPS) {
+    if (c > c0 + warp) load(c);
 #pragma unroll
-    for (int j = 0; j < JN; ++j) a[j] = fmaf(e, src[32 * j], a[j]);
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const float e = c + i * DQ_MERGE_WARPS <= c1 ? s_e[c + i * DQ_MERGE_WARPS - c0] : 0.f;
+#pragma unroll
+      for (int j = 0; j < JN; ++j) a[j] = fmaf(e, v[i][j], a[j]);
+    }
   }
 #pragma unroll
   for (int j = 0; j < JN; ++j) s_acc[warp][32 * j + lane] = a[j];

@@ -111,11 +111,11 @@ int clusters_at_once(Kernel kernel, int size, int threads, int smem_bytes, std::
 
 // How 4-bit attention shares out its work (see fa_decode_q4.cuh): clusters of 1, 2, 4 or 8 CTAs a pair, or even shares.  The lengths are
 // on the device, so this goes by max_len.  In us, measured: a launch of clusters is 4.5, 0.3 for each doubling of the cluster and a
-// round of 256 keys 1.25 for a CTA that has an SM for itself, 2.2 for two on one, at head_dim 128 (B8 H32/8, 4000 positions: 16.5
-// in clusters of two or four, 24.9 alone; B1 H32/8, 16000, clusters of eight: 15.6; 1000 positions of B4 H16/4: 8.5, 7.1, 5.9 and
-// 6.4 with 1, 2, 4 and 8).  An even launch is 16 and its rounds (one sequence of 131000, H16/2: 26, in clusters 88; B32 H32/8
-// ragged to 8190: 53, in clusters 64 and 55; 64 pairs of 4000: 24 and 16.5).  Batches are counted as three quarters full there, because
-// in clusters the longest sequence decides.
+// round of 256 keys 1.25 for a CTA that has an SM for itself, 2.2 for two on one, at head_dim 128 (B8 H32/8, 4000 positions: 16
+// in clusters of two or four, 23.4 alone; B1 H32/8, 16000, clusters of eight: 15; 1000 positions of B4 H16/4: 8.4, 7.1, 6.0 and
+// 6.6 with 1, 2, 4 and 8).  An even launch is 13.5 and its rounds (one sequence of 131000, H16/2: 21.7, in clusters 89; B32 H32/8
+// ragged to 8190: 48.5, in clusters 60, 52 and 56; 64 pairs of 4000: 20.7 and 16).  Batches are counted as three quarters full there,
+// because in clusters the longest sequence decides.
 template <typename AtOnce>
 void choose_decode_q4_plan(long long pairs, int B, int max_len, int sm_count, int per_sm, int groups, AtOnce&& at_once, int* n_splits, bool* even) {
   const double width = 0.35 + 0.65 * groups / 4, two = 2.2 * width, one = per_sm == 1 ? two : 1.25 * width;
@@ -130,7 +130,7 @@ void choose_decode_q4_plan(long long pairs, int B, int max_len, int sm_count, in
     }
   }
   const double rounds = static_cast<double>(pairs) * (max_len + 32.0 * it::DQ_START) / (256.0 * per_sm * sm_count);
-  *even = 16.0 + (B > 1 ? 0.75 : 1.0) * rounds * two < best;
+  *even = 13.5 + (B > 1 ? 0.75 : 1.0) * rounds * two < best;
 }
 
 // Floats of the parts that a persistent attention launch leaves: outputs, then maxima and sums.
@@ -299,17 +299,18 @@ it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype,
   p.units = reinterpret_cast<int*>(ws + decode_q4_part_floats(D));
   int n = 1;
   bool even = false;
-  auto main_launch = [&](auto ng, auto terms, auto hd) -> it_status {
+  auto main_launch = [&](auto ng, auto terms, auto hd, auto paired) -> it_status {
     constexpr int NG = decltype(ng)::value, TERMS = decltype(terms)::value, HEADS = decltype(hd)::value;
+    constexpr bool PAIRED = decltype(paired)::value;
     constexpr int warps = it::dq_warps(TERMS, HEADS, it::PLAN_CLUSTER), even_warps = it::dq_warps(TERMS, HEADS, it::PLAN_EVEN);
     constexpr int bytes = warps * it::DecodeQ4Stage<NG>::WARP_BYTES, even_bytes = even_warps * it::DecodeQ4Stage<NG>::WARP_BYTES;
     static std::atomic<bool> attr_set[16];
     if (!attr_set[ctx->device & 15]) {
-      IT_CUDA(cudaFuncSetAttribute(it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-      IT_CUDA(cudaFuncSetAttribute(it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_EVEN>, cudaFuncAttributeMaxDynamicSharedMemorySize, even_bytes));
+      IT_CUDA(cudaFuncSetAttribute(it::fa_decode_q4_kernel<NG, TERMS, HEADS, PAIRED, it::PLAN_CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+      IT_CUDA(cudaFuncSetAttribute(it::fa_decode_q4_kernel<NG, TERMS, HEADS, PAIRED, it::PLAN_EVEN>, cudaFuncAttributeMaxDynamicSharedMemorySize, even_bytes));
       attr_set[ctx->device & 15] = true;
     }
-    const auto in_clusters = it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_CLUSTER>;
+    const auto in_clusters = it::fa_decode_q4_kernel<NG, TERMS, HEADS, PAIRED, it::PLAN_CLUSTER>;
     static std::atomic<int> at_once[16][9];
     choose_decode_q4_plan(pairs, B, max_len, ctx->sm_count, resident / ctx->sm_count, NG,
                           [&](int size) { return clusters_at_once(in_clusters, size, 32 * warps, bytes, at_once[ctx->device & 15][size]); }, &n, &even);
@@ -320,7 +321,7 @@ it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype,
       ctx->launches += 1;
       return IT_OK;
     }
-    IT_CUDA(launch_dependent(it::fa_decode_q4_kernel<NG, TERMS, HEADS, it::PLAN_EVEN>, grid, 32 * even_warps, even_bytes, stream->s, p));
+    IT_CUDA(launch_dependent(it::fa_decode_q4_kernel<NG, TERMS, HEADS, PAIRED, it::PLAN_EVEN>, grid, 32 * even_warps, even_bytes, stream->s, p));
     using ST = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
     const bool few = B * H < ctx->sm_count;
     IT_CUDA(launch_dependent(few ? it::fa_decode_q4_merge_kernel<ST, NG, HEADS, 1> : it::fa_decode_q4_merge_kernel<ST, NG, HEADS, NG>,
@@ -332,8 +333,9 @@ it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype,
   using three = std::integral_constant<int, 3>;
   using eight = std::integral_constant<int, 8>;
   return by_groups(D, [&](auto ng) {
-    if (dtype == IT_F32) return main_launch(ng, three{}, eight{});
-    return wide ? main_launch(ng, one{}, std::integral_constant<int, 16>{}) : main_launch(ng, one{}, eight{});
+    if (dtype == IT_F32) return main_launch(ng, three{}, eight{}, std::false_type{});
+    if (wide) return main_launch(ng, one{}, std::integral_constant<int, 16>{}, std::false_type{});
+    return G <= 4 ? main_launch(ng, one{}, eight{}, std::true_type{}) : main_launch(ng, one{}, eight{}, std::false_type{});
   });
 }
 
