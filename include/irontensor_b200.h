@@ -284,7 +284,8 @@ it_status it_rope_positions(it_ctx* ctx, it_stream* stream, it_dtype dtype, int3
  * for keys and for values each; 4.5 bits a value where head_dim is a multiple of 32.  32 columns whose largest magnitude is below
  * 2^-100 are zeros, one above 7 * 2^122 saturates, and with a NaN or an infinity among them all 32 read back as NaN.
  * head_dim a multiple of 8 up to 128.  A length below 0 or above max_len is taken as the nearest that is not, no memory outside the
- * cache is touched, and the context's status word reports it (IT_ERR_INVALID_ARG from it_stream_sync and the like). */
+ * cache is touched, and the context reports it (IT_ERR_INVALID_ARG from it_stream_sync and the like, until it_attention_status_poll);
+ * other sequences and later launches are not affected. */
 
 /* k, v [batch, tokens, kv_heads, head_dim] into the cache behind the lengths[b] positions of each sequence: of sequence b its first
  * counts[b] tokens (null: all).  new_lengths[b] = what is there afterwards; it must not be `lengths`.  Nothing else of the cache is

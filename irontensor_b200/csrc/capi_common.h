@@ -47,8 +47,9 @@ struct CaptureSlots {
 struct it_ctx {
   int device = 0;
   int sm_count = 0;
-  int* d_status = nullptr;      // device status word written by kernels whose waits run out
+  int* d_status = nullptr;      // two device status words: of kernels whose waits run out, and of lengths outside a quantised cache
   int* h_status = nullptr;      // pinned mirror
+  int* range_status() const { return d_status + 1; }   // kernels do not stop for this one
   cudaStream_t status_stream = nullptr;   // reads the status word without touching a caller's stream
   std::mutex status_mutex;      // h_status and status_stream are shared by every thread using the context
   EncodeTiledFn encode = nullptr;

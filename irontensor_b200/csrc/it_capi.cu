@@ -131,23 +131,24 @@ struct it_host_step {
 
 namespace {
 
-// Copies the device status word to the host on the context's own stream.  Called after a caller's
-// stream or event has been waited for, so every kernel that could have written the word is done.
+// Copies the device status words to the host on the context's own stream.  Called after a caller's
+// stream or event has been waited for, so every kernel that could have written them is done.  *out: the first that is set.
 it_status read_device_status(it_ctx* ctx, int* out) {
   std::lock_guard<std::mutex> lock(ctx->status_mutex);
-  IT_CUDA(cudaMemcpyAsync(ctx->h_status, ctx->d_status, sizeof(int), cudaMemcpyDeviceToHost, ctx->status_stream));
+  IT_CUDA(cudaMemcpyAsync(ctx->h_status, ctx->d_status, 2 * sizeof(int), cudaMemcpyDeviceToHost, ctx->status_stream));
   IT_CUDA(cudaStreamSynchronize(ctx->status_stream));
-  *out = *ctx->h_status;
+  *out = ctx->h_status[0] != 0 ? ctx->h_status[0] : ctx->h_status[1];
   return IT_OK;
 }
 
 // The error that a device status word stands for.  `left`: it stays set.
 it_status device_status_error(int st, bool left) {
+  if (st == it::DEV_ERR_CACHE_RANGE)
+    return fail(IT_ERR_INVALID_ARG, "a sequence's length lay outside its quantised cache (device status %d)%s", st,
+                left ? ", until it_attention_status_poll clears it" : "");
   const char* then = left ? ": results of launches since then are invalid, and further launches on this context do nothing until "
                             "it_attention_status_poll clears it"
                           : "";
-  if (st == it::DEV_ERR_CACHE_RANGE)
-    return fail(IT_ERR_INVALID_ARG, "a sequence's length lay outside its quantised cache (device status %d)%s", st, then);
   return fail(IT_ERR_TIMEOUT, "a bounded wait inside a kernel ran out (device status %d)%s", st, then);
 }
 
@@ -981,11 +982,11 @@ it_status it_ctx_create(int device, it_ctx** out) {
     return fail(IT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   }
   c->encode = reinterpret_cast<EncodeTiledFn>(fn);
-  if (cudaMalloc(&c->d_status, sizeof(int)) != cudaSuccess || cudaMemset(c->d_status, 0, sizeof(int)) != cudaSuccess ||
+  if (cudaMalloc(&c->d_status, 2 * sizeof(int)) != cudaSuccess || cudaMemset(c->d_status, 0, 2 * sizeof(int)) != cudaSuccess ||
       cudaMalloc(&c->d_work_pool, it_ctx::WORK_BYTES) != cudaSuccess ||
       cudaMemset(c->d_work_pool, 0, it_ctx::WORK_BYTES) != cudaSuccess ||
       cudaStreamSynchronize(cudaStreamLegacy) != cudaSuccess ||   // streams that do not wait for the legacy stream may be the first to launch
-      cudaMallocHost(&c->h_status, sizeof(int)) != cudaSuccess ||
+      cudaMallocHost(&c->h_status, 2 * sizeof(int)) != cudaSuccess ||
       cudaStreamCreateWithFlags(&c->status_stream, cudaStreamNonBlocking) != cudaSuccess) {
     delete c;
     return fail(IT_ERR_CUDA, "could not allocate the status word");
@@ -1775,7 +1776,7 @@ it_status it_attention_status_poll(it_ctx* ctx, it_stream* stream, int32_t* devi
   if (rc != IT_OK) return rc;
   *device_status = word;
   if (*device_status != 0) {
-    IT_CUDA(cudaMemsetAsync(ctx->d_status, 0, sizeof(int), stream->s));
+    IT_CUDA(cudaMemsetAsync(ctx->d_status, 0, 2 * sizeof(int), stream->s));
     IT_CUDA(cudaStreamSynchronize(stream->s));
     return device_status_error(*device_status, false);
   }

@@ -26,6 +26,7 @@ it_status check_cache(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t B,
   if (st != IT_OK) return st;
   if (B < 0 || n < 0 || Hkv < 1 || max_len < 1) return fail(IT_ERR_INVALID_ARG, "bad dimension: batch %d, %d, kv_heads %d, max_len %d", B, n, Hkv, max_len);
   if (D < 8 || D > 128 || (D & 7)) return fail(IT_ERR_UNSUPPORTED_SHAPE, "a quantised cache needs head_dim a multiple of 8 in 8..128, got %d", D);
+  if (max_len > 0x7fffffff - 65536) return fail(IT_ERR_UNSUPPORTED_SHAPE, "max_len must be at most 2^31 - 65537");   // positions are stepped over
   if (B == 0) return IT_OK;
   if (kc == nullptr || ks == nullptr || vc == nullptr || vs == nullptr) return fail(IT_ERR_INVALID_ARG, "null cache");
   if (!aligned16(kc) || !aligned16(vc)) return fail(IT_ERR_ALIGNMENT, "codes must be 16-byte aligned");
@@ -130,7 +131,8 @@ void choose_decode_q4_plan(long long pairs, int B, int max_len, int sm_count, in
     }
   }
   const double rounds = static_cast<double>(pairs) * (max_len + 32.0 * it::DQ_START) / (256.0 * per_sm * sm_count);
-  *even = 13.5 + (B > 1 ? 0.75 : 1.0) * rounds * two < best;
+  const bool countable = static_cast<double>(pairs) * (max_len / 32 + it::DQ_START + 1) < 2e9;   // the shares are counted in 32 bits
+  *even = countable && 13.5 + (B > 1 ? 0.75 : 1.0) * rounds * two < best;
 }
 
 // Floats of the parts that a persistent attention launch leaves: outputs, then maxima and sums.
@@ -210,7 +212,7 @@ it_status it_kv_cache_q4_append(it_ctx* ctx, it_stream* stream, it_dtype dtype, 
   grid.x = std::min<unsigned>(grid.x, std::max(1u, 12u * static_cast<unsigned>(ctx->sm_count) / (2 * grid.y)));
   auto launch = [&](auto kernel, auto* kk, auto* vv) -> it_status {
     IT_CUDA(launch_dependent(kernel, grid, 256, 0, stream->s, kk, vv, half_of(k_codes, k_scales), half_of(v_codes, v_scales), lengths, counts,
-                             new_lengths, B, T, Hkv, D, max_len, at_once, ctx->d_status));
+                             new_lengths, B, T, Hkv, D, max_len, at_once, ctx->range_status()));
     ctx->launches += 1;
     return IT_OK;
   };
@@ -284,7 +286,7 @@ it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype,
   p.lengths = lengths;
   p.o = o;
   p.lse = lse;
-  p.status = ctx->d_status;
+  p.status = ctx->range_status();
   p.H = H;
   p.Hkv = Hkv;
   p.D = D;
@@ -347,6 +349,7 @@ it_status it_quantize_rows_i8(it_ctx* ctx, it_stream* stream, it_dtype dtype, in
   it_status st = check_call(ctx, stream, dtype);
   if (st != IT_OK) return st;
   if (rows < 0 || cols < 0) return fail(IT_ERR_INVALID_ARG, "negative dimension");
+  if (cols > 0x7fffffff - 65536) return fail(IT_ERR_UNSUPPORTED_SHAPE, "too many columns");
   if (cols == 0 || (cols & 15)) return fail(IT_ERR_UNSUPPORTED_SHAPE, "rows to quantise need a multiple of 16 columns, got %d", cols);
   if (rows == 0) return IT_OK;
   if (x == nullptr || codes == nullptr || scales == nullptr) return fail(IT_ERR_INVALID_ARG, "null tensor");
@@ -442,6 +445,7 @@ extern "C" it_status it_linear_i8_fwd(it_ctx* ctx, it_stream* stream, it_dtype o
   it_status st = check_call(ctx, stream, out_dtype);
   if (st != IT_OK) return st;
   if (n < 0 || in_dim < 0 || out_dim < 0) return fail(IT_ERR_INVALID_ARG, "negative dimension");
+  if (n > 0x7fffffff - 65536 || out_dim > 0x7fffffff - 65536) return fail(IT_ERR_UNSUPPORTED_SHAPE, "n and out_dim must be at most 2^31 - 65537");
   if (in_dim < 16 || in_dim > 65536 || (in_dim & 15))
     return fail(IT_ERR_UNSUPPORTED_SHAPE, "in_dim must be a multiple of 16 in 16..65536, got %d", in_dim);
   if (n_outs < 1 || n_outs > 3 || widths == nullptr || outs == nullptr) return fail(IT_ERR_INVALID_ARG, "1 to 3 results, got %d", n_outs);

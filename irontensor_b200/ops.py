@@ -804,6 +804,10 @@ class QuantizedCache:
 
     def __init__(self, codes, scales, head_dim):
         self.codes, self.scales, self.head_dim = codes, scales, head_dim
+        self._check()
+
+    def _check(self):
+        codes, scales, head_dim = self.codes, self.scales, self.head_dim
         if _host_ops.is_cache(codes, scales, head_dim):
             return
         import torch
@@ -833,6 +837,7 @@ class QuantizedCache:
 
     def _halves(self):
         """Addresses of the keys' codes and scales and of the values'."""
+        self._check()   # the attributes may have been set anew
         _on_current_device(self.codes, self.scales)
         k, ks = self.codes.data_ptr(), self.scales.data_ptr()
         return k, ks, k + self.codes.numel() // 2, ks + self.scales.numel()
@@ -844,7 +849,8 @@ def kv_cache_append(cache, k, v, lengths, counts=None):
     (prompts padded to one length).  Returns the new lengths, an int32 tensor [batch].
 
     lengths and counts are int32 tensors [batch] on the device and read there, so that the call can be captured in a CUDA graph.  A
-    token that does not fit into max_len positions is dropped and reported when the stream is next synchronised (ITError)."""
+    token that does not fit into max_len positions is dropped and reported when the stream is next synchronised (ITError); other
+    sequences and later calls are not affected."""
     new = _host_ops.kv_cache_append(cache, k, v, lengths, counts)
     if new is not None:
         return new
@@ -923,6 +929,10 @@ class QuantizedRows:
 
     def __init__(self, codes, scales):
         self.codes, self.scales = codes, scales
+        self._check()
+
+    def _check(self):
+        codes, scales = self.codes, self.scales
         if _host_ops.is_rows(codes, scales):
             return
         import torch
@@ -962,6 +972,8 @@ def linear_int8_forward(input, weight, precision=Precision.BF16, splits=None):
     out = _host_ops.linear_int8_forward(input.codes, input.scales, weight.codes, weight.scales, precision, splits)
     if out is not None:
         return out
+    for rows in (input, weight):
+        rows._check()   # the attributes may have been set anew
     n, k = input.shape()
     out_dim, k2 = weight.shape()
     assert k == k2, "inner dimensions must match"

@@ -127,6 +127,30 @@ def test_append_beyond_the_cache_is_dropped_and_reported(it_ctx):
     assert new.tolist() == [0, 2, 2, 0]
 
 
+def test_a_full_cache_stops_nothing_else(it_ctx):
+    """Launches between the one that found a sequence outside its cache and the report of it do their work: whole tiles of 8-bit
+    products, attention, and the cache itself."""
+    import torch
+    from irontensor_b200 import attention
+    rng = np.random.default_rng(51)
+    x, w = (quantize_rows(to_tensor(values(rng, s, BF16), BF16)) for s in ((200, 256), (136, 256)))
+    a = [to_tensor(values(rng, (1, 256, 2, 64), BF16), BF16) for _ in range(3)]
+    q, k = to_tensor(values(rng, (2, 4, 64), BF16), BF16), to_tensor(values(rng, (2, 3, 2, 64), BF16), BF16)
+    cache = QuantizedCache.zeros(2, 4, 2, 64)
+    run = lambda n: [t.torch().clone() for t in (linear_int8_forward(x, w, FP32), attention(*a, True), attention_decode_quantized(q, cache, n))]
+    kv_cache_append(cache, k, k, ints([0, 0]))
+    want = run(ints([3, 3]))
+    torch.cuda.synchronize()
+    assert it_ctx.poll_status() == 0
+    n = kv_cache_append(cache, k, k, ints([3, 4]), ints([0, 1]))     # sequence 1 is full
+    got = run(torch.minimum(n, ints([3, 3])))
+    torch.cuda.synchronize()
+    with pytest.raises(_lib.ITError, match="length lay outside"):
+        it_ctx.poll_status()
+    assert it_ctx.poll_status() == 0 and n.tolist() == [3, 4]
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 @pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("B,L,Hkv,D,count,starts,lengths", [
     (1, 1, 1, 8, 1, None, None), (2, 9, 3, 64, 9, None, None), (3, 17, 2, 80, 5, [0, 12, 16], None), (2, 9, 1, 128, 12, [-2, 5], [9, 7]),
@@ -338,7 +362,7 @@ def test_rope_inverse_is_the_gradient(it_ctx):
     assert abs((grad * d).sum() - diff) <= 2.0 ** -20 * (np.abs(g) * (np.abs(x) + np.abs(d)) * 4).sum()
 
 
-def test_rope_in_place_and_of_odd_addresses(it_ctx):
+def test_rope_of_odd_addresses(it_ctx):
     """Rows that start between 16-byte boundaries go in pairs."""
     import torch
     rng = np.random.default_rng(22)
@@ -349,6 +373,23 @@ def test_rope_in_place_and_of_odd_addresses(it_ctx):
     a = rope_positions(Tensor(flat[2:], list(x.shape), BF16), None, at)
     b = rope_positions(to_tensor(x, BF16), None, at)
     assert it_ctx.poll_status() == 0 and torch.equal(a.torch(), b.torch())
+
+
+@pytest.mark.parametrize("precision,D,offset", [(BF16, 64, 0), (FP32, 96, 0), (BF16, 20, 0), (BF16, 64, 2)])
+def test_rope_in_place(it_ctx, precision, D, offset):
+    """By the C entry, whose results may lie where q and k are."""
+    import ctypes
+    import torch
+    rng = np.random.default_rng(52)
+    q, k = to_tensor(values(rng, (2, 37, 5, D), precision), precision), to_tensor(values(rng, (2, 37, 3, D), precision), precision)
+    at = ints(rng.integers(0, 5000, (2, 37)))
+    want = [t.torch().flatten() for t in rope_positions(q, k, at)]
+    def shifted(t):
+        return torch.cat([torch.zeros(offset, dtype=t.dtype, device="cuda"), t.flatten()])[offset:]
+    tq, tk = shifted(q.torch()), shifted(k.torch())
+    _lib.check(it_ctx.lib.it_rope_positions(it_ctx.handle, it_ctx.stream(), _lib.IT_BF16 if precision is BF16 else _lib.IT_F32, 2, 37, 5, 3, D, 10000.0, 1,
+                                            (ctypes.c_int32 * 1)(D // 2), 0, 0, at.data_ptr(), tq.data_ptr(), tk.data_ptr(), tq.data_ptr(), tk.data_ptr()))
+    assert it_ctx.poll_status() == 0 and torch.equal(tq, want[0]) and torch.equal(tk, want[1])
 
 
 # ------------------------------------------------------------------------------------------------ 8-bit projections

@@ -44,6 +44,19 @@ def test_cache_form_is_checked():
         QuantizedRows(torch.zeros((4, 16), dtype=torch.int8), torch.zeros(3))
 
 
+def test_attributes_set_anew_are_checked_when_they_are_used():
+    c, r = cache(), QuantizedRows(torch.zeros((4, 16), dtype=torch.int8), torch.zeros(4))
+    c.scales, r.scales = c.scales[:, :, :, 1:], torch.zeros(3)
+    for call in (lambda: kv_cache_append(c, tensor(2, 1, 2, 64), tensor(2, 1, 2, 64), ints(0, 0)), lambda: kv_cache_read(c, 1),
+                 lambda: attention_decode_quantized(tensor(2, 4, 64), c, ints(0, 0))):
+        with pytest.raises(AssertionError, match="scales must be bfloat16"):
+            call()
+    good = QuantizedRows(torch.zeros((4, 16), dtype=torch.int8), torch.zeros(4))
+    for x, w in ((r, good), (good, r)):
+        with pytest.raises(AssertionError, match="scales must be float32"):
+            linear_int8_forward(x, w)
+
+
 @pytest.mark.parametrize("call,match", [
     (lambda: kv_cache_append(cache(), tensor(2, 1, 2, 64), tensor(2, 1, 2, 64, precision=FP32), ints(0, 0)), "same shape and precision"),
     (lambda: kv_cache_append(cache(), tensor(2, 1, 2, 32), tensor(2, 1, 2, 32), ints(0, 0)), "of the cache"),
