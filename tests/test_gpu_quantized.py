@@ -221,6 +221,54 @@ def test_decode_in_even_shares(it_ctx, precision, H, Hkv, D, max_len, lengths):
     check_decode(it_ctx, precision, q, k, v, lengths, max_len)
 
 
+@pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("H,Hkv", [(3, 3), (4, 2), (3, 1), (8, 2), (5, 1), (12, 2), (8, 1), (9, 1), (32, 2), (17, 1)])
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 72])
+def test_decode_of_groups_of_every_kind(it_ctx, precision, H, Hkv, D):
+    """Up to four heads of a K/V head, up to eight, up to sixteen and more, for each number of groups of 32 columns; by a cluster and in
+    even shares."""
+    rng = np.random.default_rng(100 * D + H)
+    lengths = [130, 0, 1, 700]
+    q = values(rng, (4, H, D), precision)
+    k, v = values(rng, (4, 700, Hkv, D), FP32), values(rng, (4, 700, Hkv, D), FP32)
+    check_decode(it_ctx, precision, q, k, v, lengths, 700)
+    check_decode(it_ctx, precision, q, k, v, lengths, 1 << 17)
+
+
+def test_decode_of_the_most_rows(it_ctx):
+    rng = np.random.default_rng(53)
+    B, H, D = 4369, 15, 8
+    q, k, v = values(rng, (B, H, D), BF16), values(rng, (B, 2, 1, D), FP32), values(rng, (B, 2, 1, D), FP32)
+    check_decode(it_ctx, BF16, q, k, v, rng.integers(0, 3, B), 2)
+
+
+def test_decode_by_two_graphs_at_once(it_ctx):
+    """Captured on one stream, replayed on two: a graph's scratch memory is its own."""
+    import torch
+    rng = np.random.default_rng(54)
+    cases = []
+    for lengths in ([2900, 40], [1500, 2000]):
+        q, k, v = values(rng, (2, 8, 64), BF16), values(rng, (2, 3000, 2, 64), FP32), values(rng, (2, 3000, 2, 64), FP32)
+        want, cache = check_decode(it_ctx, BF16, q, k, v, lengths, 1 << 17)
+        cases.append((want.torch().clone(), to_tensor(q, BF16), cache, ints(lengths)))
+    side, graphs, outs = torch.cuda.Stream(), [], []
+    torch.cuda.synchronize()
+    for _, q, cache, n in cases:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            outs.append([attention_decode_quantized(q, cache, n) for _ in range(10)])
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert it_ctx.poll_status() == 0
+    for (want, *_), got in zip(cases, outs):
+        assert all(torch.equal(x.torch(), want) for x in got)
+    del graphs, g
+
+
 def test_decode_of_many_sequences_in_even_shares(it_ctx):
     """More sequences than a CTA has threads."""
     rng = np.random.default_rng(19)
