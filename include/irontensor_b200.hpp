@@ -8,6 +8,7 @@
 //   attention                    src/ops/attention.rs:286-377          [B,S,H,D]
 //   attention_backward_recompute src/train/helpers.rs:120-193          [B,H,S,D]
 //   attention_gqa / rope_qk / attention_decode: the callers' steps around attention folded in (see each)
+//   rope_positions / QuantizedCache / QuantizedRows and their calls: serving in fewer bits, which the reference does not have
 // Where the reference panics (assert!), these throw std::logic_error with the same message; failures of
 // the library itself throw it::Error carrying the status code.  Header-only; link libirontensor_b200.so.
 // No CPU fallback: every operation needs the CUDA library and a device.
@@ -456,6 +457,172 @@ inline std::tuple<Tensor, Tensor, Tensor> qkv_rope_forward(const Tensor& x, cons
                         static_cast<int32_t>(head_dim), rope_base, position_offset, x.ptr(), w_qkv.ptr(), q.ptr(), k.ptr(), v.ptr(),
                         ws, ws_bytes));
   return {q, k, v};
+}
+
+// ---- serving from 8-bit weights and a 4-bit key/value cache (see the same section of irontensor_b200.h) ----------------
+
+// `size()` numbers on the device: lengths and positions (int32_t), codes and scales.  Copies share the buffer, as Tensors do.
+template <typename T>
+class Array {
+ public:
+  Array() = default;
+  explicit Array(size_t n) : n_(n), buf_(std::make_shared<Buf>()) {
+    if (n > 0) check(it_buf_alloc(Context::global().raw(), n * sizeof(T), &buf_->dev));
+  }
+  static Array from_host(const std::vector<T>& data) {
+    Array a(data.size());
+    if (a.n_ == 0) return a;
+    check(it_buf_upload(Context::global().raw(), Context::global().stream(), a.ptr(), data.data(), a.n_ * sizeof(T)));
+    CommandBatch::sync();   // `data` may go away after the call
+    return a;
+  }
+  std::vector<T> to_host() const {
+    std::vector<T> out(n_);
+    if (n_ == 0) return out;
+    check(it_buf_download(Context::global().raw(), Context::global().stream(), out.data(), ptr(), n_ * sizeof(T)));
+    CommandBatch::sync();
+    return out;
+  }
+  size_t size() const { return n_; }
+  T* ptr() const { return buf_ ? static_cast<T*>(buf_->dev) : nullptr; }
+
+ private:
+  struct Buf {
+    void* dev = nullptr;
+    ~Buf() {
+      if (dev) it_buf_free(Context::global().raw(), dev);
+    }
+  };
+  size_t n_ = 0;
+  std::shared_ptr<Buf> buf_;
+};
+
+inline int32_t dim32(size_t n) {
+  require(n < (size_t{1} << 31), "sizes must be below 2^31");
+  return static_cast<int32_t>(n);
+}
+
+// rope_qk at positions given per token: positions [axes, batch, seq], `sections` dimension pairs by each axis (empty: all by one).
+// k may have no heads, or be an empty Tensor.
+inline std::pair<Tensor, Tensor> rope_positions(const Tensor& q, const Tensor& k, const Array<int32_t>& positions, float base = 10000.f,
+                                                const std::vector<int32_t>& sections = {}, bool per_axis = false, bool inverse = false) {
+  require(q.shape().size() == 4, "q must be 4D [batch, seq, heads, head_dim]");
+  const size_t B = q.shape()[0], S = q.shape()[1], D = q.shape()[3];
+  const bool two = !k.shape().empty();
+  if (two) {
+    require(k.shape().size() == 4 && k.precision() == q.precision(), "k must be 4D and have the precision of q");
+    require(k.shape()[0] == B && k.shape()[1] == S && k.shape()[3] == D, "k must be [batch, seq, kv_heads, head_dim]");
+  }
+  const std::vector<int32_t> parts = sections.empty() ? std::vector<int32_t>{static_cast<int32_t>(D / 2)} : sections;
+  require(positions.size() == parts.size() * B * S, "positions must be [axes, batch, seq], one section for each axis");
+  Tensor qo = Tensor::empty(q.shape(), q.precision()), ko = two ? Tensor::empty(k.shape(), k.precision()) : Tensor();
+  check(it_rope_positions(Context::global().raw(), Context::global().stream(), dtype_code(q.precision()), dim32(B), dim32(S), dim32(q.shape()[2]),
+                          two ? dim32(k.shape()[2]) : 0, dim32(D), base, static_cast<int32_t>(parts.size()), parts.data(), per_axis ? 1 : 0,
+                          inverse ? 1 : 0, positions.ptr(), q.ptr(), k.ptr(), qo.ptr(), ko.ptr()));
+  return {qo, ko};
+}
+
+// A key/value cache in 4 bits.  How many positions of each sequence are valid is the caller's, an Array [batch].
+struct QuantizedCache {
+  size_t batch = 0, max_len = 0, kv_heads = 0, head_dim = 0;
+  Array<uint8_t> codes;      // keys, then values
+  Array<uint16_t> scales;
+  static QuantizedCache zeros(size_t batch, size_t max_len, size_t kv_heads, size_t head_dim) {
+    require(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0, "head_dim must be a multiple of 8 in 8..128");
+    require(kv_heads >= 1 && max_len >= 1, "kv_heads and max_len must be positive");
+    const size_t groups = (head_dim + 31) / 32, rows = batch * kv_heads * max_len;
+    QuantizedCache c{batch, max_len, kv_heads, head_dim, Array<uint8_t>(2 * rows * 16 * groups), Array<uint16_t>(2 * rows * groups)};
+    if (rows == 0) return c;
+    check(it_buf_memset_async(Context::global().raw(), Context::global().stream(), c.codes.ptr(), 0x88, c.codes.size()));
+    check(it_buf_memset_async(Context::global().raw(), Context::global().stream(), c.scales.ptr(), 0, 2 * c.scales.size()));
+    return c;
+  }
+  uint8_t* k_codes() const { return codes.ptr(); }
+  uint8_t* v_codes() const { return codes.ptr() + codes.size() / 2; }
+  uint16_t* k_scales() const { return scales.ptr(); }
+  uint16_t* v_scales() const { return scales.ptr() + scales.size() / 2; }
+};
+
+// New tokens k, v [batch, tokens, kv_heads, head_dim] behind the first lengths[b] positions (of sequence b the first counts[b], null:
+// all); returns the new lengths.
+inline Array<int32_t> kv_cache_append(const QuantizedCache& c, const Tensor& k, const Tensor& v, const Array<int32_t>& lengths,
+                                      const Array<int32_t>* counts = nullptr) {
+  require(k.shape() == v.shape() && k.precision() == v.precision(), "k and v must have the same shape and precision");
+  require(k.shape().size() == 4 && k.shape()[0] == c.batch && k.shape()[2] == c.kv_heads && k.shape()[3] == c.head_dim,
+          "k and v must be [batch, tokens, kv_heads, head_dim] of the cache");
+  require(lengths.size() == c.batch && (counts == nullptr || counts->size() == c.batch), "lengths and counts must have one number a sequence");
+  Array<int32_t> out(c.batch);
+  check(it_kv_cache_q4_append(Context::global().raw(), Context::global().stream(), dtype_code(k.precision()), dim32(c.batch), dim32(k.shape()[1]),
+                              dim32(c.kv_heads), dim32(c.head_dim), dim32(c.max_len), k.ptr(), v.ptr(), lengths.ptr(),
+                              counts != nullptr ? counts->ptr() : nullptr, out.ptr(), c.k_codes(), c.k_scales(), c.v_codes(), c.v_scales()));
+  return out;
+}
+
+// Positions starts[b] .. starts[b] + tokens - 1 (null: from 0) as k, v [batch, tokens, kv_heads, head_dim]; zeros outside 0 .. lengths[b] - 1
+// (null: max_len).
+inline std::pair<Tensor, Tensor> kv_cache_read(const QuantizedCache& c, size_t tokens, const Array<int32_t>* starts = nullptr,
+                                               const Array<int32_t>* lengths = nullptr, Precision p = Precision::BF16) {
+  require((starts == nullptr || starts->size() == c.batch) && (lengths == nullptr || lengths->size() == c.batch),
+          "starts and lengths must have one number a sequence");
+  Tensor k = Tensor::empty({c.batch, tokens, c.kv_heads, c.head_dim}, p), v = Tensor::empty({c.batch, tokens, c.kv_heads, c.head_dim}, p);
+  check(it_kv_cache_q4_read(Context::global().raw(), Context::global().stream(), dtype_code(p), dim32(c.batch), dim32(tokens), dim32(c.kv_heads),
+                            dim32(c.head_dim), dim32(c.max_len), c.k_codes(), c.k_scales(), c.v_codes(), c.v_scales(),
+                            starts != nullptr ? starts->ptr() : nullptr, lengths != nullptr ? lengths->ptr() : nullptr, k.ptr(), v.ptr()));
+  return {k, v};
+}
+
+// attention_decode against a QuantizedCache, each sequence at its own length (the new token's position included).
+inline Tensor attention_decode_quantized(const Tensor& q, const QuantizedCache& c, const Array<int32_t>& lengths) {
+  require(q.shape().size() == 3 && q.shape()[0] == c.batch && q.shape()[2] == c.head_dim, "q must be [batch, heads, head_dim] of the cache");
+  require(q.shape()[1] % c.kv_heads == 0, "num_heads must be divisible by num_kv_heads");
+  require(lengths.size() == c.batch, "lengths must have one number a sequence");
+  const int32_t B = dim32(c.batch), H = dim32(q.shape()[1]), D = dim32(c.head_dim);
+  Tensor out = Tensor::empty(q.shape(), q.precision());
+  out.lse = std::make_shared<Tensor>(Tensor::empty({c.batch, q.shape()[1]}, Precision::FP32));
+  size_t ws_bytes = 0;
+  check(it_attention_decode_q4_workspace_bytes(B, H, D, &ws_bytes));
+  void* const ws = thread_workspace(ws_bytes);
+  check(it_attention_decode_q4(Context::global().raw(), Context::global().stream(), dtype_code(q.precision()), B, H, dim32(c.kv_heads), D,
+                               dim32(c.max_len), q.ptr(), c.k_codes(), c.k_scales(), c.v_codes(), c.v_scales(), lengths.ptr(), out.ptr(),
+                               static_cast<float*>(out.lse->ptr()), ws, ws_bytes));
+  return out;
+}
+
+// A matrix [rows, cols] in 8-bit integers with a scale per row.
+struct QuantizedRows {
+  size_t rows = 0, cols = 0;
+  Array<int8_t> codes;
+  Array<float> scales;
+};
+
+inline QuantizedRows quantize_rows(const Tensor& x) {
+  require(x.shape().size() == 2, "quantize_rows takes [rows, cols]");
+  const size_t rows = x.shape()[0], cols = x.shape()[1];
+  QuantizedRows out{rows, cols, Array<int8_t>(rows * cols), Array<float>(rows)};
+  check(it_quantize_rows_i8(Context::global().raw(), Context::global().stream(), dtype_code(x.precision()), dim32(rows), dim32(cols), x.ptr(),
+                            out.codes.ptr(), out.scales.ptr()));
+  return out;
+}
+
+// output = input @ weight.T in column ranges of these widths, which add up to out (q, k and v from stacked weights).
+inline std::vector<Tensor> linear_int8_forward(const QuantizedRows& input, const QuantizedRows& weight, const std::vector<size_t>& widths,
+                                               Precision p = Precision::BF16) {
+  require(input.cols == weight.cols, "inner dimensions must match");
+  require(!widths.empty() && widths.size() <= 3, "up to three widths");
+  std::vector<Tensor> out;
+  int32_t w32[3] = {};
+  void* ptr[3] = {};
+  for (size_t i = 0; i < widths.size(); ++i) {
+    out.push_back(Tensor::empty({input.rows, widths[i]}, p));
+    w32[i] = dim32(widths[i]);
+    ptr[i] = out.back().ptr();
+  }
+  check(it_linear_i8_fwd(Context::global().raw(), Context::global().stream(), dtype_code(p), dim32(input.rows), dim32(input.cols), dim32(weight.rows),
+                         input.codes.ptr(), input.scales.ptr(), weight.codes.ptr(), weight.scales.ptr(), static_cast<int32_t>(widths.size()), w32, ptr));
+  return out;
+}
+inline Tensor linear_int8_forward(const QuantizedRows& input, const QuantizedRows& weight, Precision p = Precision::BF16) {
+  return linear_int8_forward(input, weight, std::vector<size_t>{weight.rows}, p)[0];
 }
 
 }  // namespace it
