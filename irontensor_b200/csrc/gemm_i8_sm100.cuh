@@ -266,9 +266,6 @@ gemm_i8_sm100_kernel(const __grid_constant__ GemmI8Maps maps, const GemmI8Params
     constexpr int W = 128 / sizeof(OT);      // columns of a piece
     const int row_in_tile = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    // Results of half of L2 and more are no use to their reader there, but would push out the operands, of which each is read by
-    // dozens of tiles (2999 x 2048 -> 6144 in fp32, 74 MB: 34.8 -> 32.1 us).
-    const uint64_t policy = l2_policy(sizeof(OT) * static_cast<size_t>(prm.M) * prm.N >= (size_t{64} << 20));
     uint8_t* piece = smem + T::SMEM_OUT + (warp - 4) * T::OUT_BYTES;
     int t = 0;
     bool ok = true;
@@ -330,7 +327,7 @@ gemm_i8_sm100_kernel(const __grid_constant__ GemmI8Maps maps, const GemmI8Params
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tma_store_4d(&maps.out[range], piece, col0 - begin, m0 + (warp & 3) * 32, 0, 0, policy);
+              tma_store_4d(&maps.out[range], piece, col0 - begin, m0 + (warp & 3) * 32, 0, 0);
               bulk_commit_group();
             }
           }
