@@ -176,7 +176,7 @@ it_status it_rope_positions(it_ctx* ctx, it_stream* stream, it_dtype dtype, int3
                    reinterpret_cast<uintptr_t>(k_out)) & pair_mask))
     return fail(IT_ERR_ALIGNMENT, "q and k must be aligned to a pair of elements");
   // as many tokens a CTA as have two sines per thread and eight chunks, as long as that leaves four CTAs per SM (2 x 4093 tokens of 16 + 4 heads
-  // of 128 in bf16: 17.4 us, with half as many 18.5, with twice as many 17.1; 8 x 600 of 32 + 8: 21.2, 26.6 and 23)
+  // of 128 in bf16: 13.4 us, 6.3 TB/s; 8 x 600 of 32 + 8: 16.1, 6.1 TB/s)
   const int token_chunks = (H + Hkv) * (chunks ? D * elem / 16 : half);
   const int n_pos = static_cast<int>(std::clamp<int64_t>(rows / (4LL * ctx->sm_count), 1, std::clamp(2048 / token_chunks, 1, 512 / half)));
   const int64_t ctas = (rows + n_pos - 1) / n_pos;

@@ -42,10 +42,15 @@ template <typename ST, int VEC>
 struct alignas(VEC * sizeof(ST)) RopeChunk {
   static constexpr int WORDS = VEC * sizeof(ST) / 4;
   uint32_t w[WORDS];
-  __device__ __forceinline__ void turn(const float2* cs) {
+  // c, s: the cosines and the sines of the chunk's pairs, each together and aligned to their size
+  __device__ __forceinline__ void turn(const float* c, const float* s) {
+    struct alignas(2 * VEC) Pairs {
+      float f[VEC / 2];
+    };
+    const Pairs cosines = *reinterpret_cast<const Pairs*>(c), sines = *reinterpret_cast<const Pairs*>(s);
 #pragma unroll
     for (int p = 0; p < VEC / 2; ++p) {
-      const float2 t = cs[p];
+      const float2 t = make_float2(cosines.f[p], sines.f[p]);
       if constexpr (sizeof(ST) == 2) {
         const float x0 = __uint_as_float(w[p] << 16), x1 = __uint_as_float(w[p] & 0xFFFF0000u);
         w[p] = ptx::pack_bf16(x0 * t.x - x1 * t.y, x0 * t.y + x1 * t.x);
@@ -66,7 +71,9 @@ __global__ void __launch_bounds__(256, 4)
 rope_positions_kernel(const ST* q_in, const ST* k_in, ST* q_out, ST* k_out, const int* __restrict__ positions, long long rows, int n_pos,
                       int H, int Hkv, int D, int inverse, const __grid_constant__ RopeAxes axes) {
   constexpr int U = 4;
-  __shared__ float2 tab[512];
+  // cosines and sines apart: a chunk's are a load of 16 bytes each, without bank conflicts (as pairs of both 17.4 -> 13.4 us where the comment
+  // below has its figures)
+  __shared__ __align__(16) float cosines[512], sines[512];
   __shared__ double freq[64];
   __shared__ uint8_t axis[64];
   using Chunk = RopeChunk<ST, VEC>;
@@ -104,9 +111,9 @@ rope_positions_kernel(const ST* q_in, const ST* k_in, ST* q_out, ST* k_out, cons
     if (first) {   // every thread passes here once
       for (int i = static_cast<int>(threadIdx.x); i < n_rows * half; i += 256) {
         const int tr = i / half, pair = i - tr * half;
-        float2 cs = rope_turn(positions[axis[pair] * rows + row0 + tr], freq[pair]);
-        if (inverse) cs.y = -cs.y;
-        tab[i] = cs;
+        const float2 cs = rope_turn(positions[axis[pair] * rows + row0 + tr], freq[pair]);
+        cosines[i] = cs.x;
+        sines[i] = inverse ? -cs.y : cs.y;
       }
       __syncthreads();
       first = false;
@@ -114,7 +121,7 @@ rope_positions_kernel(const ST* q_in, const ST* k_in, ST* q_out, ST* k_out, cons
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (rr[u] >= n_rows) break;
-      x[u].turn(&tab[rr[u] * half + (d >> 1)]);
+      x[u].turn(&cosines[rr[u] * half + (d >> 1)], &sines[rr[u] * half + (d >> 1)]);
       *reinterpret_cast<Chunk*>(off[u] >= 0 ? q_out + q_at + off[u] : k_out + k_at + ~off[u]) = x[u];
     }
   }
