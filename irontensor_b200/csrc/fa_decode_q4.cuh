@@ -11,7 +11,7 @@
 // with the codes as the larger operand, so that an instruction's 16 rows are all in use whatever the number of heads.
 // P goes in as two bf16 terms, 16 bits; an fp32 q as three terms, as does its P.  Where a K/V head has up to four query heads, these are
 // there twice among the instruction's eight columns, and P's terms are its columns 0-3 and 4-7: half the instructions for O (PAIRED; B32 H32/8 D128 ragged to 8190:
-// 51 -> 48.5 us).
+// 51 -> 48.5 us when it came).
 // Which key is which row of S^T, and which column of V is which row of O^T, is free as long as both products agree: the order
 // is the one in which the words lie (q4_dim_of, q4_key_of).
 //
@@ -40,9 +40,12 @@ namespace it {
 
 constexpr int DQ_BLOCK = 32, DQ_STAGES = 3, DQ_MAX_CTAS = 512, DQ_START = 12;
 enum : int { PLAN_CLUSTER = 0, PLAN_EVEN = 1 };
-// Warps of a CTA: eight, or six in the persistent launches of which two CTAs are on an SM: 168 registers a thread, which the loop needs
-// more than it needs a fourth warp on each scheduler with 128 and some of them in memory (B32 H32/8 D128 ragged to 8190: 52.7 -> 50.0 us).
-__host__ __device__ constexpr int dq_warps(int terms, int heads, int plan) { return plan == PLAN_EVEN && terms == 1 && heads == 8 ? 6 : 8; }
+// Warps of a CTA and CTAs of an SM.  The persistent launches of bf16 have three CTAs of four warps: 168 registers a thread, which the loop
+// needs more than it needs a fourth warp on each scheduler with 128 and some of them in memory (B32 H32/8 D128 ragged to 8190, where this
+// is 46.5 us: with eight warps twice 2.5 more, six warps twice 2), and few warps that wait for one another where a stretch ends.
+__host__ __device__ constexpr bool dq_threes(int terms, int heads, int plan) { return plan == PLAN_EVEN && terms == 1 && heads == 8; }
+__host__ __device__ constexpr int dq_warps(int terms, int heads, int plan) { return dq_threes(terms, heads, plan) ? 4 : 8; }
+__host__ __device__ constexpr int dq_ctas(int terms, int heads, int plan) { return dq_threes(terms, heads, plan) ? 3 : terms == 1 && heads == 8 ? 2 : 1; }
 constexpr int DQ_MERGE_WARPS = 8;
 
 struct DecodeQ4Params {
@@ -481,7 +484,7 @@ struct DecodeQ4Warp {
 // or, in bf16, 16, which share the operands made of the codes; PAIRED: there are four at most.
 // PLAN_CLUSTER: grid (n_splits, kv_heads * chunks, batch), clusters of n_splits.  PLAN_EVEN: any number of CTAs up to DQ_MAX_CTAS.
 template <int NG, int TERMS, int HEADS, bool PAIRED, int PLAN>
-__global__ void __launch_bounds__(32 * dq_warps(TERMS, HEADS, PLAN), TERMS == 1 && HEADS == 8 ? 2 : 1)
+__global__ void __launch_bounds__(32 * dq_warps(TERMS, HEADS, PLAN), dq_ctas(TERMS, HEADS, PLAN))
 fa_decode_q4_kernel(const DecodeQ4Params prm) {
   using ST = typename std::conditional<TERMS == 1, __nv_bfloat16, float>::type;
   using S = DecodeQ4Stage<NG>;
@@ -812,7 +815,7 @@ fa_decode_q4_merge_kernel(const DecodeQ4Params prm) {
   auto part_of = [&](int c) { return (2 * static_cast<size_t>(c) + (c == c0 ? 1 : 0)) * HEADS + h; };
   // The warp's parts are loaded some at a time, the first of them along with the maxima (one sequence of 131000, 148 parts a pair: 24.6 ->
   // 21.8 us in all; an even share of the work there is 10 us of it, the scan 0.8, a stretch's end 1.3, this kernel 2.5).
-  constexpr int AT_ONCE = JN == 1 ? 20 : 4;
+  constexpr int AT_ONCE = JN == 1 ? 28 : 4;
   float v[AT_ONCE][JN];
   auto load = [&](int c) {
 #pragma unroll

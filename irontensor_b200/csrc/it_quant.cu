@@ -114,8 +114,8 @@ int clusters_at_once(Kernel kernel, int size, int threads, int smem_bytes, std::
 // on the device, so this goes by max_len.  In us, measured: a launch of clusters is 4.5, 0.3 for each doubling of the cluster and a
 // round of 256 keys 1.25 for a CTA that has an SM for itself, 2.2 for two on one, at head_dim 128 (B8 H32/8, 4000 positions: 16
 // in clusters of two or four, 23.4 alone; B1 H32/8, 16000, clusters of eight: 15; 1000 positions of B4 H16/4: 8.4, 7.1, 6.0 and
-// 6.6 with 1, 2, 4 and 8).  An even launch is 13.5 and its rounds (one sequence of 131000, H16/2: 21.7, in clusters 89; B32 H32/8
-// ragged to 8190: 48.5, in clusters 60, 52 and 56; 64 pairs of 4000: 20.7 and 16).  Batches are counted as three quarters full there,
+// 6.6 with 1, 2, 4 and 8).  An even launch is 13.5 and its rounds (one sequence of 131000, H16/2: 22, in clusters 89; B32 H32/8
+// ragged to 8190: 46.5, in clusters 60, 52 and 56; 64 pairs of 4000: 20 and 16).  Batches are counted as three quarters full there,
 // because in clusters the longest sequence decides.
 template <typename AtOnce>
 void choose_decode_q4_plan(long long pairs, int B, int max_len, int sm_count, int per_sm, int groups, AtOnce&& at_once, int* n_splits, bool* even) {
@@ -298,7 +298,6 @@ it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype,
   const bool wide = dtype == IT_BF16 && G > 8;
   const int heads = wide ? 16 : 8, chunks = (G + heads - 1) / heads;
   const long long pairs = static_cast<long long>(B) * Hkv * chunks;
-  const int resident = (dtype == IT_BF16 && !wide ? 2 : 1) * ctx->sm_count;
   float* ws = static_cast<float*>(workspace);
   p.part_o = ws;
   p.part_ml = ws + static_cast<size_t>(2 * it::DQ_MAX_CTAS * 8) * (32 * ((D + 31) / 32));
@@ -318,10 +317,10 @@ it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype,
     }
     const auto in_clusters = it::fa_decode_q4_kernel<NG, TERMS, HEADS, PAIRED, it::PLAN_CLUSTER>;
     static std::atomic<int> at_once[16][9];
-    choose_decode_q4_plan(pairs, B, max_len, ctx->sm_count, resident / ctx->sm_count, NG,
+    choose_decode_q4_plan(pairs, B, max_len, ctx->sm_count, it::dq_ctas(TERMS, HEADS, it::PLAN_CLUSTER), NG,
                           [&](int size) { return clusters_at_once(in_clusters, size, 32 * warps, bytes, at_once[ctx->device & 15][size]); }, &n, &even);
     p.n_splits = n;
-    const dim3 grid = even ? dim3(std::min(resident, wide ? it::DQ_MAX_CTAS / 2 : it::DQ_MAX_CTAS)) : dim3(n, Hkv * chunks, B);
+    const dim3 grid = even ? dim3(std::min(it::dq_ctas(TERMS, HEADS, it::PLAN_EVEN) * ctx->sm_count, wide ? it::DQ_MAX_CTAS / 2 : it::DQ_MAX_CTAS)) : dim3(n, Hkv * chunks, B);
     if (!even) {
       IT_CUDA(launch_cluster(in_clusters, grid, 32 * warps, bytes, stream->s, n, p));
       ctx->launches += 1;
