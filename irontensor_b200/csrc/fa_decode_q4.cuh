@@ -9,14 +9,16 @@
 //   O^T = V^T P^T A: 16 columns by 16 keys.  A register holds one column of two keys, so two keys' words are interleaved by
 //                 halves first (four byte permutes for 32 codes); B: P of 16 keys and 8 heads, S^T transposed in 8 x 8 tiles
 // with the codes as the larger operand, so that an instruction's 16 rows are all in use whatever the number of heads.
-// P goes in as two bf16 terms, 16 bits; an fp32 q as three terms, as does its P.  Where a K/V head has up to four query heads, these are
-// there twice among the instruction's eight columns, and P's terms are its columns 0-3 and 4-7: half the instructions for O (PAIRED; B32 H32/8 D128 ragged to 8190:
-// 51 -> 48.5 us when it came).
+// P goes in as two bf16 terms, 16 bits; an fp32 q as three terms, as does its P.  Where a K/V head has up to four query heads and q is
+// bf16, these are there twice among the instruction's eight columns, and P's terms are its columns 0-3 and 4-7: half the
+// instructions for O (PAIRED; B32 H32/8 D128 ragged to 8190: 51 -> 48.5 us when it came).
 // Which key is which row of S^T, and which column of V is which row of O^T, is free as long as both products agree: the order
 // is the one in which the words lie (q4_dim_of, q4_key_of).
 //
-// The work is bound by reading the cache, 144 bytes a position of a K/V head at head_dim 128, and close behind by the instructions
-// that make operands of it: about 2.3 a value, 600 for the 32 keys that a warp takes at a time.  So
+// What has to be read is 144 bytes a position of a K/V head at head_dim 128; what bounds the work is the instructions that make operands
+// of them: 680 for the 32 keys that a warp takes at a time, 300 of them on the integer unit, beside which matrix instructions of this
+// kind hardly run (4 TB/s of the 6.5 of a copy).  tcgen05 would free that unit of nothing, since the operands are made all the same, and put
+// them through shared or tensor memory and a chain of waits for each tile: 75 us where this takes 46.5.  So
 //   * a warp has a ring of three stages of 32 keys in shared memory, filled by asynchronous copies that nobody but it waits for;
 //     no barrier until a CTA's warps merge what they found;
 //   * long caches: a persistent launch (PLAN_EVEN), in which every CTA takes the same number of 32-key units of the whole batch,

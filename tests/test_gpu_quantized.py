@@ -32,7 +32,7 @@ def values(rng, shape, precision, scale=1.0):
 
 
 def cache_of(k, v, max_len, junk=True):
-    """A QuantizedCache [B, max_len] of rows k, v [B, L, Hkv, D] laid out by the checker; positions behind L hold all bits and NaN."""
+    """A QuantizedCache [B, max_len] of rows k, v [B, L, Hkv, D] laid out by quant_ref.py; positions behind L hold all bits and NaN."""
     import torch
     B, L, Hkv, D = k.shape
     g = -(-D // 32)

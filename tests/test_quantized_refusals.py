@@ -126,7 +126,7 @@ def test_c_entries_refuse_before_the_gpu():
 
 
 def test_reference_bytes_hold_the_reference_values():
-    """The checker's own packing, read back by the formula of the header."""
+    """quant_ref.py packs rows, read back by the formula of the header."""
     x = np.random.default_rng(1).standard_normal((5, 80))
     c, s = qr.q4(x)
     b = qr.q4_bytes(c)
