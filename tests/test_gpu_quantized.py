@@ -104,6 +104,59 @@ def test_append_writes_the_documented_bytes_and_nothing_else(it_ctx, precision, 
     assert np.array_equal(got_codes, codes)
 
 
+@pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B,T,Hkv,D", [(16, 1000, 8, 128), (2, 5000, 40, 24)])
+def test_append_of_many_tokens_padded_to_one_length(it_ctx, precision, B, T, Hkv, D):
+    """A CTA goes on to other tokens, of sequences of which each ends somewhere else."""
+    rng = np.random.default_rng(55)
+    k, v = hard_rows(rng, (B, T, Hkv, D), precision), hard_rows(rng, (B, T, Hkv, D), precision)
+    counts = rng.integers(0, T + 1, B)
+    counts[0], starts = T, rng.integers(0, 4, B)
+    cache = QuantizedCache.zeros(B, T + 4, Hkv, D)
+    new = kv_cache_append(cache, to_tensor(k, precision), to_tensor(v, precision), ints(starts), ints(counts))
+    assert it_ctx.poll_status() == 0 and new.tolist() == (starts + counts).tolist()
+    got_codes, got_scales = host(cache)
+    for i, x in enumerate((k, v)):
+        c, s = qr.q4(x)
+        bytes_ = qr.q4_bytes(c)
+        for b in range(B):
+            there = slice(starts[b], starts[b] + counts[b])
+            assert np.array_equal(got_scales[i, b, :, there], s[b, :counts[b]].swapaxes(0, 1), equal_nan=True)
+            assert np.array_equal(got_codes[i, b, :, there], bytes_[b, :counts[b]].swapaxes(0, 1))
+            got_codes[i, b, :, there], got_scales[i, b, :, there] = 0x88, 0
+    assert np.all(got_codes == 0x88) and np.all(got_scales == 0)
+
+
+def every_bf16_quotient(cols, exponents):
+    """Rows of `cols` whose largest value goes through all 128 mantissas, each beside all mantissas of the given exponents below it."""
+    x = np.concatenate([np.ldexp(np.arange(128, 256), e) for e in exponents])
+    rows = []
+    for largest in range(128, 256):
+        below = x[x <= largest]
+        below = np.concatenate([below, np.zeros(-len(below) % (cols - 1))]).reshape(-1, cols - 1)
+        rows.append(np.concatenate([np.full((len(below), 1), largest), below], 1))
+    x = np.concatenate(rows)
+    x[:, 1::2] *= -1
+    return x
+
+
+def test_every_quotient_of_bf16_values(it_ctx):
+    """Ties and all: what decides between two whole numbers is exact."""
+    x = np.ldexp(every_bf16_quotient(32, range(-7, 1)), -7)
+    L = len(x)
+    t = to_tensor(x.reshape(1, L, 1, 32), BF16)
+    cache = QuantizedCache.zeros(1, L, 1, 32)
+    kv_cache_append(cache, t, t, ints([0]))
+    rows = every_bf16_quotient(1168, range(-9, 1))
+    got = quantize_rows(to_tensor(rows, BF16))
+    assert it_ctx.poll_status() == 0
+    c, s = qr.q4(x.reshape(1, L, 1, 32))
+    codes, scales = host(cache)
+    assert np.array_equal(scales[0, 0, 0], s[0, :, 0]) and np.array_equal(codes[0, 0, 0], qr.q4_bytes(c)[0, :, 0])
+    c, s = qr.q8(rows)
+    assert np.array_equal(got.scales.double().cpu().numpy(), s) and np.array_equal(got.codes.cpu().numpy(), c.astype(np.int8))
+
+
 def test_append_beyond_the_cache_is_dropped_and_reported(it_ctx):
     """max_len 6: sequence 0 has room for one of two tokens, sequence 1 starts before the cache, sequence 2 behind it, 3 fits."""
     import torch
