@@ -322,8 +322,10 @@ kv_q4_read_kernel(ST* __restrict__ k, ST* __restrict__ v, KvQ4 ck, KvQ4 cv, cons
   ST* dst = blockIdx.z ? v : k;
   const KvQ4& c = blockIdx.z ? cv : ck;
   for (int bh0 = static_cast<int>(blockIdx.y) * heads; bh0 < B * Hkv; bh0 += static_cast<int>(gridDim.y) * heads) {
-    const bool none = !at.in || bh0 + at.head >= B * Hkv || d0 >= D;   // or columns that only pad a group; they stay for the exchange below
-    const int bh = none ? bh0 : bh0 + at.head, b = bh / Hkv, h = bh - b * Hkv;
+    // A thread whose columns only pad a group has nothing of its own, but stays with its row: in the exchange below it stores half of
+    // what its neighbour holds, at an address made from the row that both are in.
+    const bool row = at.in && bh0 + at.head < B * Hkv, none = !row || d0 >= D;
+    const int bh = row ? bh0 + at.head : bh0, b = bh / Hkv, h = bh - b * Hkv;
     const long long start = starts != nullptr ? starts[b] : 0;
     const int end = lengths != nullptr ? min(lengths[b], max_len) : max_len;
     uint32_t w[U], s2[U];

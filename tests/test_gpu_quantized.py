@@ -225,6 +225,24 @@ def test_read_gives_the_held_values_and_zeros_outside(it_ctx, precision, B, L, H
         assert y.precision() is precision and np.array_equal(y.to_f32_host(), want)
 
 
+@pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B,T,Hkv", [(2, 1, 2), (3, 5, 2), (2, 9, 3), (7, 2, 5)])
+@pytest.mark.parametrize("D", [8, 24, 40, 56, 72, 88, 104, 120, 16, 128])
+def test_read_of_few_tokens_writes_every_value_of_every_head(it_ctx, precision, D, B, T, Hkv):
+    """Several heads share a CTA, and with an odd number of 8 columns a head's last ones have no neighbour: by the C entry into memory
+    that is NaN beforehand, with as much behind it that stays so."""
+    import torch
+    rng = np.random.default_rng(D + T)
+    k, v = values(rng, (B, T, Hkv, D), FP32), values(rng, (B, T, Hkv, D), FP32)
+    cache, n = cache_of(k, v, T + 3), B * T * Hkv * D
+    out = torch.full((2, 2 * n), math.nan, dtype=torch.float32 if precision is FP32 else torch.bfloat16, device="cuda")
+    _lib.check(it_ctx.lib.it_kv_cache_q4_read(it_ctx.handle, it_ctx.stream(), _lib.IT_F32 if precision is FP32 else _lib.IT_BF16, B, T, Hkv, D, T + 3,
+                                              *cache._halves(), None, None, out[0].data_ptr(), out[1].data_ptr()))
+    assert it_ctx.poll_status() == 0
+    for x, y in zip((k, v), out.double().cpu().numpy()):
+        assert np.array_equal(y[:n].reshape(B, T, Hkv, D), qr.q4_values(x)) and np.isnan(y[n:]).all()
+
+
 # ------------------------------------------------------------------------------------------------ attention
 def check_decode(it_ctx, precision, q, k, v, lengths, max_len, bound=1.0):
     """Error against 64 bits on the held values.  A score is a sum of D exact products in fp32, off by at most 2^-20 of the products'
