@@ -39,6 +39,11 @@ inline void check(it_status s) {
 inline void require(bool cond, const char* msg) {
   if (!cond) throw std::logic_error(msg);
 }
+// A size as the C entries take it.
+inline int32_t dim32(size_t n) {
+  require(n < (size_t{1} << 31), "sizes must be below 2^31");
+  return static_cast<int32_t>(n);
+}
 
 enum class Precision { FP32, BF16 };
 inline size_t byte_size(Precision p) { return p == Precision::FP32 ? 4 : 2; }
@@ -244,8 +249,7 @@ inline Tensor flash_attention(const Tensor& q, const Tensor& k, const Tensor& v,
   out.lse = std::make_shared<Tensor>(Tensor::zeros({s[0], s[1], s[2]}, Precision::FP32));
   if (s[2] == 0 || s[0] * s[1] == 0) return out;
   check(it_flash_attention_fwd(Context::global().raw(), Context::global().stream(), dtype_code(q.precision()),
-                               static_cast<int32_t>(s[0]), static_cast<int32_t>(s[1]), static_cast<int32_t>(s[2]),
-                               static_cast<int32_t>(s[3]), causal ? 1 : 0, q.ptr(), k.ptr(), v.ptr(), out.ptr(),
+                               dim32(s[0]), dim32(s[1]), dim32(s[2]), dim32(s[3]), causal ? 1 : 0, q.ptr(), k.ptr(), v.ptr(), out.ptr(),
                                static_cast<float*>(out.lse->ptr())));
   return out;
 }
@@ -268,13 +272,10 @@ inline std::tuple<Tensor, Tensor, Tensor> attention_backward_recompute(const Ten
     o = &fwd;
   }
   size_t ws_bytes = 0;
-  check(it_flash_attention_bwd_workspace_bytes(dtype_code(q.precision()), static_cast<int32_t>(s[0]),
-                                               static_cast<int32_t>(s[1]), static_cast<int32_t>(s[2]),
-                                               static_cast<int32_t>(s[3]), &ws_bytes));
+  check(it_flash_attention_bwd_workspace_bytes(dtype_code(q.precision()), dim32(s[0]), dim32(s[1]), dim32(s[2]), dim32(s[3]), &ws_bytes));
   void* const ws = thread_workspace(ws_bytes);
   check(it_flash_attention_bwd(Context::global().raw(), Context::global().stream(), dtype_code(q.precision()),
-                               static_cast<int32_t>(s[0]), static_cast<int32_t>(s[1]), static_cast<int32_t>(s[2]),
-                               static_cast<int32_t>(s[3]), causal ? 1 : 0, q.ptr(), k.ptr(), v.ptr(), o->ptr(),
+                               dim32(s[0]), dim32(s[1]), dim32(s[2]), dim32(s[3]), causal ? 1 : 0, q.ptr(), k.ptr(), v.ptr(), o->ptr(),
                                grad_output.ptr(), static_cast<const float*>(o->lse->ptr()), dq.ptr(), dk.ptr(), dv.ptr(),
                                ws, ws_bytes));
   return {dq, dk, dv};
@@ -300,13 +301,12 @@ inline Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, bool 
   if (causal) require(k.shape()[1] == S, "Causal attention requires Q and K to have same seq_len");
   if (k.shape()[1] != S) {
     check(it_attention_cross_fwd(Context::global().raw(), Context::global().stream(), dtype_code(q.precision()),
-                                 static_cast<int32_t>(B), static_cast<int32_t>(S), static_cast<int32_t>(k.shape()[1]),
-                                 static_cast<int32_t>(H), static_cast<int32_t>(D), q.ptr(), k.ptr(), v.ptr(), out.ptr(),
+                                 dim32(B), dim32(S), dim32(k.shape()[1]), dim32(H), dim32(D), q.ptr(), k.ptr(), v.ptr(), out.ptr(),
                                  static_cast<float*>(out.lse->ptr())));
     return out;
   }
   check(it_attention_fwd(Context::global().raw(), Context::global().stream(), dtype_code(q.precision()),
-                         static_cast<int32_t>(B), static_cast<int32_t>(S), static_cast<int32_t>(H), static_cast<int32_t>(D),
+                         dim32(B), dim32(S), dim32(H), dim32(D),
                          causal ? 1 : 0, q.ptr(), k.ptr(), v.ptr(), out.ptr(), static_cast<float*>(out.lse->ptr())));
   return out;
 }
@@ -320,13 +320,10 @@ inline std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor& grad_
   Tensor dq = Tensor::zeros(s, q.precision()), dk = Tensor::zeros(s, q.precision()), dv = Tensor::zeros(s, q.precision());
   if (s[1] == 0 || s[0] * s[2] == 0) return {dq, dk, dv};
   size_t ws_bytes = 0;
-  check(it_flash_attention_bwd_workspace_bytes(dtype_code(q.precision()), static_cast<int32_t>(s[0]),
-                                               static_cast<int32_t>(s[2]), static_cast<int32_t>(s[1]),
-                                               static_cast<int32_t>(s[3]), &ws_bytes));
+  check(it_flash_attention_bwd_workspace_bytes(dtype_code(q.precision()), dim32(s[0]), dim32(s[2]), dim32(s[1]), dim32(s[3]), &ws_bytes));
   void* const ws = thread_workspace(ws_bytes);
   check(it_attention_bwd(Context::global().raw(), Context::global().stream(), dtype_code(q.precision()),
-                         static_cast<int32_t>(s[0]), static_cast<int32_t>(s[1]), static_cast<int32_t>(s[2]),
-                         static_cast<int32_t>(s[3]), causal ? 1 : 0, q.ptr(), k.ptr(), v.ptr(), o.ptr(), grad_output.ptr(),
+                         dim32(s[0]), dim32(s[1]), dim32(s[2]), dim32(s[3]), causal ? 1 : 0, q.ptr(), k.ptr(), v.ptr(), o.ptr(), grad_output.ptr(),
                          static_cast<const float*>(o.lse->ptr()), dq.ptr(), dk.ptr(), dv.ptr(), ws, ws_bytes));
   return {dq, dk, dv};
 }
@@ -344,8 +341,7 @@ inline Tensor attention_gqa(const Tensor& q, const Tensor& k, const Tensor& v, b
   out.lse = std::make_shared<Tensor>(Tensor::zeros({B, H, S}, Precision::FP32));
   if (B * S * H == 0) return out;
   check(it_attention_gqa_fwd(Context::global().raw(), Context::global().stream(), dtype_code(q.precision()),
-                             static_cast<int32_t>(B), static_cast<int32_t>(S), static_cast<int32_t>(H),
-                             static_cast<int32_t>(Hkv), static_cast<int32_t>(D), causal ? 1 : 0, q.ptr(), k.ptr(), v.ptr(),
+                             dim32(B), dim32(S), dim32(H), dim32(Hkv), dim32(D), causal ? 1 : 0, q.ptr(), k.ptr(), v.ptr(),
                              out.ptr(), static_cast<float*>(out.lse->ptr())));
   return out;
 }
@@ -360,8 +356,7 @@ inline std::tuple<Tensor, Tensor, Tensor> attention_gqa_backward(const Tensor& g
   const auto& s = q.shape();
   require(s.size() == 4 && grad_output.shape() == s && o.shape() == s && k.shape() == v.shape(), "shape mismatch");
   require(static_cast<bool>(o.lse), "o must come from attention_gqa()");
-  const int32_t B = static_cast<int32_t>(s[0]), S = static_cast<int32_t>(s[1]), H = static_cast<int32_t>(s[2]),
-                D = static_cast<int32_t>(s[3]), Hkv = static_cast<int32_t>(k.shape()[2]);
+  const int32_t B = dim32(s[0]), S = dim32(s[1]), H = dim32(s[2]), D = dim32(s[3]), Hkv = dim32(k.shape()[2]);
   Tensor dq = Tensor::zeros(s, q.precision()), dk = Tensor::zeros(k.shape(), q.precision()), dv = Tensor::zeros(k.shape(), q.precision());
   if (s[0] * s[1] * s[2] == 0) return {dq, dk, dv};
   size_t ws_bytes = 0;
@@ -389,8 +384,8 @@ inline std::pair<Tensor, Tensor> rope_qk(const Tensor& q, const Tensor& k, float
   require(k.shape()[0] == q.shape()[0] && k.shape()[1] == q.shape()[1] && k.shape()[3] == q.shape()[3], "q and k must agree");
   Tensor qo = Tensor::empty(q.shape(), q.precision()), ko = Tensor::empty(k.shape(), q.precision());
   check(it_rope_qk(Context::global().raw(), Context::global().stream(), dtype_code(q.precision()),
-                   static_cast<int32_t>(q.shape()[0]), static_cast<int32_t>(q.shape()[1]), static_cast<int32_t>(q.shape()[2]),
-                   static_cast<int32_t>(k.shape()[2]), static_cast<int32_t>(q.shape()[3]), base, position_offset, inverse ? 1 : 0,
+                   dim32(q.shape()[0]), dim32(q.shape()[1]), dim32(q.shape()[2]),
+                   dim32(k.shape()[2]), dim32(q.shape()[3]), base, position_offset, inverse ? 1 : 0,
                    q.ptr(), k.ptr(), qo.ptr(), ko.ptr()));
   return {qo, ko};
 }
@@ -400,16 +395,16 @@ inline std::pair<Tensor, Tensor> rope_qk(const Tensor& q, const Tensor& k, float
 // forward per token, src/inference/generator.rs:146-200.)
 inline Tensor attention_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, size_t kv_len) {
   require(q.shape().size() == 3 && k_cache.shape().size() == 4 && k_cache.shape() == v_cache.shape(), "shape mismatch");
-  const int32_t B = static_cast<int32_t>(q.shape()[0]), H = static_cast<int32_t>(q.shape()[1]),
-                D = static_cast<int32_t>(q.shape()[2]), max_len = static_cast<int32_t>(k_cache.shape()[1]),
-                Hkv = static_cast<int32_t>(k_cache.shape()[2]);
+  const int32_t B = dim32(q.shape()[0]), H = dim32(q.shape()[1]),
+                D = dim32(q.shape()[2]), max_len = dim32(k_cache.shape()[1]),
+                Hkv = dim32(k_cache.shape()[2]);
   Tensor out = Tensor::zeros(q.shape(), q.precision());
   out.lse = std::make_shared<Tensor>(Tensor::zeros({q.shape()[0], q.shape()[1]}, Precision::FP32));
   size_t ws_bytes = 0;
   check(it_attention_decode_workspace_bytes(B, H, D, &ws_bytes));
   void* const ws = thread_workspace(ws_bytes);
   check(it_attention_decode(Context::global().raw(), Context::global().stream(), dtype_code(q.precision()), B, H, Hkv, D,
-                            static_cast<int32_t>(kv_len), max_len, q.ptr(), k_cache.ptr(), v_cache.ptr(), out.ptr(),
+                            dim32(kv_len), max_len, q.ptr(), k_cache.ptr(), v_cache.ptr(), out.ptr(),
                             static_cast<float*>(out.lse->ptr()), ws, ws_bytes));
   return out;
 }
@@ -420,8 +415,8 @@ inline Tensor linear_forward(const Tensor& input, const Tensor& weight) {
   require(input.shape().size() == 2 && weight.shape().size() == 2 && input.shape()[1] == weight.shape()[1],
           "inner dimensions must match");
   Tensor y = Tensor::empty({input.shape()[0], weight.shape()[0]}, Precision::BF16);
-  check(it_linear_fwd(Context::global().raw(), Context::global().stream(), static_cast<int32_t>(input.shape()[0]),
-                      static_cast<int32_t>(input.shape()[1]), static_cast<int32_t>(weight.shape()[0]), input.ptr(), weight.ptr(),
+  check(it_linear_fwd(Context::global().raw(), Context::global().stream(), dim32(input.shape()[0]),
+                      dim32(input.shape()[1]), dim32(weight.shape()[0]), input.ptr(), weight.ptr(),
                       y.ptr()));
   return y;
 }
@@ -433,8 +428,7 @@ inline std::pair<Tensor, Tensor> linear_backward(const Tensor& grad_output, cons
   const size_t n = grad_output.shape()[0], out = grad_output.shape()[1], in = input.shape()[1];
   require(input.shape()[0] == n && weight.shape()[0] == out && weight.shape()[1] == in, "shape mismatch");
   Tensor dx = Tensor::empty({n, in}, Precision::BF16), dw = Tensor::empty({out, in}, Precision::FP32);
-  check(it_linear_bwd(Context::global().raw(), Context::global().stream(), static_cast<int32_t>(n), static_cast<int32_t>(in),
-                      static_cast<int32_t>(out), grad_output.ptr(), input.ptr(), weight.ptr(), dx.ptr(),
+  check(it_linear_bwd(Context::global().raw(), Context::global().stream(), dim32(n), dim32(in), dim32(out), grad_output.ptr(), input.ptr(), weight.ptr(), dx.ptr(),
                       static_cast<float*>(dw.ptr())));
   return {dx, dw};
 }
@@ -450,11 +444,10 @@ inline std::tuple<Tensor, Tensor, Tensor> qkv_rope_forward(const Tensor& x, cons
   Tensor q = Tensor::empty({B, S, heads, head_dim}, Precision::BF16), k = Tensor::empty({B, S, kv_heads, head_dim}, Precision::BF16),
          v = Tensor::empty({B, S, kv_heads, head_dim}, Precision::BF16);
   size_t ws_bytes = 0;
-  check(it_qkv_rope_workspace_bytes(static_cast<int32_t>(S), static_cast<int32_t>(head_dim), &ws_bytes));
+  check(it_qkv_rope_workspace_bytes(dim32(S), dim32(head_dim), &ws_bytes));
   void* const ws = thread_workspace(ws_bytes);
-  check(it_qkv_rope_fwd(Context::global().raw(), Context::global().stream(), static_cast<int32_t>(B), static_cast<int32_t>(S),
-                        static_cast<int32_t>(hidden), static_cast<int32_t>(heads), static_cast<int32_t>(kv_heads),
-                        static_cast<int32_t>(head_dim), rope_base, position_offset, x.ptr(), w_qkv.ptr(), q.ptr(), k.ptr(), v.ptr(),
+  check(it_qkv_rope_fwd(Context::global().raw(), Context::global().stream(), dim32(B), dim32(S),
+                        dim32(hidden), dim32(heads), dim32(kv_heads), dim32(head_dim), rope_base, position_offset, x.ptr(), w_qkv.ptr(), q.ptr(), k.ptr(), v.ptr(),
                         ws, ws_bytes));
   return {q, k, v};
 }
@@ -496,11 +489,6 @@ class Array {
   size_t n_ = 0;
   std::shared_ptr<Buf> buf_;
 };
-
-inline int32_t dim32(size_t n) {
-  require(n < (size_t{1} << 31), "sizes must be below 2^31");
-  return static_cast<int32_t>(n);
-}
 
 // rope_qk at positions given per token: positions [axes, batch, seq], `sections` dimension pairs by each axis (empty: all by one).
 // k may have no heads, or be an empty Tensor.

@@ -140,12 +140,18 @@ bool call(F&& f) {
   return raise_status(rc);
 }
 
-// The plain case: a contiguous, non-empty fp32 or bf16 tensor of `dim` dimensions on the current device.
+// Sizes that the C entries' 32-bit arguments hold.
+bool sizes_fit(const at::Tensor& t) {
+  for (const int64_t n : t.sizes())
+    if (n > INT32_MAX) return false;
+  return true;
+}
+// The plain case: a contiguous, non-empty fp32 or bf16 tensor of `dim` dimensions, none of 2^31 or more, on the current device.
 bool plain(PyObject* o, int64_t dim) {
   if (!is_tensor(o)) return false;
   const at::Tensor& t = ten(o);
   return (is_bf16(t) || t.scalar_type() == at::kFloat) && t.dim() == dim && t.is_cuda() && t.numel() > 0 && t.is_contiguous() &&
-         t.get_device() == c10::cuda::current_device();
+         t.get_device() == c10::cuda::current_device() && sizes_fit(t);
 }
 bool same(const at::Tensor& a, const at::Tensor& b) { return a.sizes() == b.sizes() && a.scalar_type() == b.scalar_type(); }
 it_dtype dtype_of(const at::Tensor& t) { return is_bf16(t) ? IT_BF16 : IT_F32; }
@@ -538,6 +544,11 @@ struct Cache {
   static void* w(const T* p) { return const_cast<void*>(static_cast<const void*>(p)); }
 };
 
+// A torch tensor: whether the ops take one of its sizes.
+PyObject* fits(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  IT_ARGS(1);
+  return PyBool_FromLong(THPVariable_Check(a[0]) && sizes_fit(THPVariable_Unpack(a[0])));
+}
 // codes, scales, head_dim: whether they are a QuantizedCache's
 PyObject* is_cache(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   IT_ARGS(3);
@@ -903,6 +914,7 @@ PyMethodDef methods[] = {{"setup", setup, METH_VARARGS, nullptr},
                          IT_FN(linear_forward),
                          IT_FN(linear_backward),
                          IT_FN(qkv_rope_forward),
+                         IT_FN(fits),
                          IT_FN(is_cache),
                          IT_FN(is_rows),
                          IT_FN(rope_positions),

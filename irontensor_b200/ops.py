@@ -422,6 +422,11 @@ def _workspace(nbytes):
     return w
 
 
+def _c_ints(*values):
+    """Refuses sizes that the C entries' 32-bit arguments would cut off."""
+    assert all(0 <= v < 1 << 31 for v in values), "sizes must be below 2^31"
+
+
 def flash_attention(q, k, v, causal):
     """FlashAttention forward on [batch, heads, seq, head_dim] (src/ops/flash_attention.rs:76-193).
 
@@ -440,6 +445,7 @@ def flash_attention(q, k, v, causal):
     assert qs == ks, "Q and K must have same shape"
     assert qs == vs, "Q and V must have same shape"
     B, H, S, D = qs
+    _c_ints(B, H, S)
     assert D <= 128, "head_dim must be <= 128"
     if S == 0 or B * H == 0:
         out = Tensor.zeros([B, H, S, D], p)
@@ -474,6 +480,7 @@ def attention(q, k, v, causal):
     assert ks[2] == H and vs[2] == H, "Num heads mismatch"
     assert ks[3] == D and vs[3] == D, "Head dim mismatch"
     assert vs[1] == ks[1], "K and V seq_len must match"
+    _c_ints(*qs, ks[1])
     if B == 0 or Sq == 0 or ks[1] == 0:
         return Tensor.zeros([B, Sq, H, D], p)
     if causal:
@@ -501,6 +508,7 @@ def attention_backward(grad_output, q, k, v, o, causal=True):
     B, S, H, D = q.shape()
     for t in (grad_output, k, v, o):
         assert t.precision() is p and t.shape() == [B, S, H, D], "shape or precision mismatch"
+    _c_ints(B, S, H, D)
     assert o.lse is not None, "o must come from attention()"
     if S == 0 or B * H == 0:
         return Tensor.zeros([B, S, H, D], p), Tensor.zeros([B, S, H, D], p), Tensor.zeros([B, S, H, D], p)
@@ -529,6 +537,7 @@ def attention_gqa(q, k, v, causal=True):
     Hkv = k.shape()[2]
     assert k.shape() == [B, S, Hkv, D], "K/V must be [batch, seq, kv_heads, head_dim]"
     assert Hkv >= 1 and H % Hkv == 0, "num_heads must be divisible by num_kv_heads"   # src/ops/repeat_kv.rs:77-80
+    _c_ints(B, S, H, D)
     out = Tensor.empty([B, S, H, D], p)
     out.lse = Tensor.empty([B, H, S], Precision.FP32)
     if B * S * H == 0:
@@ -546,6 +555,7 @@ def rope(input, base=10000.0, position_offset=0):
     assert len(input.shape()) == 4, "Input must be 4D [batch, seq_len, num_heads, head_dim]"
     B, S, H, D = input.shape()
     assert D % 2 == 0, "head_dim must be even for RoPE"
+    _c_ints(B, S, H, D)
     out = Tensor.empty([B, S, H, D], input.precision())
     raw.rope_qk(_dtype_code(input.precision()), B, S, H, 0, D, base, position_offset, False, input.data_ptr(), None,
                 out.data_ptr(), None)
@@ -561,6 +571,7 @@ def rope_qk(q, k, base=10000.0, position_offset=0, inverse=False):
     B, S, H, D = q.shape()
     Hkv = k.shape()[2]
     assert k.shape() == [B, S, Hkv, D] and k.precision() is q.precision() and D % 2 == 0
+    _c_ints(B, S, H, Hkv, D)
     qo, ko = Tensor.empty([B, S, H, D], q.precision()), Tensor.empty([B, S, Hkv, D], q.precision())
     raw.rope_qk(_dtype_code(q.precision()), B, S, H, Hkv, D, base, position_offset, inverse, q.data_ptr(), k.data_ptr(),
                 qo.data_ptr(), ko.data_ptr())
@@ -582,6 +593,7 @@ def attention_gqa_backward(grad_output, q, k, v, o, causal=True, rope_base=None,
     assert grad_output.shape() == [B, S, H, D] and o.shape() == [B, S, H, D]
     assert k.shape() == [B, S, Hkv, D] and v.shape() == [B, S, Hkv, D] and H % Hkv == 0
     assert o.lse is not None, "o must come from attention_gqa()"
+    _c_ints(B, S, H, Hkv, D)
     dq, dk, dv = Tensor.empty([B, S, H, D], p), Tensor.empty([B, S, Hkv, D], p), Tensor.empty([B, S, Hkv, D], p)
     if B * S * H == 0:
         return dq, dk, dv
@@ -611,6 +623,7 @@ def attention_decode(q, k_cache, v_cache, kv_len):
     B, H, D = q.shape()
     Bc, max_len, Hkv, Dc = k_cache.shape()
     assert Bc == B and Dc == D and H % Hkv == 0 and 1 <= kv_len <= max_len
+    _c_ints(B, H, Hkv, D, max_len)
     out = Tensor.empty([B, H, D], p)
     out.lse = Tensor.empty([B, H], Precision.FP32)
     nbytes = raw.decode_workspace_bytes(B, H, D)
@@ -629,6 +642,7 @@ def linear_forward(input, weight):
     n, k = input.shape()
     out_dim, k2 = weight.shape()
     assert k == k2, "inner dimensions must match"
+    _c_ints(n, k, out_dim)
     y = Tensor.empty([n, out_dim], Precision.BF16)
     raw.linear_fwd(n, k, out_dim, input.data_ptr(), weight.data_ptr(), y.data_ptr())
     return y
@@ -645,6 +659,7 @@ def qkv_rope_forward(x, w_qkv, heads, kv_heads, head_dim, rope_base=10000.0, pos
     assert x.precision() is Precision.BF16 and w_qkv.precision() is Precision.BF16
     B, S, hidden = x.shape()
     assert w_qkv.shape() == [(heads + 2 * kv_heads) * head_dim, hidden], "w_qkv must be [Wq; Wk; Wv] stacked by rows"
+    _c_ints(B, S, hidden, heads, kv_heads, head_dim)
     if packed:
         qkv = Tensor.empty([B, S, (heads + 2 * kv_heads) * head_dim], Precision.BF16)
         raw.qkv_rope_fwd(B, S, hidden, heads, kv_heads, head_dim, 0.0 if rope_base is None else rope_base, position_offset,
@@ -666,6 +681,7 @@ def attention_packed(qkv, heads, kv_heads, head_dim, causal=True):
         return out
     B, S, W = qkv.shape()
     assert qkv.precision() is Precision.BF16 and W == (heads + 2 * kv_heads) * head_dim
+    _c_ints(B, S, heads, kv_heads, head_dim)
     out = Tensor.empty([B, S, heads, head_dim], Precision.BF16)
     out.lse = Tensor.empty([B, heads, S], Precision.FP32)
     raw.packed_fwd(B, S, heads, kv_heads, head_dim, causal, qkv.data_ptr(), out.data_ptr(), out.lse.data_ptr())
@@ -682,6 +698,7 @@ def attention_packed_backward(grad_output, qkv, o, heads, kv_heads, head_dim, ca
         return out
     B, S, W = qkv.shape()
     assert grad_output.shape() == [B, S, heads, head_dim] and o.lse is not None
+    _c_ints(B, S, heads, kv_heads, head_dim)
     dqkv = Tensor.empty([B, S, W], Precision.BF16)
     nbytes = raw.bwd_workspace_bytes(_lib.IT_BF16, B, heads, S, head_dim)
     ws = _workspace(nbytes)
@@ -699,6 +716,7 @@ def linear_backward(grad_output, input, weight):
     n, out_dim = grad_output.shape()
     k = input.shape()[1]
     assert input.shape() == [n, k] and weight.shape() == [out_dim, k]
+    _c_ints(n, k, out_dim)
     dx = Tensor.empty([n, k], Precision.BF16)
     dw = Tensor.empty([out_dim, k], Precision.FP32)
     raw.linear_bwd(n, k, out_dim, grad_output.data_ptr(), input.data_ptr(), weight.data_ptr(), dx.data_ptr(), dw.data_ptr())
@@ -720,6 +738,7 @@ def attention_backward_recompute(grad_output, q, k, v, o=None, lse=None, causal=
     B, H, S, D = q.shape()
     for t in (grad_output, k, v):
         assert t.shape() == [B, H, S, D], "shape mismatch"
+    _c_ints(B, H, S, D)
     if S == 0 or B * H == 0:
         return Tensor.zeros([B, H, S, D], p), Tensor.zeros([B, H, S, D], p), Tensor.zeros([B, H, S, D], p)
     dq, dk, dv = Tensor.empty([B, H, S, D], p), Tensor.empty([B, H, S, D], p), Tensor.empty([B, H, S, D], p)
@@ -740,11 +759,6 @@ def _on_current_device(*tensors):
     for t in tensors:
         assert t.is_cuda and t.get_device() == device, f"tensors must be on the current CUDA device {device}, got one on {t.device}"
         assert t.is_contiguous(), "tensors must be contiguous"
-
-
-def _c_ints(*values):
-    """Refuses sizes that the C entries' 32-bit arguments would cut off."""
-    assert all(0 <= v < 1 << 31 for v in values), "sizes must be below 2^31"
 
 
 def _int32(t, shape, name):

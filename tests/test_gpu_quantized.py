@@ -511,6 +511,22 @@ def test_rope_in_place(it_ctx, precision, D, offset):
     assert it_ctx.poll_status() == 0 and torch.equal(tq, want[0]) and torch.equal(tk, want[1])
 
 
+def test_sizes_that_32_bits_would_cut_off_are_refused(it_ctx):
+    """In front of any allocation of results: a prompt of 2^31 tokens in two columns."""
+    import torch
+    from irontensor_b200 import rope, rope_qk
+    S = 2 ** 31
+    x = Tensor(torch.empty((1, S, 1, 2), dtype=torch.bfloat16, device="cuda"), [1, S, 1, 2], BF16)
+    at = torch.empty((1, S), dtype=torch.int32, device="cuda")
+    before = it_ctx.launch_count()
+    for call in (lambda: rope_positions(x, None, at), lambda: rope_positions(x, x, at), lambda: rope(x), lambda: rope_qk(x, x)):
+        with pytest.raises(AssertionError, match="below 2\\^31"):
+            call()
+    assert it_ctx.launch_count() == before and it_ctx.poll_status() == 0
+    del x, at
+    torch.cuda.empty_cache()
+
+
 # ------------------------------------------------------------------------------------------------ 8-bit projections
 @pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("rows,cols", [(1, 16), (12, 48), (5, 2048), (3, 8192), (25, 8208), (2, 20000)])

@@ -7,7 +7,7 @@ import torch
 
 import quant_ref as qr
 from irontensor_b200 import (Precision, QuantizedCache, QuantizedRows, Tensor, _lib, attention_decode_quantized, kv_cache_append,
-                             kv_cache_read, linear_int8_forward, quantize_rows, rope_positions)
+                             kv_cache_read, linear_int8_forward, ops, quantize_rows, rope_positions)
 
 FP32, BF16 = Precision.FP32, Precision.BF16
 
@@ -136,3 +136,50 @@ def test_reference_bytes_hold_the_reference_values():
         u = (words[:, t * 3 + j] >> (4 * (e // 2) + 16 * (e % 2))) & 15
         assert np.array_equal(u.astype(int) - 8, c[:, d].astype(int))
     assert np.abs(c).max() == 7 and np.all(np.abs(qr.q4_values(x) - x) <= 0.5 * np.repeat(s, 32, -1)[:, :80] * 1.0000001)
+
+
+# ------------------------------------------------------------------------------------------------ sizes of 2^31 and more
+def shapeless(*shape, precision=BF16):
+    """A tensor of this shape without memory."""
+    return Tensor(torch.empty(shape, dtype=torch.float32 if precision is FP32 else torch.bfloat16, device="meta"), list(shape), precision)
+
+
+def test_the_native_path_takes_sizes_below_2_31_only():
+    for shape, ok in (((1, 2 ** 31 - 1, 1, 2), True), ((1, 2 ** 31, 1, 2), False), ((1, 2 ** 32 + 5, 1, 2), False), ((2 ** 32, 8), False), ((3, 0, 2 ** 40), False),
+                      ((), True), ((0,), True)):
+        assert ops._host_ops.fits(torch.empty(shape, dtype=torch.bfloat16, device="meta")) is ok, shape
+    assert ops._host_ops.fits(None) is False
+
+
+FAR = 2 ** 32 + 5
+
+
+def with_lse(o, *shape):
+    o.lse = shapeless(*shape, precision=FP32)
+    return o
+
+
+@pytest.mark.parametrize("call", [
+    lambda: rope_positions(shapeless(1, FAR, 1, 2), None, torch.empty((1, FAR), dtype=torch.int32, device="meta")),
+    lambda: rope_positions(shapeless(2 ** 32, 1, 1, 2), shapeless(2 ** 32, 1, 1, 2), torch.empty((2 ** 32, 1), dtype=torch.int32, device="meta")),
+    lambda: ops.rope(shapeless(1, FAR, 1, 2)),
+    lambda: ops.rope_qk(shapeless(1, FAR, 1, 2), shapeless(1, FAR, 1, 2)),
+    lambda: ops.flash_attention(*[shapeless(1, 1, FAR, 1)] * 3, True),
+    lambda: ops.attention(*[shapeless(1, FAR, 1, 1)] * 3, True),
+    lambda: ops.attention(shapeless(1, 4, 1, 1), *[shapeless(1, FAR, 1, 1)] * 2, False),
+    lambda: ops.attention_backward(*[shapeless(1, FAR, 1, 1)] * 4, with_lse(shapeless(1, FAR, 1, 1), 1, 1, FAR)),
+    lambda: ops.attention_gqa(shapeless(FAR, 1, 2, 1), *[shapeless(FAR, 1, 1, 1)] * 2),
+    lambda: ops.attention_gqa_backward(shapeless(FAR, 1, 2, 1), shapeless(FAR, 1, 2, 1), *[shapeless(FAR, 1, 1, 1)] * 2,
+                                       with_lse(shapeless(FAR, 1, 2, 1), FAR, 2, 1)),
+    lambda: ops.attention_backward_recompute(*[shapeless(1, 1, FAR, 1)] * 4),
+    lambda: ops.attention_decode(shapeless(1, 1, 8), *[shapeless(1, FAR, 1, 8)] * 2, 5),
+    lambda: ops.attention_packed(shapeless(1, FAR, 3), 1, 1, 1),
+    lambda: ops.attention_packed_backward(shapeless(1, FAR, 1, 1), shapeless(1, FAR, 3), with_lse(shapeless(1, FAR, 1, 1), 1, 1, FAR), 1, 1, 1),
+    lambda: ops.linear_forward(shapeless(FAR, 8), shapeless(8, 8)),
+    lambda: ops.linear_backward(shapeless(FAR, 8), shapeless(FAR, 8), shapeless(8, 8)),
+    lambda: ops.qkv_rope_forward(shapeless(1, FAR, 8), shapeless(6, 8), 1, 1, 2),
+    lambda: quantize_rows(shapeless(FAR, 16)),
+])
+def test_sizes_that_32_bits_would_cut_off_are_refused(call):
+    with pytest.raises(AssertionError, match="below 2\\^31"):
+        call()
