@@ -270,7 +270,8 @@ it_status it_attention_packed_bwd(it_ctx* ctx, it_stream* stream, it_dtype dtype
  * none), positions [axes, batch, seq].  Dimension pair i (columns 2i, 2i + 1) turns by positions[axis(i)][token] * f(i), an angle
  * in 64 bits.  sections[a], a < axes (1 to 4), pairs belong to axis a, in order; they add up to head_dim / 2.  per_axis 0: f(i) =
  * base^(-2i / head_dim), one ladder over all pairs (text and video tokens of one model).  per_axis 1: the j-th of an axis's n
- * pairs has f = base^(-j / n), a ladder per axis (images).  inverse != 0 turns back: the gradient.  In place is allowed. */
+ * pairs has f = base^(-j / n), a ladder per axis (images).  A base so far below 1 that an f is above 512 is refused
+ * (IT_ERR_INVALID_ARG).  inverse != 0 turns back: the gradient.  In place is allowed. */
 it_status it_rope_positions(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t batch, int32_t seq, int32_t heads,
                             int32_t kv_heads, int32_t head_dim, float rope_base, int32_t axes, const int32_t* sections,
                             int32_t per_axis, int32_t inverse, const int32_t* positions, const void* q_in, const void* k_in,

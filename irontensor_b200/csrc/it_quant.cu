@@ -36,6 +36,14 @@ it_status check_cache(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t B,
   return IT_OK;
 }
 
+// The largest frequency of the dimension pairs: 1, or with a base below 1 that of the last pair of all or of the longest section.
+double largest_frequency(int D, float base, int n_axes, const int32_t* sections, int per_axis) {
+  if (base >= 1.f) return 1.0;
+  if (!per_axis) return std::pow(static_cast<double>(base), -(D - 2.0) / D);
+  const int n = *std::max_element(sections, sections + n_axes);
+  return std::pow(static_cast<double>(base), -(n - 1.0) / n);
+}
+
 // Frequencies and axes of the dimension pairs.  64 powers in 64 bits take as long as the launch: the last ones are kept, by value.
 const it::RopeAxes& rope_axes(int D, float base, int n_axes, const int32_t* sections, int per_axis) {
   struct Last {
@@ -161,6 +169,8 @@ it_status it_rope_positions(it_ctx* ctx, it_stream* stream, it_dtype dtype, int3
     pairs += sections[a];
   }
   if (pairs != D / 2) return fail(IT_ERR_INVALID_ARG, "sections must add up to head_dim / 2 = %d", D / 2);
+  if (!(largest_frequency(D, rope_base, n_axes, sections, per_axis) <= it::ROPE_MOST_FREQ))
+    return fail(IT_ERR_INVALID_ARG, "rotary base %g makes frequencies above %g", static_cast<double>(rope_base), it::ROPE_MOST_FREQ);
   const int64_t rows = static_cast<int64_t>(B) * S;
   if (rows == 0 || (H == 0 && Hkv == 0)) return IT_OK;
   if (static_cast<int64_t>(H) + Hkv > 65535) return fail(IT_ERR_UNSUPPORTED_SHAPE, "heads + kv_heads must be at most 65535");

@@ -21,9 +21,14 @@ struct RopeAxes {
   uint8_t axis[64];
 };
 
-// (cos, sin) of position * freq.  Quarter turns are taken off in 64 bits: |position| < 2^31 and freq is at most a few, so there are up
-// to 2^32 of them, and pi / 2 is given in two parts, the product with the first of which is exact in the fma.  What is left, at most
-// pi / 4, goes through the Taylor series in 32 bits (their next terms are below 2^-29 there), and the quarter says which is which.
+// A base below 1 makes frequencies above 1.  Up to this one there are at most 2^40 quarter turns to take off, and what is left is right to
+// 2^-53; at 2^20 it is no longer below pi / 4, and behind 2^31 the quarters cannot be counted.
+constexpr double ROPE_MOST_FREQ = 512.0;
+
+// (cos, sin) of position * freq.  Quarter turns are taken off in 64 bits: |position| <= 2^31 and freq <= ROPE_MOST_FREQ, so there are up
+// to 2^40 of them, and pi / 2 is given in two parts, the product with the first of which is exact in the fma, as is the difference.  What
+// is left, at most pi / 4 and 2^-11 of it, goes through the Taylor series in 32 bits (their next terms are below 2^-29 there), and the
+// quarter says which is which.
 __device__ __forceinline__ float2 rope_turn(int position, double freq) {
   const double a = static_cast<double>(position) * freq;
   const double n = rint(a * 0.6366197723675814);             // 2 / pi

@@ -775,7 +775,8 @@ def rope_positions(q, k, positions, base=10000.0, sections=None, per_axis=False,
 
     `sections` says how many of the head_dim / 2 dimension pairs turn by each axis, in order (None: all by the one axis).  Pair i turns
     by position * base^(-2i / head_dim); with `per_axis`, the j-th of an axis's n pairs by position * base^(-j / n).  Angles are
-    in 64 bits: far positions keep their digits.  `inverse` turns back, which is the gradient."""
+    in 64 bits: far positions keep their digits.  A base so far below 1 that a pair turns by more than 512 a position is refused.
+    `inverse` turns back, which is the gradient."""
     out = _host_ops.rope_positions(q, k, positions, base, sections, per_axis, inverse)
     if out is not None:
         return out

@@ -470,6 +470,21 @@ def test_rope_at_given_positions(it_ctx, precision, B, S, H, Hkv, D, sections, p
             assert np.all(np.abs(y.to_f32_host() - want) <= limit)
 
 
+@pytest.mark.parametrize("base,D,sections,per_axis", [(0.5, 64, [32], False), (0.25, 16, [3, 5], True), (2.0 ** -9, 20, [10], False)])
+def test_rope_with_a_base_below_one(it_ctx, base, D, sections, per_axis):
+    """Frequencies above 1, at positions near enough for both sides' angles: below 2^20 x 2^9, which 64 bits hold to 2^-24 (and the
+    powers, off by 2^-52 of themselves on either side, to 2^-22), so a result is off by 2^-20 (|x0| + |x1|) and its roundings."""
+    rng = np.random.default_rng(61)
+    x, at = values(rng, (2, 50, 3, D), FP32), rng.integers(-2 ** 20, 2 ** 20, (len(sections), 2, 50))
+    got = rope_positions(to_tensor(x, FP32), None, ints(at if len(sections) > 1 else at[0]), base, sections, per_axis)
+    want = qr.rope(x, at, base, sections, per_axis)
+    size = np.repeat(np.abs(x[..., 0::2]) + np.abs(x[..., 1::2]), 2, -1)
+    assert it_ctx.poll_status() == 0 and np.all(np.abs(got.to_f32_host() - want) <= 2.0 ** -20 * size + 2.0 ** -24 * np.abs(want))
+    with pytest.raises(_lib.ITError, match="frequencies above 512") as e:
+        rope_positions(to_tensor(x, FP32), None, ints(at if len(sections) > 1 else at[0]), 1e-20, sections, per_axis)
+    assert e.value.status == _lib.IT_ERR_INVALID_ARG
+
+
 def test_rope_inverse_is_the_gradient(it_ctx):
     """Against differences: the rotation is linear, so with L = sum(g * rope(x)), dL/dx . d = L(x + d) - L(x) but for rounding."""
     rng = np.random.default_rng(21)

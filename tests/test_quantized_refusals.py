@@ -183,3 +183,19 @@ def with_lse(o, *shape):
 def test_sizes_that_32_bits_would_cut_off_are_refused(call):
     with pytest.raises(AssertionError, match="below 2\\^31"):
         call()
+
+
+# ------------------------------------------------------------------------------------------------ bases below 1
+@pytest.mark.parametrize("base,D,sections,per_axis,refused", [
+    (1e-20, 128, [64], 0, True), (1e-3, 128, [64], 0, True), (5.5e-3, 4, [2], 0, False), (1e-7, 4, [2], 0, True), (1e-38, 2, [1], 0, False),
+    (1e-3, 128, [32, 30, 2], 1, True), (1e-20, 12, [1, 5], 1, True), (1e-20, 6, [1, 1, 1], 1, False), (2e-3, 128, [64], 0, False), (0.0, 8, [4], 0, True),
+])
+def test_bases_whose_frequencies_leave_the_reduction_are_refused(base, D, sections, per_axis, refused):
+    """By the entry itself, with a context that it must not look at (or, with nothing to rotate, need not)."""
+    lib, nothing = _lib.load(), ctypes.create_string_buffer(4096)
+    tokens = 1 if refused else 0
+    rc = lib.it_rope_positions(nothing, nothing, _lib.IT_F32, tokens, 1, 1, 0, D, base, len(sections), (ctypes.c_int32 * len(sections))(*sections), per_axis, 0,
+                               nothing, nothing, None, nothing, None)
+    assert rc == (_lib.IT_ERR_INVALID_ARG if refused else _lib.IT_OK)
+    if refused:
+        assert b"base" in lib.it_last_error()
