@@ -66,7 +66,7 @@ it_status it_stream_create(it_ctx* ctx, it_stream** out);
 it_status it_stream_wrap(it_ctx* ctx, void* cuda_stream, it_stream** out);
 it_status it_stream_destroy(it_ctx* ctx, it_stream* stream);
 /* CommandBatch::sync / ::end (src/command_batch.rs:191-226): block until the queue drains.  Returns
- * IT_ERR_TIMEOUT (without clearing anything) when the device status word is set, see
+ * IT_ERR_TIMEOUT or IT_ERR_INVALID_ARG (without clearing anything) when a device status word is set, see
  * it_attention_status_poll; so does it_event_wait. */
 it_status it_stream_sync(it_ctx* ctx, it_stream* stream);
 
@@ -284,19 +284,19 @@ it_status it_rope_positions(it_ctx* ctx, it_stream* stream, it_dtype dtype, int3
  *   scales [batch, kv_heads, max_len, groups] bf16
  * for keys and for values each; 4.5 bits a value where head_dim is a multiple of 32.  32 columns whose largest magnitude is below
  * 2^-100 are zeros, one above 7 * 2^122 saturates, and with a NaN or an infinity among them all 32 read back as NaN.
- * head_dim a multiple of 8 up to 128.  A length below 0 or above max_len is taken as the nearest that is not, no memory outside the
- * cache is touched, and the context reports it (IT_ERR_INVALID_ARG from it_stream_sync and the like, until it_attention_status_poll);
- * other sequences and later launches are not affected. */
+ * head_dim a multiple of 8 up to 128.  A length below 0 or above max_len is taken as the nearest that is not (by attention), no memory outside
+ * the cache is touched, and the context reports it (IT_ERR_INVALID_ARG from it_stream_sync and the like, until it_attention_status_poll);
+ * other sequences and later launches are not affected, but every stream's synchronisation reports it until then. */
 
 /* k, v [batch, tokens, kv_heads, head_dim] into the cache behind the lengths[b] positions of each sequence: of sequence b its first
  * counts[b] tokens (null: all).  new_lengths[b] = what is there afterwards; it must not be `lengths`.  Nothing else of the cache is
- * written.  A token that does not fit is dropped and reported as above. */
+ * written.  A token that does not fit, in front of position 0 or behind the last, is dropped and reported as above. */
 it_status it_kv_cache_q4_append(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t batch, int32_t tokens, int32_t kv_heads,
                                 int32_t head_dim, int32_t max_len, const void* k, const void* v, const int32_t* lengths,
                                 const int32_t* counts, int32_t* new_lengths, void* k_codes, void* k_scales, void* v_codes,
                                 void* v_scales);
 /* Positions starts[b] .. starts[b] + tokens - 1 (starts null: from 0) out of the cache as k, v [batch, tokens, kv_heads,
- * head_dim]; zeros where a position is negative or not below lengths[b] (null: max_len). */
+ * head_dim]; zeros where a position is negative or not below lengths[b] (null: max_len), of which none is reported. */
 it_status it_kv_cache_q4_read(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t batch, int32_t tokens, int32_t kv_heads,
                               int32_t head_dim, int32_t max_len, const void* k_codes, const void* k_scales, const void* v_codes,
                               const void* v_scales, const int32_t* starts, const int32_t* lengths, void* k, void* v);
@@ -377,10 +377,14 @@ it_status it_flash_attention_bwd_noalloc(it_ctx* ctx, it_stream* stream, it_dtyp
  * and it_stream_sync, it_event_wait and it_ctx_check_status report IT_ERR_TIMEOUT.
  * it_attention_status_poll drains `stream`, returns the word in *device_status (0 = clean) and CLEARS it,
  * after which launches compute again.  Returns IT_ERR_TIMEOUT when the word was non-zero.
+ * A second word says that a sequence's length lay outside its quantised cache.  It stops no launch and spoils no result but that
+ * sequence's, and the same calls report it, as IT_ERR_INVALID_ARG.  It is the context's, so every thread and stream that
+ * synchronises sees it, again and again, until a poll clears it; the new_lengths of it_kv_cache_q4_append tell which
+ * sequence had no room.  A poll reports and clears one word, the wait's first: where both are set, the next poll reports the other.
  * (The reference never checks command-buffer errors; src/command_batch.rs:191-226.) */
 it_status it_attention_status_poll(it_ctx* ctx, it_stream* stream, int32_t* device_status);
 /* Reads the status word without draining a caller's stream and without clearing it: IT_OK when zero,
- * IT_ERR_TIMEOUT otherwise; *device_status (may be null) gets the word.  For hosts that synchronise by
+ * IT_ERR_TIMEOUT or IT_ERR_INVALID_ARG otherwise; *device_status (may be null) gets the word.  For hosts that synchronise by
  * other means (their own events, a blocking copy) before they read results. */
 it_status it_ctx_check_status(it_ctx* ctx, int32_t* device_status);
 

@@ -124,7 +124,9 @@ struct CommandBatch {
     check(it_event_wait(Context::global().raw(), pending()));
     recorded() = false;
   }
-  // Raises it::Error(IT_ERR_TIMEOUT) if a kernel's bounded wait ran out since the last poll.
+  // Raises it::Error(IT_ERR_TIMEOUT) if a kernel's bounded wait ran out since the last poll, and IT_ERR_INVALID_ARG if a sequence's
+  // length lay outside its quantised cache (results are valid then); clears what it reports.  sync and wait_for_completion
+  // raise the same and clear nothing.
   static void poll_device_status() {
     int32_t st = 0;
     check(it_attention_status_poll(Context::global().raw(), Context::global().stream(), &st));

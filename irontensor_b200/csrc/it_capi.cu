@@ -132,12 +132,15 @@ struct it_host_step {
 namespace {
 
 // Copies the device status words to the host on the context's own stream.  Called after a caller's
-// stream or event has been waited for, so every kernel that could have written them is done.  *out: the first that is set.
-it_status read_device_status(it_ctx* ctx, int* out) {
+// stream or event has been waited for, so every kernel that could have written them is done.  *out: the first that is set;
+// *which: its place.
+it_status read_device_status(it_ctx* ctx, int* out, int* which = nullptr) {
   std::lock_guard<std::mutex> lock(ctx->status_mutex);
   IT_CUDA(cudaMemcpyAsync(ctx->h_status, ctx->d_status, 2 * sizeof(int), cudaMemcpyDeviceToHost, ctx->status_stream));
   IT_CUDA(cudaStreamSynchronize(ctx->status_stream));
-  *out = ctx->h_status[0] != 0 ? ctx->h_status[0] : ctx->h_status[1];
+  const int first = ctx->h_status[0] != 0 ? 0 : 1;
+  *out = ctx->h_status[first];
+  if (which != nullptr) *which = first;
   return IT_OK;
 }
 
@@ -1771,12 +1774,12 @@ it_status it_attention_status_poll(it_ctx* ctx, it_stream* stream, int32_t* devi
   if (ctx == nullptr || stream == nullptr || device_status == nullptr)
     return fail(IT_ERR_INVALID_ARG, "null argument");
   IT_CUDA(cudaStreamSynchronize(stream->s));
-  int word = 0;
-  it_status rc = read_device_status(ctx, &word);
+  int word = 0, which = 0;
+  it_status rc = read_device_status(ctx, &word, &which);
   if (rc != IT_OK) return rc;
   *device_status = word;
   if (*device_status != 0) {
-    IT_CUDA(cudaMemsetAsync(ctx->d_status, 0, 2 * sizeof(int), stream->s));
+    IT_CUDA(cudaMemsetAsync(ctx->d_status + which, 0, sizeof(int), stream->s));   // the other one is the next call's to report
     IT_CUDA(cudaStreamSynchronize(stream->s));
     return device_status_error(*device_status, false);
   }

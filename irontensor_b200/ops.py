@@ -91,12 +91,14 @@ class _Context:
 
     def check_status(self):
         """Raises ITError(IT_ERR_TIMEOUT) if a kernel's bounded wait ran out on this context (every later launch
-        is then a no-op and its outputs are garbage).  Does not drain a stream and does not clear the word;
-        call it after the results have been waited for.  poll_status() clears."""
+        is then a no-op and its outputs are garbage), and ITError(IT_ERR_INVALID_ARG) if a sequence's length lay outside its
+        QuantizedCache (later launches compute, and results are valid but for that sequence's).  Does not drain a stream and does
+        not clear the word; call it after the results have been waited for.  poll_status() clears."""
         _lib.check(self.lib.it_ctx_check_status(self.handle, None))
 
     def poll_status(self):
-        """Drains the current stream; raises ITError(IT_ERR_TIMEOUT) if a kernel's wait ran out."""
+        """Drains the current stream; raises what check_status() does, and clears what it raises.  Where both have happened, the
+        next call raises the other."""
         st = ctypes.c_int32()
         rc = self.lib.it_attention_status_poll(self.handle, self.stream(), ctypes.byref(st))
         _lib.check(rc)
@@ -119,7 +121,9 @@ class CommandBatch:
     """The reference batches encoded work per thread and flushes on sync (src/command_batch.rs:167-391).
     Here work is enqueued on the thread's current CUDA stream as soon as an op is called; these
     functions keep the same call sites meaningful.  sync, end and wait_for_completion raise ITError(IT_ERR_TIMEOUT)
-    when a kernel's bounded wait ran out (it_stream_sync / it_event_wait report the device status word)."""
+    when a kernel's bounded wait ran out (it_stream_sync / it_event_wait report the device status words), and
+    ITError(IT_ERR_INVALID_ARG) when a sequence's length lay outside its QuantizedCache: on every thread and stream of the device,
+    until context().poll_status() clears it, although results are valid then."""
 
     @staticmethod
     def begin():
@@ -864,8 +868,10 @@ def kv_cache_append(cache, k, v, lengths, counts=None):
     (prompts padded to one length).  Returns the new lengths, an int32 tensor [batch].
 
     lengths and counts are int32 tensors [batch] on the device and read there, so that the call can be captured in a CUDA graph.  A
-    token that does not fit into max_len positions is dropped and reported when the stream is next synchronised (ITError); other
-    sequences and later calls are not affected."""
+    token that does not fit into max_len positions is dropped (in front of position 0 or behind the last) and reported: whatever
+    synchronises with the device next, on any thread or stream, and whatever copies a tensor to the host, raises
+    ITError(IT_ERR_INVALID_ARG), until context().poll_status() clears it.  Results of other sequences and later calls are not
+    affected; the new length of a sequence that had no room is below lengths[b] and its tokens."""
     new = _host_ops.kv_cache_append(cache, k, v, lengths, counts)
     if new is not None:
         return new

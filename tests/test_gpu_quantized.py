@@ -204,6 +204,30 @@ def test_a_full_cache_stops_nothing_else(it_ctx):
     assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+def test_a_full_cache_and_a_wait_that_ran_out_are_both_reported(it_ctx):
+    """One poll each, the wait (20 ms on a barrier nothing arrives on) first; until then every synchronisation reports one of them."""
+    import ctypes
+    import torch
+    from irontensor_b200 import CommandBatch
+    k, cache = Tensor.zeros([1, 2, 1, 32], BF16), QuantizedCache.zeros(1, 3, 1, 32)
+    assert kv_cache_append(cache, k, k, ints([2])).tolist() == [3]
+    torch.cuda.synchronize()
+    with pytest.raises(_lib.ITError, match="length lay outside") as e:    # of another stream
+        with torch.cuda.stream(torch.cuda.Stream()):
+            CommandBatch.sync()
+    assert e.value.status == _lib.IT_ERR_INVALID_ARG
+    _lib.check(it_ctx.lib.it_selftest_wait_timeout(it_ctx.handle, it_ctx.stream(), 20))
+    with pytest.raises(_lib.ITError, match="ran out"):
+        CommandBatch.sync()
+    for text, word in (("ran out", 6), ("length lay outside", 7)):
+        st = ctypes.c_int32()
+        with pytest.raises(_lib.ITError, match=text):
+            _lib.check(it_ctx.lib.it_attention_status_poll(it_ctx.handle, it_ctx.stream(), ctypes.byref(st)))
+        assert st.value == word
+    assert it_ctx.poll_status() == 0
+    CommandBatch.sync()
+
+
 @pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("B,L,Hkv,D,count,starts,lengths", [
     (1, 1, 1, 8, 1, None, None), (2, 9, 3, 64, 9, None, None), (3, 17, 2, 80, 5, [0, 12, 16], None), (2, 9, 1, 128, 12, [-2, 5], [9, 7]),
