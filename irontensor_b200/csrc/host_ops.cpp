@@ -715,7 +715,7 @@ PyObject* linear_int8_forward(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   return guard([&]() -> PyObject* {
     if (!packed(a[0], at::kChar) || !packed(a[1], at::kFloat) || !packed(a[2], at::kChar) || !packed(a[3], at::kFloat)) Py_RETURN_NONE;
     const at::Tensor &x = THPVariable_Unpack(a[0]), &sx = THPVariable_Unpack(a[1]), &wt = THPVariable_Unpack(a[2]), &sw = THPVariable_Unpack(a[3]);
-    if (x.dim() != 2 || wt.dim() != 2 || x.size(1) != wt.size(1) || sx.numel() != x.size(0) || sw.numel() != wt.size(0) || x.numel() == 0 ||
+    if (x.dim() != 2 || wt.dim() != 2 || x.size(1) != wt.size(1) || sx.dim() != 1 || sw.dim() != 1 || sx.size(0) != x.size(0) || sw.size(0) != wt.size(0) || x.numel() == 0 ||
         wt.numel() == 0 || (a[4] != g_fp32 && a[4] != g_bf16))
       Py_RETURN_NONE;
     const int64_t n = x.size(0), in = x.size(1), out = wt.size(0);

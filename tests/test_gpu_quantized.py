@@ -643,6 +643,17 @@ def test_refusals_on_the_device(it_ctx):
         rope_positions(to_tensor(np.zeros((1, 1, 1, 8)), FP32), None, ints([[0]]), base=-1.0)
 
 
+def test_scales_set_anew_have_one_dimension(it_ctx):
+    x, w = (quantize_rows(to_tensor(np.ones((n, 16)), BF16)) for n in (2, 8))
+    for rows in (x, w):
+        good, rows.scales = rows.scales, rows.scales[:, None]
+        with pytest.raises(AssertionError, match="scales must be float32"):
+            linear_int8_forward(x, w)
+        rows.scales = good
+    y = linear_int8_forward(x, w, FP32).to_f32_host()
+    assert np.all(y == np.float32(127 * 127 * 16 * float(x.scales[0]) * float(w.scales[0])))   # 18 and 16 bits: rounded once
+
+
 def test_empty_calls(it_ctx):
     import torch
     z = lambda *s: Tensor.zeros(list(s), BF16)
