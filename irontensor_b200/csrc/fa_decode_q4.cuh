@@ -167,15 +167,14 @@ struct DecodeQ4Warp {
   static constexpr float RANGE = 8.f;   // in the exp2 domain
   float m[R][2], limit[R][2], l[R][2];
   // fp32 q: K's values are made in bf16 like V's, and q has three bf16 terms.  bf16 q: K's codes alone are the operand, in fp16,
-  // whose ten bits of mantissa take two nibbles by a mask each: u in the lowest is 1024 + u, less 1032 by an addition; u in the next
-  // is 64 + u, and the 72 times the sum of q that this is too much is what the sums begin with.  A shift by 8 brings the other two.
-  // So a word costs five instructions of the unit that this kernel waits for and not eight; its scale is applied to the sums of its
-  // 32 columns in fp32.  q is scaled by a power of two to a largest magnitude in 1 .. 2 for this (fp16 rounds what is below 2^-14
+  // whose ten bits of mantissa take two nibbles by a mask each: u in the lowest is 1024 + u and u in the next is 64 + u, less 1032 and
+  // 72 by an addition, both exact.  A shift by 8 brings the other two.  (Adding 72 times the sum of q to the sums instead would save
+  // half of the additions, and leave in a score 2^-24 of that, whatever small codes the score is made of.)
+  // So a word costs five instructions of the integer unit and not eight; its scale is applied to the sums of its 32 columns in fp32.  q is scaled by a power of two to a largest magnitude in 1 .. 2 for this (fp16 rounds what is below 2^-14
   // of the largest, by at most 2^-25 of it).
   static constexpr bool F16 = TERMS == 1;
   uint32_t magic, magic0, magic1;
   uint32_t qb[TERMS][R][4 * NG];    // register 4 j + r: columns 32 j + 8 t + 2 r and the next of head g
-  float init[R][NG][2];             // what the sums of group j begin with, heads 2t and 2t + 1
   float scale[R][2];                // of the scores of these heads, in the exp2 domain
 
   __device__ __forceinline__ void begin() {
@@ -219,18 +218,12 @@ struct DecodeQ4Warp {
         const float down = as_is ? 1.f : __uint_as_float((254u - min(field, 253u)) << 23), up = as_is ? 1.f : __uint_as_float(min(field, 253u) << 23);
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
-          float sum = 0.f;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             uint32_t& x = qb[0][h][4 * j + r];
             const __half2 y = __floats2half2_rn(__uint_as_float(x << 16) * down, __uint_as_float(x & 0xFFFF0000u) * down);
             x = *reinterpret_cast<const uint32_t*>(&y);
-            if (r & 1) sum += __low2float(y) + __high2float(y);   // the nibbles that come as 64 + u
           }
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) init[h][j][e] = -72.f * __shfl_sync(0xffffffffu, sum, 8 * t + 4 * e);
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) scale[h][e] = scale_log2 * __shfl_sync(0xffffffffu, up, 8 * t + 4 * e);
@@ -296,17 +289,17 @@ struct DecodeQ4Warp {
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
         if constexpr (F16) {
-          constexpr uint32_t LESS = 0xE408E408u;   // -1032 in fp16
+          constexpr uint32_t LESS = 0xE408E408u, LESS1 = 0xD480D480u;   // -1032 and -72 in fp16
           const uint32_t u0 = w[0][j] >> 8, u1 = w[1][j] >> 8;
           const uint32_t a0 = q4_add2_f16(q4_and_or<0x000F000Fu>(w[0][j], magic0), LESS), a1 = q4_add2_f16(q4_and_or<0x000F000Fu>(w[1][j], magic0), LESS);
-          const uint32_t a2 = q4_and_or<0x00F000F0u>(w[0][j], magic1), a3 = q4_and_or<0x00F000F0u>(w[1][j], magic1);
+          const uint32_t a2 = q4_add2_f16(q4_and_or<0x00F000F0u>(w[0][j], magic1), LESS1), a3 = q4_add2_f16(q4_and_or<0x00F000F0u>(w[1][j], magic1), LESS1);
           const uint32_t a4 = q4_add2_f16(q4_and_or<0x000F000Fu>(u0, magic0), LESS), a5 = q4_add2_f16(q4_and_or<0x000F000Fu>(u1, magic0), LESS);
-          const uint32_t a6 = q4_and_or<0x00F000F0u>(u0, magic1), a7 = q4_and_or<0x00F000F0u>(u1, magic1);
+          const uint32_t a6 = q4_add2_f16(q4_and_or<0x00F000F0u>(u0, magic1), LESS1), a7 = q4_add2_f16(q4_and_or<0x00F000F0u>(u1, magic1), LESS1);
           const float f0 = __uint_as_float(sc[0][j] << 16), f1 = __uint_as_float(sc[1][j] << 16);
 #pragma unroll
           for (int h = 0; h < R; ++h) {
             float d[4];
-            mma_f16_16816(d, a0, a1, a2, a3, qb[0][h][4 * j], qb[0][h][4 * j + 1], init[h][j][0], init[h][j][1], init[h][j][0], init[h][j][1]);
+            mma_f16_16816(d, a0, a1, a2, a3, qb[0][h][4 * j], qb[0][h][4 * j + 1], 0.f, 0.f, 0.f, 0.f);
             mma_f16_16816(d, a4, a5, a6, a7, qb[0][h][4 * j + 2], qb[0][h][4 * j + 3], d[0], d[1], d[2], d[3]);
             s[i][h][0] = fmaf(f0, d[0], s[i][h][0]);
             s[i][h][1] = fmaf(f0, d[1], s[i][h][1]);

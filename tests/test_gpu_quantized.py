@@ -390,6 +390,32 @@ def test_decode_of_scales_far_apart(it_ctx, precision):
     check_decode(it_ctx, precision, q, k, v, lengths, 256)
 
 
+@pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("H,Hkv,D,L,max_len", [(8, 2, 128, 300, 300), (8, 1, 64, 100, 128), (16, 1, 96, 77, 100), (4, 4, 40, 65, 1 << 18), (6, 1, 128, 200, 1 << 18)])
+def test_decode_of_keys_with_one_large_channel(it_ctx, precision, H, Hkv, D, L, max_len):
+    """Every group of 32 columns has one value some hundred times the others, whose codes are then 0, in a column where q is small; the
+    rest of q is large and of one sign.  A score is as good as the few products that it is a sum of, whatever the sum of q: off by
+    E = 2^-20 of the products' magnitudes at most (as check_decode has it), a p by 2 E of itself, and so the result by 2 E A
+    beside what check_decode counts."""
+    rng = np.random.default_rng(62)
+    q = np.abs(values(rng, (1, H, D), precision)) + 1
+    q[..., ::4] *= 2.0 ** -9
+    q = q if precision is FP32 else synth.round_bf16(q.astype(np.float32)).reshape(q.shape)
+    k, v = values(rng, (1, L, Hkv, D), FP32), values(rng, (1, L, Hkv, D), FP32)
+    for j in range(0, D, 32):
+        at = j + 4 * rng.integers(0, min(32, D - j) // 4, (L, Hkv))
+        k[0, np.arange(L)[:, None], np.arange(Hkv), at] = 1000.0 + 10 * rng.standard_normal((L, Hkv))
+    o = attention_decode_quantized(to_tensor(q, precision), cache_of(k, v, max_len), ints([L]))
+    assert it_ctx.poll_status() == 0
+    hk, hv = qr.q4_values(k), qr.q4_values(v)
+    want, lse = qr.decode(q, hk, hv, [L])
+    products = np.einsum("hd,lhd->hl", np.abs(q[0]).astype(np.float64), np.repeat(np.abs(hk[0]), H // Hkv, 1)).max(1) / math.sqrt(D)
+    E, A = 2.0 ** -20 * products[None, :], np.abs(hv).max()
+    assert np.all(np.abs(o.lse.to_f32_host() - lse) <= E + 2.0 ** -15 + 2.0 ** -23 * np.abs(lse)), np.abs(o.lse.to_f32_host() - lse).max()
+    limit = (2 * E[..., None] + 2.0 ** -15) * A + (2.0 ** -8 if precision is BF16 else 2.0 ** -24) * np.abs(want)
+    assert np.all(np.abs(o.to_f32_host() - want) <= limit)
+
+
 def test_decode_with_one_overwhelming_key(it_ctx):
     """The maximum arrives late and dwarfs what was summed before it: the result is that key's value alone."""
     rng = np.random.default_rng(12)
