@@ -531,12 +531,22 @@ struct QuantizedCache {
   uint8_t* v_codes() const { return codes.ptr() + codes.size() / 2; }
   uint16_t* k_scales() const { return scales.ptr(); }
   uint16_t* v_scales() const { return scales.ptr() + scales.size() / 2; }
+  // The members may have been set one by one: the calls below refuse sizes that the buffers do not have.
+  void check_form() const {
+    require(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0, "head_dim must be a multiple of 8 in 8..128");
+    require(kv_heads >= 1 && max_len >= 1, "kv_heads and max_len must be positive");
+    const size_t groups = (head_dim + 31) / 32;
+    const size_t heads = 2 * static_cast<size_t>(dim32(batch)) * dim32(kv_heads), len = dim32(max_len);
+    const bool fits = heads == 0 || len <= scales.size() / heads;   // else the products below might not fit into 64 bits
+    require(fits && scales.size() == heads * len * groups && codes.size() == heads * len * 16 * groups, "codes and scales must be of the cache's sizes");
+  }
 };
 
 // New tokens k, v [batch, tokens, kv_heads, head_dim] behind the first lengths[b] positions (of sequence b the first counts[b], null:
 // all); returns the new lengths.
 inline Array<int32_t> kv_cache_append(const QuantizedCache& c, const Tensor& k, const Tensor& v, const Array<int32_t>& lengths,
                                       const Array<int32_t>* counts = nullptr) {
+  c.check_form();
   require(k.shape() == v.shape() && k.precision() == v.precision(), "k and v must have the same shape and precision");
   require(k.shape().size() == 4 && k.shape()[0] == c.batch && k.shape()[2] == c.kv_heads && k.shape()[3] == c.head_dim,
           "k and v must be [batch, tokens, kv_heads, head_dim] of the cache");
@@ -552,6 +562,7 @@ inline Array<int32_t> kv_cache_append(const QuantizedCache& c, const Tensor& k, 
 // (null: max_len).
 inline std::pair<Tensor, Tensor> kv_cache_read(const QuantizedCache& c, size_t tokens, const Array<int32_t>* starts = nullptr,
                                                const Array<int32_t>* lengths = nullptr, Precision p = Precision::BF16) {
+  c.check_form();
   require((starts == nullptr || starts->size() == c.batch) && (lengths == nullptr || lengths->size() == c.batch),
           "starts and lengths must have one number a sequence");
   Tensor k = Tensor::empty({c.batch, tokens, c.kv_heads, c.head_dim}, p), v = Tensor::empty({c.batch, tokens, c.kv_heads, c.head_dim}, p);
@@ -563,6 +574,7 @@ inline std::pair<Tensor, Tensor> kv_cache_read(const QuantizedCache& c, size_t t
 
 // attention_decode against a QuantizedCache, each sequence at its own length (the new token's position included).
 inline Tensor attention_decode_quantized(const Tensor& q, const QuantizedCache& c, const Array<int32_t>& lengths) {
+  c.check_form();
   require(q.shape().size() == 3 && q.shape()[0] == c.batch && q.shape()[2] == c.head_dim, "q must be [batch, heads, head_dim] of the cache");
   require(q.shape()[1] % c.kv_heads == 0, "num_heads must be divisible by num_kv_heads");
   require(lengths.size() == c.batch, "lengths must have one number a sequence");
@@ -583,6 +595,9 @@ struct QuantizedRows {
   size_t rows = 0, cols = 0;
   Array<int8_t> codes;
   Array<float> scales;
+  void check_form() const {
+    require(static_cast<size_t>(dim32(rows)) * static_cast<size_t>(dim32(cols)) == codes.size() && scales.size() == rows, "codes and scales must be of the rows' sizes");
+  }
 };
 
 inline QuantizedRows quantize_rows(const Tensor& x) {
@@ -597,6 +612,8 @@ inline QuantizedRows quantize_rows(const Tensor& x) {
 // output = input @ weight.T in column ranges of these widths, which add up to out (q, k and v from stacked weights).
 inline std::vector<Tensor> linear_int8_forward(const QuantizedRows& input, const QuantizedRows& weight, const std::vector<size_t>& widths,
                                                Precision p = Precision::BF16) {
+  input.check_form();
+  weight.check_form();
   require(input.cols == weight.cols, "inner dimensions must match");
   require(!widths.empty() && widths.size() <= 3, "up to three widths");
   std::vector<Tensor> out;
