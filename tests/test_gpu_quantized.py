@@ -375,6 +375,44 @@ def test_decode_of_many_sequences_in_even_shares(it_ctx):
     check_decode(it_ctx, BF16, q, k, v, np.zeros(B, int), 2048)
 
 
+def launches_of(it_ctx, call):
+    """2 for even shares (the attention and its merge), 1 for clusters."""
+    before = it_ctx.launch_count()
+    call()
+    return it_ctx.launch_count() - before
+
+
+@pytest.mark.parametrize("B", [127, 128, 129, 255, 256, 257, 600])
+@pytest.mark.parametrize("precision,H,Hkv,D", [(BF16, 2, 1, 32), (BF16, 16, 2, 32), (BF16, 16, 1, 128), (FP32, 2, 1, 128), (FP32, 8, 1, 104)])
+def test_even_shares_of_more_sequences_than_a_cta_has_threads(it_ctx, precision, H, Hkv, D, B):
+    """The work in front of each sequence is added up 128 or 256 sequences at a time, in two passes: with empty sequences on both sides of
+    every border, with only the last one not empty, and with nothing but empty ones."""
+    rng = np.random.default_rng(B + D)
+    lengths = rng.integers(0, 100, B)
+    for border in (128, 256, 512):
+        lengths[border - 2:border + 1] = 0
+    lengths[[1, B - 1]] = [99, 33]
+    q = values(rng, (B, H, D), precision)
+    k, v = values(rng, (B, 99, Hkv, D), FP32), values(rng, (B, 99, Hkv, D), FP32)
+    for n in (lengths, lengths * (np.arange(B) == B - 1), np.zeros(B, int)):
+        assert launches_of(it_ctx, lambda: check_decode(it_ctx, precision, q, k, v, n, 1 << 15)) == 2
+
+
+@pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("B,H,Hkv,D,max_len", [
+    (5, 8, 2, 128, 1 << 17), (3, 12, 1, 64, 1 << 18), (2, 4, 4, 32, 1 << 17), (3, 6, 2, 96, 1 << 17), (2, 32, 2, 80, 1 << 17), (1, 5, 1, 16, 1 << 19),
+    (2, 2, 2, 48, 1 << 18), (4, 3, 3, 32, 1 << 17), (4, 3, 1, 64, 1 << 17), (4, 8, 1, 72, 1 << 17), (4, 32, 2, 128, 1 << 17), (4, 17, 1, 96, 1 << 17),
+    (2, 8, 2, 64, 1 << 17), (1, 6, 1, 128, 1 << 18), (4, 4, 4, 40, 1 << 18),
+])
+def test_caches_with_that_much_room_are_attended_to_in_even_shares(it_ctx, precision, B, H, Hkv, D, max_len):
+    """The shapes by which the tests above and below mean to reach the persistent launch."""
+    cache, q = QuantizedCache.zeros(B, max_len, Hkv, D), Tensor.zeros([B, H, D], precision)
+    assert launches_of(it_ctx, lambda: attention_decode_quantized(q, cache, ints([1] * B))) == 2
+    small = QuantizedCache.zeros(B, 256, Hkv, D)
+    assert launches_of(it_ctx, lambda: attention_decode_quantized(q, small, ints([1] * B))) == 1
+    assert it_ctx.poll_status() == 0
+
+
 @pytest.mark.parametrize("precision", [BF16, FP32], ids=["bf16", "fp32"])
 def test_decode_of_scales_far_apart(it_ctx, precision):
     """Values over many powers of two: a scale is taken as it is, and a group of zeros stays zero."""
