@@ -283,7 +283,8 @@ it_status it_rope_positions(it_ctx* ctx, it_stream* stream, it_dtype dtype, int3
  *          t * groups + j holds columns 32 j + 8 t + e, e = 0..7, as c + 8 in the 4 bits from 4 * (e / 2) + 16 * (e % 2)
  *   scales [batch, kv_heads, max_len, groups] bf16
  * for keys and for values each; 4.5 bits a value where head_dim is a multiple of 32.  32 columns whose largest magnitude is below
- * 2^-100 are zeros, one above 7 * 2^122 saturates, and with a NaN or an infinity among them all 32 read back as NaN.
+ * 2^-100 are zeros, one above 7 * 2^122 saturates, and with a NaN or an infinity among them all 32 read back as NaN.  Scales that
+ * the caller writes must have 5 significant bits at most, too: with more, values are read back, and V is used, rounded.
  * head_dim a multiple of 8 up to 128.  A length below 0 or above max_len is taken as the nearest that is not (by attention), no memory outside
  * the cache is touched, and the context reports it (IT_ERR_INVALID_ARG from it_stream_sync and the like, until it_attention_status_poll);
  * other sequences and later launches are not affected, but every stream's synchronisation reports it until then. */
@@ -301,7 +302,8 @@ it_status it_kv_cache_q4_read(it_ctx* ctx, it_stream* stream, it_dtype dtype, in
                               int32_t head_dim, int32_t max_len, const void* k_codes, const void* k_scales, const void* v_codes,
                               const void* v_scales, const int32_t* starts, const int32_t* lengths, void* k, void* v);
 /* it_attention_decode over such a cache, sequence b over its first lengths[b] positions: q, o [batch, heads, head_dim], lse [batch,
- * heads] (may be null).  A sequence without positions gives zeros, and -inf in lse.  fp32 math; results repeat bit for bit. */
+ * heads] (may be null).  A sequence without positions gives zeros, and -inf in lse.  Sums in fp32 (which values near its range leave:
+ * a product of P and V may be 2^8 times V, and there are as many as positions); results repeat bit for bit. */
 it_status it_attention_decode_q4_workspace_bytes(int32_t batch, int32_t heads, int32_t head_dim, size_t* out_bytes);
 it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t batch, int32_t heads, int32_t kv_heads,
                                  int32_t head_dim, int32_t max_len, const void* q, const void* k_codes, const void* k_scales,
@@ -312,7 +314,7 @@ it_status it_attention_decode_q4(it_ctx* ctx, it_stream* stream, it_dtype dtype,
  * row's scale is (its largest magnitude / 127) rounded to 8 significant bits, a value is scale * c with c in -127..127 (rows below
  * 2^-100: zeros; with a NaN or an infinity: the scale is NaN).  Tokens are rows of activations, channels rows of weights.
  * it_linear_i8_fwd: y[i, o] = sum_k x_codes[i, k] w_codes[o, k] * (x_scales[i] * w_scales[o]) with exact 32-bit sums, on tcgen05
- * (kind::i8).  The columns of y go to n_outs (1 to 3) tensors [n, widths[r]] of the given type, side by side: one call for the
+ * (kind::i8); the product of two scales is one of fp32, and has to be in its range.  The columns of y go to n_outs (1 to 3) tensors [n, widths[r]] of the given type, side by side: one call for the
  * stacked weights [Wq; Wk; Wv].  in_dim a multiple of 16 up to 65536; out_dim = the sum of the widths, multiples of 8 each. */
 it_status it_quantize_rows_i8(it_ctx* ctx, it_stream* stream, it_dtype dtype, int32_t rows, int32_t cols, const void* x,
                               int8_t* codes, float* scales);

@@ -9,16 +9,20 @@
 //   O^T = V^T P^T A: 16 columns by 16 keys.  A register holds one column of two keys, so two keys' words are interleaved by
 //                 halves first (four byte permutes for 32 codes); B: P of 16 keys and 8 heads, S^T transposed in 8 x 8 tiles
 // with the codes as the larger operand, so that an instruction's 16 rows are all in use whatever the number of heads.
-// P goes in as two bf16 terms, 16 bits; an fp32 q as three terms, as does its P.  Where a K/V head has up to four query heads and q is
-// bf16, these are there twice among the instruction's eight columns, and P's terms are its columns 0-3 and 4-7: half the
-// instructions for O (PAIRED; B32 H32/8 D128 ragged to 8190: 51 -> 48.5 us when it came).
+// P goes in as two bf16 terms, 16 bits, which is 2^-17 of each p: of the bf16 results for B32 H32/8 D128 ragged to 8190, 0.2 % are not
+// the nearest to the exact value, where sums in plain fp32 leave 0.07 %, and both are 0.00166 away from it (the rounding to bf16 itself).
+// A third term would be half of V's matrix instructions again.  An fp32 q goes in as three terms, as does its P.  Where a K/V head has up
+// to four query heads and q is bf16, these are there twice among the instruction's eight columns, and P's terms are its columns 0-3
+// and 4-7: half the instructions for O (PAIRED; the same case: 51 -> 48.5 us when it came).
 // Which key is which row of S^T, and which column of V is which row of O^T, is free as long as both products agree: the order
 // is the one in which the words lie (q4_dim_of, q4_key_of).
 //
-// What has to be read is 144 bytes a position of a K/V head at head_dim 128; what bounds the work is the instructions that make operands
-// of them: 680 for the 32 keys that a warp takes at a time, 300 of them on the integer unit, beside which matrix instructions of this
-// kind hardly run (4 TB/s of the 6.5 of a copy).  tcgen05 would free that unit of nothing, since the operands are made all the same, and put
-// them through shared or tensor memory and a chain of waits for each tile: 75 us where this takes 46.5.  So
+// What has to be read is 144 bytes a position of a K/V head at head_dim 128: 23 us of the 47.7 that the case above takes, 3.2 TB/s
+// (sixteen sequences of 16000: 74.7 us, 3.9 TB/s).  No unit is full: over 32 sequences of 8192 the schedulers issue in 61 % of the
+// cycles, the integer unit is busy in 53 %, the matrix unit in 22 %, with 706 instructions for the 32 keys that a warp takes at a time.
+// A block of keys is one chain (codes, scores, vote, exponentials, transposes, values), a scheduler has fewer than three warps, and in
+// 40 % of the cycles none of them can go on; registers leave no room for a fourth.  tcgen05 makes the chain longer: the operands are
+// made all the same, and go through shared or tensor memory and a wait for each tile: 75 us where this took 46.5.  So
 //   * a warp has a ring of three stages of 32 keys in shared memory, filled by asynchronous copies that nobody but it waits for;
 //     no barrier until a CTA's warps merge what they found;
 //   * long caches: a persistent launch (PLAN_EVEN), in which every CTA takes the same number of 32-key units of the whole batch,
@@ -42,9 +46,9 @@ namespace it {
 
 constexpr int DQ_BLOCK = 32, DQ_STAGES = 3, DQ_MAX_CTAS = 512, DQ_START = 12;
 enum : int { PLAN_CLUSTER = 0, PLAN_EVEN = 1 };
-// Warps of a CTA and CTAs of an SM.  The persistent launches of bf16 have three CTAs of four warps: 168 registers a thread, which the loop
+// Warps of a CTA and CTAs of an SM.  The persistent launches of bf16 have three CTAs of four warps: up to 168 registers a thread, which the loop
 // needs more than it needs a fourth warp on each scheduler with 128 and some of them in memory (B32 H32/8 D128 ragged to 8190, where this
-// is 46.5 us: with eight warps twice 2.5 more, six warps twice 2), and few warps that wait for one another where a stretch ends.
+// was 46.5 us: with eight warps twice 2.5 more, six warps twice 2), and few warps that wait for one another where a stretch ends.
 __host__ __device__ constexpr bool dq_threes(int terms, int heads, int plan) { return plan == PLAN_EVEN && terms == 1 && heads == 8; }
 __host__ __device__ constexpr int dq_warps(int terms, int heads, int plan) { return dq_threes(terms, heads, plan) ? 4 : 8; }
 __host__ __device__ constexpr int dq_ctas(int terms, int heads, int plan) { return dq_threes(terms, heads, plan) ? 3 : terms == 1 && heads == 8 ? 2 : 1; }
@@ -167,7 +171,7 @@ struct DecodeQ4Warp {
   static constexpr float RANGE = 8.f;   // in the exp2 domain
   float m[R][2], limit[R][2], l[R][2];
   // fp32 q: K's values are made in bf16 like V's, and q has three bf16 terms.  bf16 q: K's codes alone are the operand, in fp16,
-  // whose ten bits of mantissa take two nibbles by a mask each: u in the lowest is 1024 + u and u in the next is 64 + u, less 1032 and
+  // whose ten bits of mantissa take two nibbles by a mask each, the known way of making numbers of them: u in the lowest is 1024 + u and u in the next is 64 + u, less 1032 and
   // 72 by an addition, both exact.  A shift by 8 brings the other two.  (Adding 72 times the sum of q to the sums instead would save
   // half of the additions, and leave in a score 2^-24 of that, whatever small codes the score is made of.)
   // So a word costs five instructions of the integer unit and not eight; its scale is applied to the sums of its 32 columns in fp32.  q is scaled by a power of two to a largest magnitude in 1 .. 2 for this (fp16 rounds what is below 2^-14
@@ -808,8 +812,9 @@ fa_decode_q4_merge_kernel(const DecodeQ4Params prm) {
   }
   if (c0 == c1) return;
   auto part_of = [&](int c) { return (2 * static_cast<size_t>(c) + (c == c0 ? 1 : 0)) * HEADS + h; };
-  // The warp's parts are loaded some at a time, the first of them along with the maxima (one sequence of 131000, 148 parts a pair: 24.6 ->
-  // 21.8 us in all; an even share of the work there is 10 us of it, the scan 0.8, a stretch's end 1.3, this kernel 2.5).
+  // The warp's parts are loaded some at a time, the first of them along with the maxima (one sequence of 131000 with two K/V heads, 148
+  // parts a pair then: 24.6 -> 21.8 us in all; an even share of the work there is 10 us of it, the scan 0.8, a stretch's end 1.3, this
+  // kernel 2.5).  28 for each of eight warps are the 222 parts that half of 444 CTAs may leave a pair.
   constexpr int AT_ONCE = JN == 1 ? 28 : 4;
   float v[AT_ONCE][JN];
   auto load = [&](int c) {

@@ -119,12 +119,15 @@ int clusters_at_once(Kernel kernel, int size, int threads, int smem_bytes, std::
 }
 
 // How 4-bit attention shares out its work (see fa_decode_q4.cuh): clusters of 1, 2, 4 or 8 CTAs a pair, or even shares.  The lengths are
-// on the device, so this goes by max_len.  In us, measured: a launch of clusters is 4.5, 0.3 for each doubling of the cluster and a
-// round of 256 keys 1.25 for a CTA that has an SM for itself, 2.2 for two on one, at head_dim 128 (B8 H32/8, 4000 positions: 16
-// in clusters of two or four, 23.4 alone; B1 H32/8, 16000, clusters of eight: 15; 1000 positions of B4 H16/4: 8.4, 7.1, 6.0 and
-// 6.6 with 1, 2, 4 and 8).  An even launch is 13.5 and its rounds (one sequence of 131000, H16/2: 22, in clusters 89; B32 H32/8
-// ragged to 8190: 46.5, in clusters 60, 52 and 56; 64 pairs of 4000: 20 and 16).  Batches are counted as three quarters full there,
-// because in clusters the longest sequence decides.
+// on the device, so this goes by max_len.  In us, for bf16 at head_dim 128, a fit: a launch of clusters is 4.5, 0.3 for each doubling
+// of the cluster and a round of 256 keys 1.25 for a CTA that has an SM for itself, 2.2 for two on one (in clusters of 1, 2, 4 and 8:
+// B8 H32/8, 4000 positions, 23.7, 15.7, 16.1 and 22.9; B1 H32/8, 16000: 77, 42.7, 24.5 and 15.4; B4 H16/4, 1000: 8.2, 7.0, 5.8 and 6.9).
+// An even launch is 13.5 and its rounds.  The 13.5 is the fit's intercept, over caches that are as full as they may be: launch, scan,
+// merge, and the least share, 16 units, which leaves most CTAs of a short launch without work (B1 H32/8, 4000 positions: 13.4, in
+// clusters 7.4); 100 positions in a cache of 131072 take 6.9.  (One sequence of 131000, H16/2: 22.4, in clusters of 8 90; B32 H32/8
+// ragged to 8190: 47.7, in clusters 69, 56, 55 and 77; 64 pairs of 4000: 20.4 and 15.7.)  Batches are counted as three quarters full
+// there, because in clusters the longest sequence decides.  What going by max_len costs: B4 H16/4 ragged to 1000 takes 5.6 in a cache of
+// 1024 positions and 12.9 in one of 131072, where clusters of 8 would take 6.6.
 template <typename AtOnce>
 void choose_decode_q4_plan(long long pairs, int B, int max_len, int sm_count, int per_sm, int groups, AtOnce&& at_once, int* n_splits, bool* even) {
   const double width = 0.35 + 0.65 * groups / 4, two = 2.2 * width, one = per_sm == 1 ? two : 1.25 * width;
@@ -186,7 +189,7 @@ it_status it_rope_positions(it_ctx* ctx, it_stream* stream, it_dtype dtype, int3
                    reinterpret_cast<uintptr_t>(k_out)) & pair_mask))
     return fail(IT_ERR_ALIGNMENT, "q and k must be aligned to a pair of elements");
   // as many tokens a CTA as have two sines per thread and eight chunks, as long as that leaves four CTAs per SM (2 x 4093 tokens of 16 + 4 heads
-  // of 128 in bf16: 13.4 us, 6.3 TB/s; 8 x 600 of 32 + 8: 16.1, 6.1 TB/s)
+  // of 128 in bf16, tensors that left L2: 14.8 us, 5.7 TB/s; 8 x 600 of 32 + 8: 16.7, 5.9 TB/s)
   const int token_chunks = (H + Hkv) * (chunks ? D * elem / 16 : half);
   const int n_pos = static_cast<int>(std::clamp<int64_t>(rows / (4LL * ctx->sm_count), 1, std::clamp(2048 / token_chunks, 1, 512 / half)));
   const int64_t ctas = (rows + n_pos - 1) / n_pos;
@@ -219,7 +222,7 @@ it_status it_kv_cache_q4_append(it_ctx* ctx, it_stream* stream, it_dtype dtype, 
   if ((st = cache_grid(B, T, Hkv, D, &grid, &at_once)) != IT_OK) return st;
   IT_CUDA(cudaSetDevice(ctx->device));
   // Two to three rounds of CTAs, each of which then goes on to other tokens: 8 x 2999 tokens of 8 heads of 128, all of them or padded to half,
-  // 23.8 and 14.9 us; with 8 CTAs an SM 26 and 15.3, with one for every 64 tokens 26 and 19.3.
+  // 23.8 and 14.9 us (in fp32 37.4 and 22.5); with 8 CTAs an SM 26 and 15.3, with one for every 64 tokens 26 and 19.3.
   grid.x = std::min<unsigned>(grid.x, std::max(1u, 12u * static_cast<unsigned>(ctx->sm_count) / (2 * grid.y)));
   auto launch = [&](auto kernel, auto* kk, auto* vv) -> it_status {
     IT_CUDA(launch_dependent(kernel, grid, 256, 0, stream->s, kk, vv, half_of(k_codes, k_scales), half_of(v_codes, v_scales), lengths, counts,

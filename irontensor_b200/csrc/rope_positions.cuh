@@ -76,8 +76,8 @@ __global__ void __launch_bounds__(256, 4)
 rope_positions_kernel(const ST* q_in, const ST* k_in, ST* q_out, ST* k_out, const int* __restrict__ positions, long long rows, int n_pos,
                       int H, int Hkv, int D, int inverse, const __grid_constant__ RopeAxes axes) {
   constexpr int U = 4;
-  // cosines and sines apart: a chunk's are a load of 16 bytes each, without bank conflicts (as pairs of both 17.4 -> 13.4 us where the comment
-  // below has its figures)
+  // cosines and sines apart: a chunk's are a load of 16 bytes each, without bank conflicts (as pairs of both 17.4 -> 13.4 us for 2 x 4093
+  // tokens of 16 + 4 heads of 128 in bf16 that L2 holds)
   __shared__ __align__(16) float cosines[512], sines[512];
   __shared__ double freq[64];
   __shared__ uint8_t axis[64];

@@ -816,7 +816,8 @@ class QuantizedCache:
     -7..7.  4.5 bits a value where head_dim is a multiple of 32; the form is described at it_kv_cache_q4_append.
 
     codes: uint8 [2, batch, kv_heads, max_len, 16 * groups] and scales: bfloat16 [2, batch, kv_heads, max_len, groups], keys first,
-    groups = ceil(head_dim / 32).  The object holds these two torch tensors and nothing else; how many positions of each sequence
+    groups = ceil(head_dim / 32).  Scales have 5 significant bits, and a cache that the caller fills keeps to that: with more, V and what
+    kv_cache_read returns are rounded, by up to 0.06 of a step.  The object holds these two torch tensors and nothing else; how many positions of each sequence
     are valid is the caller's, an int32 tensor [batch] on the device, as kv_len is for attention_decode."""
 
     __slots__ = ("codes", "scales", "head_dim")
