@@ -11,7 +11,7 @@
 // with the codes as the larger operand, so that an instruction's 16 rows are all in use whatever the number of heads.
 // P goes in as two bf16 terms, 16 bits, which is 2^-17 of each p: of the bf16 results for B32 H32/8 D128 ragged to 8190, 0.2 % are not
 // the nearest to the exact value, where sums in plain fp32 leave 0.07 %, and both are 0.00166 away from it (the rounding to bf16 itself).
-// A third term would be half of V's matrix instructions again.  An fp32 q goes in as three terms, as does its P.  Where a K/V head has up
+// A third term would be half of V's matrix instructions again, and with PAIRED columns as many.  An fp32 q goes in as three terms, as does its P.  Where a K/V head has up
 // to four query heads and q is bf16, these are there twice among the instruction's eight columns, and P's terms are its columns 0-3
 // and 4-7: half the instructions for O (PAIRED; the same case: 51 -> 48.5 us when it came).
 // Which key is which row of S^T, and which column of V is which row of O^T, is free as long as both products agree: the order
